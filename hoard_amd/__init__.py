@@ -14,10 +14,12 @@ HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libhoard_moe.so"
 
 TYPE_F32 = 0
+TYPE_F16 = 1
 TYPE_Q3_K = 11
 TYPE_Q4_K = 12
 TYPE_Q5_K = 13
 TYPE_Q6_K = 14
+TYPE_BF16 = 30
 BLOCK_BYTES = {TYPE_Q3_K: 110, TYPE_Q4_K: 144, TYPE_Q5_K: 176, TYPE_Q6_K: 210}
 
 OK = 0
@@ -94,6 +96,24 @@ class StoreStats(ctypes.Structure):
                [("direct", ctypes.c_int32), ("ram_experts", ctypes.c_int32)]
 
 
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
+
+
+class Q4Matrix(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("codes", "scales", "zeros")] + \
+               [(n, ctypes.c_int32) for n in ("rows", "cols", "group", "n_mat", "scale_type")]
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("type", "res_type", "gate_kind", "gate_sigmoid", "n_rows", "n")] + \
+               [(n, ctypes.c_float) for n in ("eps", "scale", "w_offset")] + \
+               [(n, ctypes.c_void_p) for n in ("r", "b", "gate", "w_post", "w_pre", "r_out", "h", "stats")]
+
+
+class NormGrads(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dr_out", "dh", "dr", "db", "dgate", "dw_post", "dw_pre")]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 # name -> (restype, argtypes); every symbol the public headers declare
@@ -140,6 +160,17 @@ ABI = {
     "hoard_slot_lru_create": (_I, [_I, _I, _I, _I, ctypes.POINTER(_P)]),
     "hoard_slot_lru_access": (_I, [_P, _I, _P, _I, _P, _P]),
     "hoard_slot_lru_destroy": (None, [_P]),
+    "hoard_q4_matmul": (_I, [_P, _P, _I, _I, _P, _P, _P]),
+    "hoard_q4_matmul_ids": (_I, [_P, _P, _I, _I, _P, _I, _P, _P, _P]),
+    "hoard_q4_matmul_sorted": (_I, [_P, _P, _I, _I, _P, _P, _P, _P]),
+    "hoard_sort_pairs": (_I, [_I, _I, _I, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "hoard_sort_workspace": (_I, [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
+    "hoard_sort_gather": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P]),
+    "hoard_sort_combine": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "hoard_sort_combine_grad": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
+    "hoard_norm_forward": (_I, [_P, _P]),
+    "hoard_norm_backward": (_I, [_P, _P, _P, ctypes.c_size_t, _P]),
+    "hoard_norm_workspace": (_I, [_P, ctypes.POINTER(ctypes.c_size_t)]),
     "hoard_synth_key": (ctypes.c_uint64, [ctypes.c_uint32] * 5),
     "hoard_synth_fill_blocks": (_I, [_I, ctypes.c_uint64, _P, ctypes.c_size_t, ctypes.c_float]),
     "hoard_synth_fill_normal": (None, [ctypes.c_uint64, _P, ctypes.c_size_t, ctypes.c_float]),

@@ -1,0 +1,234 @@
+// Pairs sorted by expert, their rows laid out and taken back (hoard_sort_*).
+//
+// The sort is a stable counting sort.  A block of kBlockPairs consecutive pairs
+// counts its experts; a pair's sorted row is the number of pairs of lower
+// experts, plus those of its own expert in earlier blocks, plus its rank among
+// its own block's.  The rank within a wave comes from ballots over the bits of
+// the expert id, the one across the block's waves from their counts in LDS.
+// Up to one block of pairs that is one launch; above it a launch of counts
+// comes first, and each block adds up what precedes it.
+#include "ops.h"
+#include "opsdev.h"
+
+namespace hoard {
+
+namespace {
+
+constexpr int kBlockPairs = 1024;
+constexpr int kMaxExperts = 1024;
+constexpr int kWaves = kBlockPairs / 64;
+
+// The lanes of the wave that hold the same key (of `bits` bits), as a mask.
+__device__ __forceinline__ uint64_t same_key(int key, int bits) {
+    uint64_t same = ~0ull;
+    for (int b = 0; b < bits; b++) {
+        const bool one = (key >> b) & 1;
+        const uint64_t ones = __ballot(one);
+        same &= one ? ones : ~ones;
+    }
+    return same;
+}
+
+// Pair p's expert; n_expert for a dropped pair and behind the last one.
+__device__ __forceinline__ int key_of(const PairsArgs &a, int64_t p, int64_t pairs) {
+    if (p >= pairs) return a.n_expert;
+    const int e = a.ids[p];
+    return e < 0 || e >= a.n_expert ? a.n_expert : e;
+}
+
+// counts[block][expert]
+__global__ __launch_bounds__(kBlockPairs) void count_kernel(PairsArgs a, int64_t pairs) {
+    __shared__ int cnt[kMaxExperts + 1];
+    for (int e = threadIdx.x; e <= a.n_expert; e += kBlockPairs) cnt[e] = 0;
+    __syncthreads();
+    atomicAdd(&cnt[key_of(a, (int64_t)blockIdx.x * kBlockPairs + threadIdx.x, pairs)], 1);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.n_expert; e += kBlockPairs) a.work[(size_t)blockIdx.x * a.n_expert + e] = cnt[e];
+}
+
+// blocks > 1: a.work holds every block's counts.
+__global__ __launch_bounds__(kBlockPairs) void place_kernel(PairsArgs a, int64_t pairs, int bits) {
+    __shared__ uint16_t of_wave[kWaves][kMaxExperts + 1];  // pairs of each expert in each wave, then before it
+    __shared__ int base[kMaxExperts + 1];                  // the block's first row of each expert
+    __shared__ int sums[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = a.n_expert, blocks = gridDim.x;
+    const int64_t p = (int64_t)blockIdx.x * kBlockPairs + tid;
+    const int key = key_of(a, p, pairs);
+    for (int i = tid; i < kWaves * (kMaxExperts + 1); i += kBlockPairs) (&of_wave[0][0])[i] = 0;
+    __syncthreads();
+    const uint64_t same = same_key(key, bits), before = same & ((1ull << lane) - 1ull);
+    const int rank = __popcll(before);
+    if (before == 0) of_wave[wave][key] = (uint16_t)__popcll(same);
+    __syncthreads();
+    // thread e: its expert's pairs over the waves, over the blocks before, over all
+    int mine = 0, earlier = 0, total = 0;
+    if (tid < E) {
+        for (int w = 0; w < kWaves; w++) {
+            const int c = of_wave[w][tid];
+            of_wave[w][tid] = (uint16_t)mine;
+            mine += c;
+        }
+        if (blocks == 1) {
+            total = mine;
+        } else {
+            for (int b = 0; b < blocks; b++) {
+                const int c = a.work[(size_t)b * E + tid];
+                if (b < (int)blockIdx.x) earlier += c;
+                total += c;
+            }
+        }
+    }
+    // exclusive sum of the totals over the experts
+    int incl = total;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int v = __shfl_up(incl, d);
+        if (lane >= d) incl += v;
+    }
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int first = incl - total, all = 0;
+    for (int w = 0; w < kWaves; w++) {
+        if (w < wave) first += sums[w];
+        all += sums[w];
+    }
+    if (tid < E) {
+        base[tid] = first + earlier;
+        if (blockIdx.x == 0) a.offsets[tid] = first;
+    }
+    if (blockIdx.x == 0 && tid == 0) a.offsets[E] = all;
+    __syncthreads();
+    if (p < pairs) {
+        int row = -1;
+        if (key < E) {
+            row = base[key] + of_wave[wave][key] + rank;
+            a.order[row] = (int)p;
+        }
+        a.place[p] = row;
+        if (p >= all) a.order[p] = -1;
+    }
+}
+
+// -- rows ---------------------------------------------------------------------
+
+// An item is 8 columns of a token; a wave's items are consecutive.
+__device__ __forceinline__ bool item_of(const RowsArgs &a, int64_t i, int per_row, int64_t &t, int &at, int &some) {
+    t = i / per_row;
+    at = (int)(i - t * per_row) * 8;
+    some = min(8, a.n - at);
+    return t < a.n_tokens;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void gather_kernel(RowsArgs a) {
+    const int per_row = (a.n + 7) / 8;
+    const int64_t pairs = (int64_t)a.n_tokens * a.k;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;; i += (int64_t)gridDim.x * 256) {
+        int64_t t;
+        int at, some;
+        if (!item_of(a, i, per_row, t, at, some)) return;
+        float x[8], o[8];
+        load_some(static_cast<const T *>(a.x) + t * a.n + at, some, x);
+        for (int j = 0; j < a.k; j++) {
+            const int row = a.place[t * a.k + j];
+            if (row < 0 || row >= pairs) continue;
+            const float w = a.w ? a.w[t * a.k + j] : 1.0f;
+#pragma unroll
+            for (int c = 0; c < 8; c++) o[c] = a.w ? w * x[c] : x[c];
+            store_some(static_cast<T *>(a.out) + (int64_t)row * a.n + at, some, o);
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(RowsArgs a) {
+    const int per_row = (a.n + 7) / 8;
+    const int64_t pairs = (int64_t)a.n_tokens * a.k;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;; i += (int64_t)gridDim.x * 256) {
+        int64_t t;
+        int at, some;
+        if (!item_of(a, i, per_row, t, at, some)) return;
+        float s[8] = {}, y[8];
+        if (a.res) load_some(static_cast<const T *>(a.res) + t * a.n + at, some, s);
+        for (int j = 0; j < a.k; j++) {
+            const int row = a.place[t * a.k + j];
+            if (row < 0 || row >= pairs) continue;
+            const float w = a.w ? a.w[t * a.k + j] : 1.0f;
+            load_some(static_cast<const T *>(a.x) + (int64_t)row * a.n + at, some, y);
+#pragma unroll
+            for (int c = 0; c < 8; c++) s[c] = fmaf(w, y[c], s[c]);
+        }
+        store_some(static_cast<T *>(a.out) + t * a.n + at, some, s);
+    }
+}
+
+// A wave takes a pair.
+template <typename T>
+__global__ __launch_bounds__(256) void combine_grad_kernel(RowsArgs a) {
+    const int64_t pairs = (int64_t)a.n_tokens * a.k;
+    const int lane = threadIdx.x & 63;
+    for (int64_t p = (int64_t)blockIdx.x * 4 + wave_index(); p < pairs; p += (int64_t)gridDim.x * 4) {
+        const int row = a.place[p];
+        float s = 0.0f;
+        if (row >= 0 && row < pairs) {
+            const int64_t t = p / a.k;
+            const float w = a.w[p];
+            for (int at = lane * 8; at < a.n; at += 512) {
+                const int some = min(8, a.n - at);
+                float d[8], y[8];
+                load_some(static_cast<const T *>(a.res) + t * a.n + at, some, d);
+                load_some(static_cast<const T *>(a.x) + (int64_t)row * a.n + at, some, y);
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    s = fmaf(d[c], y[c], s);
+                    d[c] *= w;
+                }
+                if (a.out) store_some(static_cast<T *>(a.out) + (int64_t)row * a.n + at, some, d);
+            }
+        }
+        s = wave_sum_f(s);
+        if (lane == 0) a.dw[p] = s;
+    }
+}
+
+int64_t rows_grid(const RowsArgs &a) {
+    const int64_t items = (int64_t)a.n_tokens * ((a.n + 7) / 8), groups = (items + 255) / 256;
+    return groups < (1 << 20) ? groups : (1 << 20);
+}
+
+#define HOARD_ROWS(KERNEL, GRID)                                                                       \
+    do {                                                                                               \
+        const unsigned grid = (unsigned)(GRID);                                                        \
+        if (a.type == HOARD_TYPE_F32) KERNEL<float><<<grid, 256, 0, s>>>(a);                           \
+        else if (a.type == HOARD_TYPE_F16) KERNEL<f16><<<grid, 256, 0, s>>>(a);                        \
+        else KERNEL<bf16><<<grid, 256, 0, s>>>(a);                                                     \
+        return hipGetLastError();                                                                      \
+    } while (0)
+
+}  // namespace
+
+size_t sort_work_bytes(int64_t pairs, int n_expert) {
+    return pairs <= kBlockPairs ? 0 : sizeof(int32_t) * (size_t)((pairs + kBlockPairs - 1) / kBlockPairs) * n_expert;
+}
+
+hipError_t launch_sort_pairs(const PairsArgs &a, hipStream_t s) {
+    const int64_t pairs = (int64_t)a.n_tokens * a.k;
+    const int blocks = pairs ? (int)((pairs + kBlockPairs - 1) / kBlockPairs) : 1;
+    int bits = 1;
+    while ((1 << bits) <= a.n_expert) bits++;  // keys 0..n_expert
+    if (blocks > 1) {
+        count_kernel<<<blocks, kBlockPairs, 0, s>>>(a, pairs);
+        const hipError_t rc = hipGetLastError();
+        if (rc != hipSuccess) return rc;
+    }
+    place_kernel<<<blocks, kBlockPairs, 0, s>>>(a, pairs, bits);
+    return hipGetLastError();
+}
+
+hipError_t launch_gather(const RowsArgs &a, hipStream_t s) { HOARD_ROWS(gather_kernel, rows_grid(a)); }
+hipError_t launch_combine(const RowsArgs &a, hipStream_t s) { HOARD_ROWS(combine_kernel, rows_grid(a)); }
+hipError_t launch_combine_grad(const RowsArgs &a, hipStream_t s) {
+    const int64_t groups = ((int64_t)a.n_tokens * a.k + 3) / 4;
+    HOARD_ROWS(combine_grad_kernel, groups < (1 << 20) ? groups : (1 << 20));
+}
+
+}  // namespace hoard
