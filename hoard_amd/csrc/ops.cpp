@@ -43,9 +43,9 @@ int q4(const hoard_q4_matrix *w, const hoard_q4_matrix *up, int mode, int type, 
     if (int rc = check_matrix("w", *w)) return rc;
     if (up) {
         if (int rc = check_matrix("up", *up)) return rc;
-        if (up->rows != w->rows || up->cols != w->cols || up->n_mat != w->n_mat)
-            return fail_fmt(HOARD_ERR_INVALID, "up is %d x %d x %d beside %d x %d x %d", up->n_mat, up->rows, up->cols,
-                            w->n_mat, w->rows, w->cols);
+        if (up->rows != w->rows || up->cols != w->cols || up->n_mat != w->n_mat || up->group != w->group)
+            return fail_fmt(HOARD_ERR_INVALID, "up is %d x %d x %d in groups of %d beside %d x %d x %d of %d", up->n_mat,
+                            up->rows, up->cols, up->group, w->n_mat, w->rows, w->cols, w->group);
     }
     if (mode == hoard::kQ4One && w->n_mat != 1) return fail_fmt(HOARD_ERR_INVALID, "n_mat %d without ids or offsets", w->n_mat);
     if (!activation_type(type)) return fail_fmt(HOARD_ERR_UNSUPPORTED, "activation type %d", type);
@@ -56,7 +56,7 @@ int q4(const hoard_q4_matrix *w, const hoard_q4_matrix *up, int mode, int type, 
     if (!x || !y || (mode != hoard::kQ4One && !sel)) return fail_fmt(HOARD_ERR_INVALID, "null argument");
     if (!aligned(x, 16)) return fail_fmt(HOARD_ERR_INVALID, "x is not 16-byte aligned");
     if (!aligned(y, type_size(type)) || !aligned(sel, 4)) return fail_fmt(HOARD_ERR_INVALID, "misaligned argument");
-    hoard::Q4Args a{*w, up ? *up : hoard_q4_matrix{}, mode, type, n_rows, x_share, x, sel, y};
+    hoard::Q4Args a{*w, up ? *up : hoard_q4_matrix{}, mode, type, n_rows, x_share, x, sel, y, 0};
     return launched("4-bit product", hoard::launch_q4(a, static_cast<hipStream_t>(stream)));
 }
 

@@ -21,6 +21,7 @@ struct Q4Args {
     const void *x;
     const int32_t *sel;
     void *y;
+    int64_t tile0;  // the first row tile of the launch (matrix tiles)
 };
 hipError_t launch_q4(const Q4Args &a, hipStream_t s);
 

@@ -1,0 +1,90 @@
+// Pieces shared by the kernels of the 4-bit products.
+#pragma once
+
+#include "ops.h"
+#include "opsdev.h"
+
+namespace hoard {
+
+typedef bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef f16 v2h __attribute__((ext_vector_type(2)));
+typedef bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef f16 v8h __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+// Codes as 16 + code in 16-bit floats: a code placed in the high fraction bits of
+// 16.0 adds exactly itself, so eight codes cost four shifts and four masked ors.
+// The sum over a group is then (sum of (16 + code) x) - (16 + zero) (sum of x),
+// whose terms are at most some five times the plain ones'.  Word j of the result
+// holds elements j (low) and j + 4 (high): x is laid out the same way (kOrder).
+template <typename T>
+struct Biased;
+template <>
+struct Biased<bf16> {
+    static constexpr uint32_t base = 0x41804180u, mask = 0x00780078u;
+    static constexpr int shift = 3;  // 16.0 has steps of 1/8
+};
+template <>
+struct Biased<f16> {
+    static constexpr uint32_t base = 0x4c004c00u, mask = 0x03c003c0u;
+    static constexpr int shift = 6;  // steps of 1/64
+};
+template <typename T>
+__device__ __forceinline__ v4u biased(uint32_t codes) {
+    typedef Biased<T> B;
+    v4u o;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int s = B::shift - 4 * j;
+        o[j] = ((s >= 0 ? codes << (s > 0 ? s : 0) : codes >> (s < 0 ? -s : 0)) & B::mask) | B::base;
+    }
+    return o;
+}
+
+// Eight consecutive 16-bit values as words {0, 4}, {1, 5}, {2, 6}, {3, 7}.
+__device__ __forceinline__ v4u paired(v4u x) {
+    v4u o;
+    o[0] = __builtin_amdgcn_perm(x[2], x[0], 0x05040100u);
+    o[1] = __builtin_amdgcn_perm(x[2], x[0], 0x07060302u);
+    o[2] = __builtin_amdgcn_perm(x[3], x[1], 0x05040100u);
+    o[3] = __builtin_amdgcn_perm(x[3], x[1], 0x07060302u);
+    return o;
+}
+
+// A scale as it is stored, and its value.
+__device__ __forceinline__ uint32_t raw_scale(const hoard_q4_matrix &m, size_t i) {
+    if (m.scale_type == HOARD_TYPE_F32) return static_cast<const uint32_t *>(m.scales)[i];
+    return static_cast<const uint16_t *>(m.scales)[i];
+}
+__device__ __forceinline__ float scale_of(int type, uint32_t raw) {
+    if (type == HOARD_TYPE_F32) return __uint_as_float(raw);
+    if (type == HOARD_TYPE_BF16) return __uint_as_float(raw << 16);
+    return (float)__builtin_bit_cast(f16, (uint16_t)raw);
+}
+
+// The matrix of row r, or -1.
+__device__ __forceinline__ int matrix_of(const Q4Args &a, int r) {
+    if (a.mode == kQ4One) return 0;
+    if (a.mode == kQ4Ids) {
+        const int e = a.sel[r];
+        return e < 0 || e >= a.w.n_mat ? -1 : e;
+    }
+    // the last e with sel[e] <= r
+    int lo = 0, hi = a.w.n_mat;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.sel[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    return a.sel[lo] <= r && r < a.sel[lo + 1] ? lo : -1;
+}
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// Matrix tiles (q4_tiles.h), by the activations' type.
+hipError_t launch_q4_tiles_f32(const Q4Args &a, hipStream_t s);
+hipError_t launch_q4_tiles_f16(const Q4Args &a, hipStream_t s);
+hipError_t launch_q4_tiles_bf16(const Q4Args &a, hipStream_t s);
+
+}  // namespace hoard

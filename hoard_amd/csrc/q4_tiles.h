@@ -1,0 +1,367 @@
+// 4-bit products on matrix instructions (v_mfma_f32_16x16x32_{bf16,f16}).
+//
+// A workgroup takes a tile of up to 16 MT rows of x (of one matrix) and NW * 16 P
+// rows of W (NW * 16 of both matrices with a second one).  Its waves are NW wide
+// over the rows of W and KS deep over the columns; the KS partial sums meet in
+// LDS.  Codes go from memory to registers, each read by one wave, one step of
+// KB * 128 columns ahead; x goes through LDS once per workgroup and step.
+//
+// x is the A operand and W the B operand: a lane then holds one row of W, its
+// scale and zero point, and 4 rows of x in an accumulator.  A lane reads 32
+// consecutive codes of its row (16 bytes) for four steps of 32 columns.  The order
+// of the columns within a step is free as long as x is read in the same one, so
+// the words are taken as they come for groups of 128; for 64 and 32 they are
+// exchanged between the lanes of a row (v_permlane32_swap, v_permlane16_swap) so
+// that a step never spans two groups.  A group's sum is scaled once it is whole.
+//
+// fp32 activations are split into three bf16 parts of 8 bits each (exactly x,
+// where x is no smaller than the smallest normal by 2^16), each a plane of its own.
+#pragma once
+
+#include "lds_dma.h"
+#include "q4.h"
+
+namespace hoard {
+
+template <typename T>
+struct Tiles {
+    typedef T elem;
+    static constexpr int planes = 1;
+};
+template <>
+struct Tiles<float> {
+    typedef bf16 elem;
+    static constexpr int planes = 3;
+};
+
+template <typename E>
+__device__ __forceinline__ v4f mfma_16x16x32(v4u x, v4u w, v4f c);
+template <>
+__device__ __forceinline__ v4f mfma_16x16x32<bf16>(v4u x, v4u w, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x), __builtin_bit_cast(v8bf, w), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ v4f mfma_16x16x32<f16>(v4u x, v4u w, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, w), c, 0, 0, 0);
+}
+
+// Four words of a lane rearranged among the four lanes (16 apart) of a row of W.
+template <int G>
+__device__ __forceinline__ v4u exchange(v4u c) {
+    if (G <= 64) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const auto r = __builtin_amdgcn_permlane32_swap(c[i], c[i + 2], false, false);
+            c[i] = r[0];
+            c[i + 2] = r[1];
+        }
+    }
+    if (G <= 32) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const auto r = __builtin_amdgcn_permlane16_swap(c[i], c[i + 1], false, false);
+            c[i] = r[0];
+            c[i + 1] = r[1];
+        }
+    }
+    return c;
+}
+// The first of the 8 columns (of 128) that word `step` of lane group `q` holds then.
+template <int G>
+__device__ __forceinline__ int column_of(int step, int q) {
+    if (G == 32) return step * 32 + q * 8;
+    if (G == 64) return ((step & 2) + (q & 1)) * 32 + ((q & 2) + (step & 1)) * 8;
+    return q * 32 + step * 8;
+}
+
+// Eight values of a row of x as they are fetched.
+template <typename T>
+struct Piece {
+    uint32_t w[2 * sizeof(T)];
+};
+
+// The tile of the workgroup: matrix, first row and row count.  Sorted rows: tile
+// number `t` over the matrices' tiles in ascending order; each lane adds up a run
+// of matrices.  False: no such tile.
+__device__ __forceinline__ bool tile_of(const Q4Args &a, int64_t t, int tm, int &e, int &r0, int &rows) {
+    if (a.mode != kQ4Sorted) {
+        e = 0;
+        r0 = (int)t * tm;
+        rows = min(tm, a.n_rows - r0);
+        return rows > 0;
+    }
+    const int lane = threadIdx.x & 63, n = a.w.n_mat, per = (n + 63) / 64, e0 = lane * per, e1 = min(n, e0 + per);
+    auto at = [&](int i) { return max(0, min(a.n_rows, a.sel[i])); };
+    int mine = 0;
+    if (e0 < e1) {
+        int lo = at(e0);
+        for (int i = e0; i < e1; i++) {
+            const int hi = at(i + 1);
+            mine += max(0, hi - lo + tm - 1) / tm;
+            lo = hi;
+        }
+    }
+    int incl = mine;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int v = __shfl_up(incl, d);
+        if (lane >= d) incl += v;
+    }
+    const uint64_t past = __ballot(incl > t);
+    if (!past) return false;
+    const int who = __ffsll((unsigned long long)past) - 1;
+    int left = (int)t - __shfl(incl - mine, who), lo = 0, hi = 0;
+    for (e = who * per;; e++) {  // ends at the matrix whose tile it is, within the lane's run
+        lo = at(e);
+        hi = at(e + 1);
+        const int tiles = max(0, hi - lo + tm - 1) / tm;
+        if (left < tiles || e + 1 >= n) break;
+        left -= tiles;
+    }
+    r0 = lo + left * tm;
+    rows = min(tm, hi - r0);
+    return rows > 0;
+}
+
+template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB>
+__global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
+    typedef typename Tiles<T>::elem E;
+    constexpr int PL = Tiles<T>::planes, TM = 16 * MT, THREADS = 64 * NW * KS;
+    constexpr int NG = 128 / G, SP = 4 / NG;               // groups in a block of 128 columns, steps in a group
+    constexpr int COLS = KS * KB * 128;                    // columns of a step of the workgroup
+    constexpr int RS = COLS * 2 + 16;                      // bytes of a row of x in LDS: 16 off the banks' period
+    constexpr int XP = TM * (COLS / 8) / THREADS;          // pieces of 8 values a thread stages
+    constexpr int XS = KS * KB * NG;                       // groups of a step
+    constexpr int MEET = KS > 1 ? (KS - 1) * NW * P * MT * 1024 : 0;  // bytes of the partial sums
+    static_assert(TM * (COLS / 8) % THREADS == 0, "whole pieces a thread");
+    static_assert(!UP || P == 2, "the second matrix is the second stream");
+    constexpr int XBYTES = PL * TM * RS;
+    __shared__ __align__(16) uint8_t lds[XBYTES > MEET ? XBYTES : MEET];
+    __shared__ __align__(16) float sums[XS][TM];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), nw = wave % NW, ks = wave / NW;
+    const int col = lane & 15, q = lane >> 4;
+    int e, r0, rows;
+    if (!tile_of(a, a.tile0 + blockIdx.y, TM, e, r0, rows)) return;
+    const int cols = a.w.cols, blocks = (cols + 127) / 128, steps = (blocks + KS * KB - 1) / (KS * KB);
+    constexpr int WIDE = UP ? 16 : 16 * P;  // rows of W of a wave
+    const int n0 = (blockIdx.x * NW + nw) * WIDE + col;
+
+    // the streams: rows of W (clamped: what lies behind the last row is not stored)
+    const uint8_t *code[P];
+    size_t sbase[P];
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
+        const size_t row = (size_t)e * a.w.rows + min(n0 + (UP ? 0 : 16 * p), a.w.rows - 1);
+        code[p] = static_cast<const uint8_t *>(m.codes) + row * (cols / 2);
+        sbase[p] = row * (cols / G);
+    }
+
+    v4u codes[P][KB];
+    uint32_t scales[P][KB][NG], zeros[P][KB][NG];
+    Piece<T> xr[XP];
+    auto fetch = [&](int step) {
+#pragma unroll
+        for (int b = 0; b < KB; b++) {
+            const int block = (step * KS + ks) * KB + b, k = block * 128 + q * 32;
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
+                codes[p][b] = (v4u)(0);
+                if (k < cols) codes[p][b] = *reinterpret_cast<const v4u *>(code[p] + k / 2);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const int gi = block * NG + g;
+                    scales[p][b][g] = 0;
+                    zeros[p][b][g] = 8;
+                    if (gi * G < cols) {
+                        scales[p][b][g] = raw_scale(m, sbase[p] + gi);
+                        if (m.zeros) zeros[p][b][g] = m.zeros[sbase[p] + gi];
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < XP; j++) {
+            const int i = tid + j * THREADS, row = i / (COLS / 8), k = step * COLS + (i % (COLS / 8)) * 8;
+            xr[j] = Piece<T>{};
+            if (row < rows && k < cols)
+                xr[j] = *reinterpret_cast<const Piece<T> *>(static_cast<const T *>(a.x) + (size_t)(r0 + row) * cols + k);
+        }
+    };
+    // x into LDS, and its sums over the groups
+    auto stage = [&]() {
+#pragma unroll
+        for (int j = 0; j < XP; j++) {
+            const int i = tid + j * THREADS, row = i / (COLS / 8), piece = i % (COLS / 8);
+            uint8_t *to = lds + row * RS + piece * 16;
+            float s = 0.0f;
+            if constexpr (PL == 1) {
+                v4u w;
+                __builtin_memcpy(&w, &xr[j], 16);
+                T v[8];
+                __builtin_memcpy(v, &xr[j], 16);
+#pragma unroll
+                for (int c = 0; c < 8; c++) s += (float)v[c];
+                *reinterpret_cast<v4u *>(to) = paired(w);
+            } else {
+                uint32_t part[3][8];
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    const uint32_t w = xr[j].w[c];
+                    const float x = __uint_as_float(w);
+                    s += x;
+                    // of an infinity or a NaN the first part says it all
+                    const float x1 = __uint_as_float(w & 0xffff0000u), rest = isfinite(x) ? x - x1 : 0.0f;
+                    const float x2 = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+                    part[0][c] = __float_as_uint(x1) | (x != x ? 0x400000u : 0u);
+                    part[1][c] = __float_as_uint(x2);
+                    part[2][c] = __float_as_uint(rest - x2);
+                }
+#pragma unroll
+                for (int l = 0; l < 3; l++) {
+                    v4u w;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) w[c] = __builtin_amdgcn_perm(part[l][c + 4], part[l][c], 0x07060302u);
+                    *reinterpret_cast<v4u *>(to + l * TM * RS) = w;
+                }
+            }
+            // a group's G / 8 pieces lie in consecutive lanes
+            s += dpp_f<kDppQuadXor1>(s);
+            s += dpp_f<kDppQuadXor2>(s);
+            if (G >= 64) s += dpp_f<kDppRowHalfMirror>(s);
+            if (G >= 128) s += dpp_f<kDppRowMirror>(s);
+            if (piece % (G / 8) == 0) sums[piece / (G / 8)][row] = s;
+        }
+    };
+
+    v4f acc[P][MT];
+#pragma unroll
+    for (int p = 0; p < P; p++)
+#pragma unroll
+        for (int t = 0; t < MT; t++) acc[p][t] = (v4f)(0.0f);
+
+    fetch(0);
+    for (int step = 0; step < steps; step++) {
+        if (step) __syncthreads();  // the last step's x has been read
+        stage();
+        v4u now[P][KB];
+        float sc[P][KB][NG], zc[P][KB][NG];
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int b = 0; b < KB; b++) {
+                now[p][b] = exchange<G>(codes[p][b]);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    sc[p][b][g] = scale_of(UP && p == 1 ? a.up.scale_type : a.w.scale_type, scales[p][b][g]);
+                    zc[p][b][g] = 16.0f + (float)zeros[p][b][g];
+                }
+            }
+        __syncthreads();
+        if (step + 1 < steps) fetch(step + 1);
+#pragma unroll
+        for (int b = 0; b < KB; b++) {
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                v4u w[P][SP];
+#pragma unroll
+                for (int p = 0; p < P; p++)
+#pragma unroll
+                    for (int i = 0; i < SP; i++) w[p][i] = biased<E>(now[p][b][g * SP + i]);
+#pragma unroll
+                for (int t = 0; t < MT; t++) {
+                    if (t * 16 >= rows) break;
+                    const v4f xs = *reinterpret_cast<const v4f *>(&sums[(ks * KB + b) * NG + g][t * 16 + 4 * q]);
+                    v4f d[P];
+#pragma unroll
+                    for (int p = 0; p < P; p++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) d[p][i] = -zc[p][b][g] * xs[i];
+                    const uint8_t *from = lds + (t * 16 + col) * RS + (ks * KB + b) * 256;
+#pragma unroll
+                    for (int i = 0; i < SP; i++)
+#pragma unroll
+                        for (int l = 0; l < PL; l++) {
+                            const v4u x = *reinterpret_cast<const v4u *>(from + l * TM * RS + 2 * column_of<G>(g * SP + i, q));
+#pragma unroll
+                            for (int p = 0; p < P; p++) d[p] = mfma_16x16x32<E>(x, w[p][i], d[p]);
+                        }
+#pragma unroll
+                    for (int p = 0; p < P; p++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[p][t][i] = fmaf(sc[p][b][g], d[p][i], acc[p][t][i]);
+                }
+            }
+        }
+    }
+    if constexpr (KS > 1) {
+        __syncthreads();
+        v4f *meet = reinterpret_cast<v4f *>(lds);
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+                if (ks) meet[((((ks - 1) * NW + nw) * P + p) * MT + t) * 64 + lane] = acc[p][t];
+        __syncthreads();
+        if (ks) return;
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int k = 1; k < KS; k++) acc[p][t] += meet[((((k - 1) * NW + nw) * P + p) * MT + t) * 64 + lane];
+    }
+    T *y = static_cast<T *>(a.y) + (size_t)r0 * a.w.rows;
+#pragma unroll
+    for (int p = 0; p < (UP ? 1 : P); p++) {
+        const int n = n0 + 16 * p;
+        if (n >= a.w.rows) continue;
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = t * 16 + 4 * q + i;
+                if (row >= rows) continue;
+                float v = acc[p][t][i];
+                if constexpr (UP) v = silu_mul(v, acc[1][t][i]);
+                y[(size_t)row * a.w.rows + n] = (T)v;
+            }
+    }
+}
+
+template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB>
+hipError_t launch_tiles_of(const Q4Args &a, hipStream_t s) {
+    constexpr int TM = 16 * MT, TN = NW * (UP ? 16 : 16 * P);
+    int64_t tiles = ((int64_t)a.n_rows + TM - 1) / TM;
+    if (a.mode == kQ4Sorted) tiles = a.n_rows / TM + (a.n_rows < a.w.n_mat ? a.n_rows : a.w.n_mat);
+    Q4Args part = a;
+    for (part.tile0 = 0; part.tile0 < tiles; part.tile0 += 65535) {  // what a grid's second dimension holds
+        const dim3 grid((a.w.rows + TN - 1) / TN, (unsigned)(tiles - part.tile0 < 65535 ? tiles - part.tile0 : 65535));
+        q4_tiles_kernel<T, G, UP, P, MT, NW, KS, KB><<<grid, 64 * NW * KS, 0, s>>>(part);
+        const hipError_t rc = hipGetLastError();
+        if (rc != hipSuccess) return rc;
+    }
+    return hipSuccess;
+}
+
+template <typename T, int G, bool UP>
+hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
+    constexpr bool WIDE = sizeof(T) == 4;  // three planes of x
+    const int per = a.mode == kQ4Sorted ? (a.n_rows + a.w.n_mat - 1) / a.w.n_mat : a.n_rows;
+    if (per <= 16) return launch_tiles_of<T, G, UP, UP ? 2 : 1, 1, 1, WIDE ? 4 : 8, 1>(a, s);
+    if (per <= 24 || WIDE) return launch_tiles_of<T, G, UP, 2, 2, 4, 1, WIDE ? 1 : 2>(a, s);
+    return launch_tiles_of<T, G, UP, 2, 4, 4, 1, 2>(a, s);
+}
+
+template <typename T>
+hipError_t launch_tiles_typed(const Q4Args &a, hipStream_t s) {
+    const bool up = a.up.codes != nullptr;
+    switch (a.w.group) {
+        case 32: return up ? launch_tiles_sized<T, 32, true>(a, s) : launch_tiles_sized<T, 32, false>(a, s);
+        case 64: return up ? launch_tiles_sized<T, 64, true>(a, s) : launch_tiles_sized<T, 64, false>(a, s);
+        default: return up ? launch_tiles_sized<T, 128, true>(a, s) : launch_tiles_sized<T, 128, false>(a, s);
+    }
+}
+
+}  // namespace hoard

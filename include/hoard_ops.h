@@ -55,7 +55,7 @@ typedef struct hoard_q4_matrix {
 } hoard_q4_matrix;
 
 /* y[r] = W x[r] for n_rows rows: x [n_rows][cols] and y [n_rows][rows] of `type`,
-   x 16-byte aligned.  With `up` (same rows, cols and n_mat; its group, zeros and
+   x 16-byte aligned.  With `up` (same rows, cols, group and n_mat; its zeros and
    scale type may differ) y[r] = silu(W x[r]) * (W_up x[r]).  W has n_mat 1.  The
    products are formed with the activations as given, not quantised.  A row of x
    that holds an infinity or a NaN gives a row of y without a defined value

@@ -66,8 +66,8 @@ def test_dense(n, rows, cols, group, dtype, scales, zeros, up):
     from hoard_amd.ops import q4_matmul
     print("q4 dense", n, rows, cols, group, dtype, flush=True)
     w = weights(1, 0, rows, cols, group, scales, zeros)
-    # the second matrix has its own group and zeros
-    u = weights(2, 0, rows, cols, 32, F32, not zeros) if up else None
+    # the second matrix has its own scale type and zeros
+    u = weights(2, 0, rows, cols, group, F32, not zeros) if up else None
     x = rows_of(3, n, cols, dtype)
     y = q4_matmul(x, op(w), op(u) if up else None)
     R.close(y, *expect(x, w, u), "y")

@@ -46,6 +46,7 @@ def test_q4_call(hlib):
     refused(hlib.hoard_q4_matmul(many, None, H.TYPE_F32, 1, A, A, None), inv, "n_mat")
     refused(hlib.hoard_q4_matmul(w, ctypes.byref(q4(rows=65)), H.TYPE_F32, 1, A, A, None), inv, "up")
     refused(hlib.hoard_q4_matmul(w, ctypes.byref(q4(cols=384)), H.TYPE_F32, 1, A, A, None), inv, "up")
+    refused(hlib.hoard_q4_matmul(w, ctypes.byref(q4(group=64)), H.TYPE_F32, 1, A, A, None), inv, "groups of 64")
     refused(hlib.hoard_q4_matmul(w, None, H.TYPE_Q4_K, 1, A, A, None), H.ERR_UNSUPPORTED, "type")
     refused(hlib.hoard_q4_matmul(w, None, H.TYPE_F32, -1, A, A, None), inv, "n_rows")
     refused(hlib.hoard_q4_matmul(w, None, H.TYPE_F32, 1, None, A, None), inv, "null")
