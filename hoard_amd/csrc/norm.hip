@@ -219,22 +219,27 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
 }
 
 // The groups' partial sums [parameter][groups][n] added: a workgroup takes 64
-// columns, its 4 waves a quarter of the groups each, in ascending order.
+// columns, its 16 waves a sixteenth of the groups each, in ascending order.
 struct SumOut {
     float *out[3];
 };
-__global__ __launch_bounds__(256) void norm_sum_kernel(const float *work, int groups, int n, SumOut o) {
-    __shared__ float part[4][64];
+__global__ __launch_bounds__(1024) void norm_sum_kernel(const float *work, int groups, int n, SumOut o) {
+    __shared__ float part[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
-    const int per = (groups + 3) / 4, g0 = wave * per, g1 = min(groups, g0 + per);
+    const int per = (groups + 15) / 16, g0 = wave * per, g1 = min(groups, g0 + per);
     float s = 0.0f;
     if (col < n) {
         const float *p = work + (size_t)blockIdx.y * groups * n + col;
+#pragma unroll 8
         for (int g = g0; g < g1; g++) s += p[(size_t)g * n];
     }
     part[wave][lane] = s;
     __syncthreads();
-    if (wave == 0 && col < n) o.out[blockIdx.y][col] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    if (wave) return;
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s += part[i][lane];
+    if (col < n) o.out[blockIdx.y][col] = s;
 }
 
 template <typename T, typename R, int BS, int NV>
@@ -290,7 +295,7 @@ hipError_t launch_norm_grad(const hoard_norm_args &a, const hoard_norm_grads &g,
     if (g.dw_post) o.out[params++] = g.dw_post;
     if (g.dgate && a.gate_kind == HOARD_GATE_CHANNEL) o.out[params++] = static_cast<float *>(g.dgate);
     if (!params) return hipSuccess;
-    norm_sum_kernel<<<dim3((a.n + 63) / 64, params), 256, 0, s>>>(work, norm_groups(a.n_rows, a.n), a.n, o);
+    norm_sum_kernel<<<dim3((a.n + 63) / 64, params), 1024, 0, s>>>(work, norm_groups(a.n_rows, a.n), a.n, o);
     return hipGetLastError();
 }
 

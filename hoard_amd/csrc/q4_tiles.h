@@ -18,7 +18,8 @@
 // where x is no smaller than the smallest normal by 2^16), each a plane of its own.
 #pragma once
 
-#include "lds_dma.h"
+#include <type_traits>
+
 #include "q4.h"
 
 namespace hoard {
@@ -157,30 +158,35 @@ __global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
         sbase[p] = row * (cols / G);
     }
 
-    v4u codes[P][KB];
-    uint32_t scales[P][KB][NG], zeros[P][KB][NG];
+    // codes two steps ahead, x one: the loads of a step are issued x first, so that
+    // staging x waits for nothing behind it
+    v4u codes[2][P][KB];
+    uint32_t scales[2][P][KB][NG], zeros[2][P][KB][NG];
     Piece<T> xr[XP];
-    auto fetch = [&](int step) {
+    auto fetch_w = [&](auto at, int step) {
+        constexpr int B = decltype(at)::value;
 #pragma unroll
         for (int b = 0; b < KB; b++) {
             const int block = (step * KS + ks) * KB + b, k = block * 128 + q * 32;
 #pragma unroll
             for (int p = 0; p < P; p++) {
                 const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
-                codes[p][b] = (v4u)(0);
-                if (k < cols) codes[p][b] = *reinterpret_cast<const v4u *>(code[p] + k / 2);
+                codes[B][p][b] = (v4u)(0);
+                if (k < cols) codes[B][p][b] = *reinterpret_cast<const v4u *>(code[p] + k / 2);
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
                     const int gi = block * NG + g;
-                    scales[p][b][g] = 0;
-                    zeros[p][b][g] = 8;
+                    scales[B][p][b][g] = 0;
+                    zeros[B][p][b][g] = 8;
                     if (gi * G < cols) {
-                        scales[p][b][g] = raw_scale(m, sbase[p] + gi);
-                        if (m.zeros) zeros[p][b][g] = m.zeros[sbase[p] + gi];
+                        scales[B][p][b][g] = raw_scale(m, sbase[p] + gi);
+                        if (m.zeros) zeros[B][p][b][g] = m.zeros[sbase[p] + gi];
                     }
                 }
             }
         }
+    };
+    auto fetch_x = [&](int step) {
 #pragma unroll
         for (int j = 0; j < XP; j++) {
             const int i = tid + j * THREADS, row = i / (COLS / 8), k = step * COLS + (i % (COLS / 8)) * 8;
@@ -241,8 +247,8 @@ __global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
 #pragma unroll
         for (int t = 0; t < MT; t++) acc[p][t] = (v4f)(0.0f);
 
-    fetch(0);
-    for (int step = 0; step < steps; step++) {
+    auto body = [&](auto at, int step) {
+        constexpr int B = decltype(at)::value;
         if (step) __syncthreads();  // the last step's x has been read
         stage();
         v4u now[P][KB];
@@ -251,15 +257,16 @@ __global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int b = 0; b < KB; b++) {
-                now[p][b] = exchange<G>(codes[p][b]);
+                now[p][b] = exchange<G>(codes[B][p][b]);
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    sc[p][b][g] = scale_of(UP && p == 1 ? a.up.scale_type : a.w.scale_type, scales[p][b][g]);
-                    zc[p][b][g] = 16.0f + (float)zeros[p][b][g];
+                    sc[p][b][g] = scale_of(UP && p == 1 ? a.up.scale_type : a.w.scale_type, scales[B][p][b][g]);
+                    zc[p][b][g] = 16.0f + (float)zeros[B][p][b][g];
                 }
             }
         __syncthreads();
-        if (step + 1 < steps) fetch(step + 1);
+        if (step + 1 < steps) fetch_x(step + 1);
+        if (step + 2 < steps) fetch_w(at, step + 2);
 #pragma unroll
         for (int b = 0; b < KB; b++) {
 #pragma unroll
@@ -294,6 +301,15 @@ __global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
                 }
             }
         }
+    };
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> odd{};
+    fetch_w(even, 0);
+    fetch_x(0);
+    if (steps > 1) fetch_w(odd, 1);
+    for (int step = 0; step < steps; step += 2) {
+        body(even, step);
+        if (step + 1 < steps) body(odd, step + 1);
     }
     if constexpr (KS > 1) {
         __syncthreads();
