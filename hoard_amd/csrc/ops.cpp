@@ -14,6 +14,8 @@ bool activation_type(int t) { return t == HOARD_TYPE_F32 || t == HOARD_TYPE_F16 
 size_t type_size(int t) { return t == HOARD_TYPE_F32 ? 4 : 2; }
 bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+constexpr int kMaxCols = 1 << 20;  // 64 rows of x lie within the kernels' 32-bit offsets
+
 int launched(const char *what, hipError_t rc) {
     if (rc == hipSuccess) {
         hoard_set_error(HOARD_OK, "");
@@ -30,6 +32,7 @@ int check_matrix(const char *what, const hoard_q4_matrix &m) {
         return fail_fmt(HOARD_ERR_UNSUPPORTED, "%s: group %d is not 32, 64 or 128", what, m.group);
     if (m.cols <= 0 || m.cols % m.group)
         return fail_fmt(HOARD_ERR_INVALID, "%s: cols %d not a positive multiple of group %d", what, m.cols, m.group);
+    if (m.cols > kMaxCols) return fail_fmt(HOARD_ERR_UNSUPPORTED, "%s: cols %d above %d", what, m.cols, kMaxCols);
     if (!activation_type(m.scale_type))
         return fail_fmt(HOARD_ERR_UNSUPPORTED, "%s: scale type %d", what, m.scale_type);
     if (!aligned(m.scales, type_size(m.scale_type)))
@@ -56,7 +59,7 @@ int q4(const hoard_q4_matrix *w, const hoard_q4_matrix *up, int mode, int type, 
     if (!x || !y || (mode != hoard::kQ4One && !sel)) return fail_fmt(HOARD_ERR_INVALID, "null argument");
     if (!aligned(x, 16)) return fail_fmt(HOARD_ERR_INVALID, "x is not 16-byte aligned");
     if (!aligned(y, type_size(type)) || !aligned(sel, 4)) return fail_fmt(HOARD_ERR_INVALID, "misaligned argument");
-    hoard::Q4Args a{*w, up ? *up : hoard_q4_matrix{}, mode, type, n_rows, x_share, x, sel, y, 0};
+    hoard::Q4Args a{*w, up ? *up : hoard_q4_matrix{}, mode, type, n_rows, x_share, x, sel, y, 0, false};
     return launched("4-bit product", hoard::launch_q4(a, static_cast<hipStream_t>(stream)));
 }
 

@@ -21,7 +21,10 @@ struct Q4Args {
     const void *x;
     const int32_t *sel;
     void *y;
-    int64_t tile0;  // the first row tile of the launch (matrix tiles)
+    // matrix tiles, set by their launch: its first tile of rows of x, and whether the
+    // workgroups of a tile go to one XCD
+    int64_t tile0;
+    bool spread;
 };
 hipError_t launch_q4(const Q4Args &a, hipStream_t s);
 

@@ -33,11 +33,15 @@ struct Biased<f16> {
 template <typename T>
 __device__ __forceinline__ v4u biased(uint32_t codes) {
     typedef Biased<T> B;
+    // in a register the compiler cannot see through: the masked or is then one
+    // instruction (v_and_or_b32 takes no two constants), not two
+    uint32_t base = B::base;
+    asm("" : "+v"(base));
     v4u o;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int s = B::shift - 4 * j;
-        o[j] = ((s >= 0 ? codes << (s > 0 ? s : 0) : codes >> (s < 0 ? -s : 0)) & B::mask) | B::base;
+        o[j] = ((s >= 0 ? codes << (s > 0 ? s : 0) : codes >> (s < 0 ? -s : 0)) & B::mask) | base;
     }
     return o;
 }
@@ -52,10 +56,21 @@ __device__ __forceinline__ v4u paired(v4u x) {
     return o;
 }
 
-// A scale as it is stored, and its value.
-__device__ __forceinline__ uint32_t raw_scale(const hoard_q4_matrix &m, size_t i) {
-    if (m.scale_type == HOARD_TYPE_F32) return static_cast<const uint32_t *>(m.scales)[i];
-    return static_cast<const uint16_t *>(m.scales)[i];
+// s + the products of two pairs of values; a pair of ones.
+template <typename T>
+__device__ __forceinline__ float dot2(uint32_t w, uint32_t x, float s) {
+    if constexpr (__is_same(T, bf16))
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, x), s, false);
+    else
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, x), s, false);
+}
+template <typename T>
+constexpr uint32_t kOnes = __is_same(T, bf16) ? 0x3f803f80u : 0x3c003c00u;
+
+// A scale as it is stored (scale `i` from `base` on), and its value.
+__device__ __forceinline__ uint32_t raw_scale(const hoard_q4_matrix &m, size_t base, uint32_t i) {
+    if (m.scale_type == HOARD_TYPE_F32) return (static_cast<const uint32_t *>(m.scales) + base)[i];
+    return (static_cast<const uint16_t *>(m.scales) + base)[i];
 }
 __device__ __forceinline__ float scale_of(int type, uint32_t raw) {
     if (type == HOARD_TYPE_F32) return __uint_as_float(raw);

@@ -20,18 +20,10 @@ struct Slice {  // 16-bit types: words of two values in the order of biased()
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const v4u w = reinterpret_cast<const v4u *>(p)[i];
-            T v[8];
-            __builtin_memcpy(v, &w, 16);
 #pragma unroll
-            for (int c = 0; c < 8; c++) sum += (float)v[c];
+            for (int c = 0; c < 4; c++) sum = dot2<T>(w[c], kOnes<T>, sum);
             x[i] = paired(w);
         }
-    }
-    static __device__ __forceinline__ float dot2(uint32_t w, uint32_t x, float s) {
-        if constexpr (sizeof(T) == 2 && __is_same(T, bf16))
-            return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, x), s, false);
-        else
-            return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, x), s, false);
     }
 };
 template <>
@@ -64,7 +56,7 @@ __device__ __forceinline__ void dots(v4u codes, float zero, const Slice<T> (&x)[
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) d[r] = Slice<T>::dot2(w[j], x[r].x[i][j], d[r]);
+                for (int j = 0; j < 4; j++) d[r] = dot2<T>(w[j], x[r].x[i][j], d[r]);
         }
     } else {
         // a byte of a masked word converts in one instruction
@@ -116,7 +108,7 @@ __global__ __launch_bounds__(256) void q4_rows_kernel(Q4Args a, int lanes_log) {
                         codes[p][j] = *reinterpret_cast<const v4u *>(static_cast<const uint8_t *>(m.codes) +
                                                                      row[j] * (cols / 2) + k / 2);
                         const size_t gi = row[j] * groups + (k >> group_log);
-                        scale[p][j] = raw_scale(m, gi);
+                        scale[p][j] = raw_scale(m, gi, 0);
                         zero[p][j] = m.zeros ? m.zeros[gi] : 8;
                     }
                 }

@@ -18,6 +18,7 @@
 // where x is no smaller than the smallest normal by 2^16), each a plane of its own.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "q4.h"
@@ -86,10 +87,11 @@ struct Piece {
 // of matrices.  False: no such tile.
 __device__ __forceinline__ bool tile_of(const Q4Args &a, int64_t t, int tm, int &e, int &r0, int &rows) {
     if (a.mode != kQ4Sorted) {
+        if (t * tm >= a.n_rows) return false;
         e = 0;
         r0 = (int)t * tm;
         rows = min(tm, a.n_rows - r0);
-        return rows > 0;
+        return true;
     }
     const int lane = threadIdx.x & 63, n = a.w.n_mat, per = (n + 63) / 64, e0 = lane * per, e1 = min(n, e0 + per);
     auto at = [&](int i) { return max(0, min(a.n_rows, a.sel[i])); };
@@ -110,7 +112,7 @@ __device__ __forceinline__ bool tile_of(const Q4Args &a, int64_t t, int tm, int 
     const uint64_t past = __ballot(incl > t);
     if (!past) return false;
     const int who = __ffsll((unsigned long long)past) - 1;
-    int left = (int)t - __shfl(incl - mine, who), lo = 0, hi = 0;
+    int left = (int)t - __builtin_amdgcn_readlane(incl - mine, who), lo = 0, hi = 0;
     for (e = who * per;; e++) {  // ends at the matrix whose tile it is, within the lane's run
         lo = at(e);
         hi = at(e + 1);
@@ -118,97 +120,123 @@ __device__ __forceinline__ bool tile_of(const Q4Args &a, int64_t t, int tm, int 
         if (left < tiles || e + 1 >= n) break;
         left -= tiles;
     }
-    r0 = lo + left * tm;
-    rows = min(tm, hi - r0);
+    e = __builtin_amdgcn_readfirstlane(e);
+    r0 = __builtin_amdgcn_readfirstlane(lo + left * tm);
+    rows = __builtin_amdgcn_readfirstlane(min(tm, hi - r0));
     return rows > 0;
 }
 
-template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB>
-__global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
+template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB, int MW>
+__global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
     typedef typename Tiles<T>::elem E;
     constexpr int PL = Tiles<T>::planes, TM = 16 * MT, THREADS = 64 * NW * KS;
     constexpr int NG = 128 / G, SP = 4 / NG;               // groups in a block of 128 columns, steps in a group
     constexpr int COLS = KS * KB * 128;                    // columns of a step of the workgroup
     constexpr int RS = COLS * 2 + 16;                      // bytes of a row of x in LDS: 16 off the banks' period
     constexpr int XP = TM * (COLS / 8) / THREADS;          // pieces of 8 values a thread stages
+    constexpr int XROWS = THREADS / (COLS / 8);            // rows of x between them
     constexpr int XS = KS * KB * NG;                       // groups of a step
     constexpr int MEET = KS > 1 ? (KS - 1) * NW * P * MT * 1024 : 0;  // bytes of the partial sums
-    static_assert(TM * (COLS / 8) % THREADS == 0, "whole pieces a thread");
+    static_assert(XROWS * (COLS / 8) == THREADS && XP * XROWS == TM, "whole pieces a thread, whole rows between them");
     static_assert(!UP || P == 2, "the second matrix is the second stream");
     constexpr int XBYTES = PL * TM * RS;
+    constexpr int RW = 16 * NW * P;                        // rows of W, both matrices'
+    // groups of a row whose scales lie in LDS at a time, a thread's share of them
+    constexpr int MINSC = XS > 16 ? XS : 16, SC = MINSC * RW < THREADS ? THREADS / RW : MINSC;
+    constexpr int SPC = SC / XS, SI = RW * SC / THREADS;
+    static_assert(SC % XS == 0 && RW * SC % THREADS == 0 && SC % SI == 0, "whole steps, whole shares");
     __shared__ __align__(16) uint8_t lds[XBYTES > MEET ? XBYTES : MEET];
     __shared__ __align__(16) float sums[XS][TM];
+    __shared__ float scale[RW][SC + 1], zero[RW][SC + 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), nw = wave % NW, ks = wave / NW;
     const int col = lane & 15, q = lane >> 4;
     int e, r0, rows;
-    if (!tile_of(a, a.tile0 + blockIdx.y, TM, e, r0, rows)) return;
+    // a tile of x in all its tiles of W: next to each other, or (a.spread) on one XCD,
+    // whose L2 then fetches the rows of x once
+    const int nt = (a.w.rows + NW * (UP ? 16 : 16 * P) - 1) / (NW * (UP ? 16 : 16 * P));
+    const int id = blockIdx.x, run = a.spread ? id >> 3 : id;
+    const int tn = run % nt;
+    const int64_t tx = a.tile0 + (a.spread ? (run / nt) * 8 + (id & 7) : run / nt);
+    if (!tile_of(a, tx, TM, e, r0, rows)) return;
     const int cols = a.w.cols, blocks = (cols + 127) / 128, steps = (blocks + KS * KB - 1) / (KS * KB);
     constexpr int WIDE = UP ? 16 : 16 * P;  // rows of W of a wave
-    const int n0 = (blockIdx.x * NW + nw) * WIDE + col;
+    const int first = (tn * NW + nw) * WIDE, n0 = first + col;
 
-    // the streams: rows of W (clamped: what lies behind the last row is not stored)
-    const uint8_t *code[P];
-    size_t sbase[P];
+    // the streams: rows of W (clamped: what lies behind the last row is not stored),
+    // as a base of the wave's and 32-bit offsets of the lanes'
+    const int top = min(first, a.w.rows - 1), groups = cols / G;
+    // the last block of a lane's 32 columns that lies inside
+    const int last_block = (cols - 32 - q * 32) >= 0 ? (cols - 32 - q * 32) / 128 : 0;
+    const size_t row0 = (size_t)e * a.w.rows + top;
+    const uint8_t *const x0 = static_cast<const uint8_t *>(a.x) + (size_t)r0 * cols * sizeof(T);
+    uint32_t code[P];
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
-        const size_t row = (size_t)e * a.w.rows + min(n0 + (UP ? 0 : 16 * p), a.w.rows - 1);
-        code[p] = static_cast<const uint8_t *>(m.codes) + row * (cols / 2);
-        sbase[p] = row * (cols / G);
+        const uint32_t row = min(n0 + (UP ? 0 : 16 * p), a.w.rows - 1) - top;
+        code[p] = row * (cols / 2) + (q * 32 < cols ? q * 16 : 0);
     }
 
-    // codes two steps ahead, x one: the loads of a step are issued x first, so that
-    // staging x waits for nothing behind it
+    // Codes two steps ahead, x one: the loads of a step are issued x first, so that
+    // staging x waits for nothing behind it.  Nothing is loaded under a condition: what
+    // lies behind the last column or row is read from a place inside instead, x is
+    // zeroed behind the last column, and rows behind the last are not stored.
     v4u codes[2][P][KB];
-    uint32_t scales[2][P][KB][NG], zeros[2][P][KB][NG];
     Piece<T> xr[XP];
     auto fetch_w = [&](auto at, int step) {
         constexpr int B = decltype(at)::value;
+        const int block = (step * KS + ks) * KB;
 #pragma unroll
-        for (int b = 0; b < KB; b++) {
-            const int block = (step * KS + ks) * KB + b, k = block * 128 + q * 32;
+        for (int p = 0; p < P; p++) {
+            const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
+            const uint8_t *const from = static_cast<const uint8_t *>(m.codes) + row0 * (cols / 2);
 #pragma unroll
-            for (int p = 0; p < P; p++) {
-                const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
-                codes[B][p][b] = (v4u)(0);
-                if (k < cols) codes[B][p][b] = *reinterpret_cast<const v4u *>(code[p] + k / 2);
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    const int gi = block * NG + g;
-                    scales[B][p][b][g] = 0;
-                    zeros[B][p][b][g] = 8;
-                    if (gi * G < cols) {
-                        scales[B][p][b][g] = raw_scale(m, sbase[p] + gi);
-                        if (m.zeros) zeros[B][p][b][g] = m.zeros[sbase[p] + gi];
-                    }
-                }
-            }
+            for (int b = 0; b < KB; b++)
+                codes[B][p][b] = *reinterpret_cast<const v4u *>(from + (code[p] + min(block + b, last_block) * 64));
         }
     };
-    auto fetch_x = [&](int step) {
+    // the scales of SC groups into LDS: read along the rows, as they lie in memory
+    auto stage_scales = [&](int chunk) {
+        const int row = tid / (SC / SI), g0 = (tid % (SC / SI)) * SI, p = row / (16 * NW), in = row % (16 * NW);
+        const int n = tn * NW * WIDE + (UP ? in : (in / 16) * WIDE + p * 16 + in % 16);
+        const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
+        const size_t from = ((size_t)e * a.w.rows + min(n, a.w.rows - 1)) * groups;
 #pragma unroll
-        for (int j = 0; j < XP; j++) {
-            const int i = tid + j * THREADS, row = i / (COLS / 8), k = step * COLS + (i % (COLS / 8)) * 8;
-            xr[j] = Piece<T>{};
-            if (row < rows && k < cols)
-                xr[j] = *reinterpret_cast<const Piece<T> *>(static_cast<const T *>(a.x) + (size_t)(r0 + row) * cols + k);
+        for (int g = 0; g < SI; g++) {
+            const int at = min(chunk * SC + g0 + g, groups - 1);
+            scale[row][g0 + g] = scale_of(m.scale_type, raw_scale(m, from, at));
+            zero[row][g0 + g] = m.zeros ? 16.0f + (float)m.zeros[from + at] : 24.0f;
         }
+    };
+    const int xrow = tid / (COLS / 8), xcol = (tid % (COLS / 8)) * 8;
+    auto fetch_x = [&](int step) {
+        const int k = min(step * COLS + xcol, cols - 8);
+#pragma unroll
+        for (int j = 0; j < XP; j++)
+            if (j * XROWS < rows)
+                xr[j] = *reinterpret_cast<const Piece<T> *>(x0 + (uint32_t)(min(xrow + j * XROWS, rows - 1) * cols + k) *
+                                                                     (uint32_t)sizeof(T));
     };
     // x into LDS, and its sums over the groups
-    auto stage = [&]() {
+    auto stage = [&](int step) {
+        if ((step + 1) * COLS > cols) {
+            const bool in = step * COLS + xcol < cols;
+#pragma unroll
+            for (int j = 0; j < XP; j++)
+#pragma unroll
+                for (int c = 0; c < (int)(2 * sizeof(T)); c++) xr[j].w[c] = in ? xr[j].w[c] : 0u;
+        }
 #pragma unroll
         for (int j = 0; j < XP; j++) {
-            const int i = tid + j * THREADS, row = i / (COLS / 8), piece = i % (COLS / 8);
+            if (j * XROWS >= rows) break;
+            const int row = xrow + j * XROWS, piece = xcol / 8;
             uint8_t *to = lds + row * RS + piece * 16;
             float s = 0.0f;
             if constexpr (PL == 1) {
                 v4u w;
                 __builtin_memcpy(&w, &xr[j], 16);
-                T v[8];
-                __builtin_memcpy(v, &xr[j], 16);
 #pragma unroll
-                for (int c = 0; c < 8; c++) s += (float)v[c];
+                for (int c = 0; c < 4; c++) s = dot2<E>(w[c], kOnes<E>, s);
                 *reinterpret_cast<v4u *>(to) = paired(w);
             } else {
                 uint32_t part[3][8];
@@ -250,20 +278,13 @@ __global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
     auto body = [&](auto at, int step) {
         constexpr int B = decltype(at)::value;
         if (step) __syncthreads();  // the last step's x has been read
-        stage();
+        if (step % SPC == 0) stage_scales(step / SPC);
+        stage(step);
         v4u now[P][KB];
-        float sc[P][KB][NG], zc[P][KB][NG];
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
-            for (int b = 0; b < KB; b++) {
-                now[p][b] = exchange<G>(codes[B][p][b]);
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    sc[p][b][g] = scale_of(UP && p == 1 ? a.up.scale_type : a.w.scale_type, scales[B][p][b][g]);
-                    zc[p][b][g] = 16.0f + (float)zeros[B][p][b][g];
-                }
-            }
+            for (int b = 0; b < KB; b++) now[p][b] = exchange<G>(codes[B][p][b]);
         __syncthreads();
         if (step + 1 < steps) fetch_x(step + 1);
         if (step + 2 < steps) fetch_w(at, step + 2);
@@ -272,6 +293,13 @@ __global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 v4u w[P][SP];
+                float sc[P], zc[P];
+#pragma unroll
+                for (int p = 0; p < P; p++) {
+                    const int at = (step % SPC) * XS + (ks * KB + b) * NG + g;
+                    sc[p] = scale[(p * NW + nw) * 16 + col][at];
+                    zc[p] = zero[(p * NW + nw) * 16 + col][at];
+                }
 #pragma unroll
                 for (int p = 0; p < P; p++)
 #pragma unroll
@@ -284,7 +312,7 @@ __global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
 #pragma unroll
                     for (int p = 0; p < P; p++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) d[p][i] = -zc[p][b][g] * xs[i];
+                        for (int i = 0; i < 4; i++) d[p][i] = -zc[p] * xs[i];
                     const uint8_t *from = lds + (t * 16 + col) * RS + (ks * KB + b) * 256;
 #pragma unroll
                     for (int i = 0; i < SP; i++)
@@ -297,7 +325,7 @@ __global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
 #pragma unroll
                     for (int p = 0; p < P; p++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) acc[p][t][i] = fmaf(sc[p][b][g], d[p][i], acc[p][t][i]);
+                        for (int i = 0; i < 4; i++) acc[p][t][i] = fmaf(sc[p], d[p][i], acc[p][t][i]);
                 }
             }
         }
@@ -346,15 +374,17 @@ __global__ __launch_bounds__(64 * NW * KS) void q4_tiles_kernel(Q4Args a) {
     }
 }
 
-template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB>
+template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB, int MW>
 hipError_t launch_tiles_of(const Q4Args &a, hipStream_t s) {
     constexpr int TM = 16 * MT, TN = NW * (UP ? 16 : 16 * P);
     int64_t tiles = ((int64_t)a.n_rows + TM - 1) / TM;
     if (a.mode == kQ4Sorted) tiles = a.n_rows / TM + (a.n_rows < a.w.n_mat ? a.n_rows : a.w.n_mat);
+    const int64_t nt = (a.w.rows + TN - 1) / TN, most = std::max<int64_t>(8, ((1 << 22) / nt) & ~7);  // tiles of a launch
     Q4Args part = a;
-    for (part.tile0 = 0; part.tile0 < tiles; part.tile0 += 65535) {  // what a grid's second dimension holds
-        const dim3 grid((a.w.rows + TN - 1) / TN, (unsigned)(tiles - part.tile0 < 65535 ? tiles - part.tile0 : 65535));
-        q4_tiles_kernel<T, G, UP, P, MT, NW, KS, KB><<<grid, 64 * NW * KS, 0, s>>>(part);
+    part.spread = tiles >= 32;
+    for (part.tile0 = 0; part.tile0 < tiles; part.tile0 += most) {
+        const int64_t now = std::min(most, tiles - part.tile0), grid = nt * (part.spread ? (now + 7) / 8 * 8 : now);
+        q4_tiles_kernel<T, G, UP, P, MT, NW, KS, KB, MW><<<(unsigned)grid, 64 * NW * KS, 0, s>>>(part);
         const hipError_t rc = hipGetLastError();
         if (rc != hipSuccess) return rc;
     }
@@ -365,9 +395,9 @@ template <typename T, int G, bool UP>
 hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
     constexpr bool WIDE = sizeof(T) == 4;  // three planes of x
     const int per = a.mode == kQ4Sorted ? (a.n_rows + a.w.n_mat - 1) / a.w.n_mat : a.n_rows;
-    if (per <= 16) return launch_tiles_of<T, G, UP, UP ? 2 : 1, 1, 1, WIDE ? 4 : 8, 1>(a, s);
-    if (per <= 24 || WIDE) return launch_tiles_of<T, G, UP, 2, 2, 4, 1, WIDE ? 1 : 2>(a, s);
-    return launch_tiles_of<T, G, UP, 2, 4, 4, 1, 2>(a, s);
+    if (per <= 16) return launch_tiles_of<T, G, UP, UP ? 2 : 1, 1, 1, WIDE ? 4 : 8, 1, 2>(a, s);
+    if (per <= 24 || WIDE) return launch_tiles_of<T, G, UP, 2, 2, 4, 1, WIDE ? 1 : 2, 2>(a, s);
+    return launch_tiles_of<T, G, UP, 2, 4, 4, 1, 1, 3>(a, s);
 }
 
 template <typename T>

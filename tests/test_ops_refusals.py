@@ -25,7 +25,7 @@ def refused(rc, code, *words):
     ("scales", None, H.ERR_INVALID, "null"), ("scales", A + 1, H.ERR_INVALID, "aligned"),
     ("rows", 0, H.ERR_INVALID, "rows"), ("rows", -4, H.ERR_INVALID, "rows"),
     ("cols", 0, H.ERR_INVALID, "cols"), ("cols", 192, H.ERR_INVALID, "cols"), ("cols", 100, H.ERR_INVALID, "cols"),
-    ("group", 16, H.ERR_UNSUPPORTED, "group"), ("group", 0, H.ERR_UNSUPPORTED, "group"),
+    ("cols", (1 << 20) + 128, H.ERR_UNSUPPORTED, "cols"), ("group", 16, H.ERR_UNSUPPORTED, "group"), ("group", 0, H.ERR_UNSUPPORTED, "group"),
     ("group", 256, H.ERR_UNSUPPORTED, "group"), ("n_mat", 0, H.ERR_INVALID, "n_mat"),
     ("scale_type", H.TYPE_Q4_K, H.ERR_UNSUPPORTED, "scale type")])
 @pytest.mark.parametrize("second", [False, True])
