@@ -46,6 +46,23 @@ __device__ __forceinline__ v4u biased(uint32_t codes) {
     return o;
 }
 
+// Codes in their own order, words {0, 1}, {2, 3}, {4, 5}, {6, 7}, for x that is not
+// rearranged: the code in the lowest fraction bits of kInOrderBias, so that a byte
+// permute and a masked or make a word.
+template <typename T>
+constexpr float kInOrderBias = __is_same(T, bf16) ? 128.0f : 1024.0f;
+template <typename T>
+__device__ __forceinline__ v4u in_order(uint32_t codes) {
+    uint32_t base = __is_same(T, bf16) ? 0x43004300u : 0x64006400u;
+    asm("" : "+v"(base));
+    const uint32_t high = codes >> 4;
+    v4u o;
+#pragma unroll
+    for (int j = 0; j < 4; j++)  // byte j of both into the two halves; the upper nibbles are masked off
+        o[j] = (__builtin_amdgcn_perm(high, codes, 0x0c040c00u + 0x00010001u * j) & 0x000f000fu) | base;
+    return o;
+}
+
 // Eight consecutive 16-bit values as words {0, 4}, {1, 5}, {2, 6}, {3, 7}.
 __device__ __forceinline__ v4u paired(v4u x) {
     v4u o;

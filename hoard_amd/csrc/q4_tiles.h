@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "lds_dma.h"
 #include "q4.h"
 
 namespace hoard {
@@ -374,21 +375,186 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
     }
 }
 
-template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB, int MW>
-hipError_t launch_tiles_of(const Q4Args &a, hipStream_t s) {
-    constexpr int TM = 16 * MT, TN = NW * (UP ? 16 : 16 * P);
+// The same product for 16-bit activations and many rows of x: x goes straight from
+// memory to LDS in its own order, the codes take that order (in_order), and the sums
+// of x come from a third product with a matrix of ones, whose accumulator holds them
+// where the scaled sums need them.  A step is 128 columns; x lies in two buffers, so
+// one barrier a step hands over what arrived and frees what was read.
+//
+// A row of x is 256 bytes of a buffer, its 16-byte pieces exchanged by the row's
+// number (piece ^ row % 16), so that 16 rows' pieces fall on all the banks.
+template <typename T, int G, bool UP, int MT, int NW, int MW>
+__global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
+    constexpr int TM = 16 * MT, THREADS = 64 * NW, P = 2, NG = 128 / G, SP = 4 / NG;
+    constexpr int CH = TM / 4 / NW;                        // copies of 1 KB a wave and step
+    constexpr int RW = 16 * NW * P, SC = 16, SPC = SC / NG, SI = RW * SC / THREADS;
+    constexpr int WIDE = UP ? 16 : 32;
+    static_assert(CH * NW * 4 == TM && SI * THREADS == RW * SC && SC % SI == 0, "whole shares");
+    __shared__ __align__(16) uint8_t lds[2][TM * 256];
+    __shared__ float scale[RW][SC + 1], zero[RW][SC + 1];
+
+    const int tid = threadIdx.x, lane = tid & 63, nw = wave_index(), col = lane & 15, q = lane >> 4;
+    int e, r0, rows, tn;
+    {
+        const int nt = (a.w.rows + NW * WIDE - 1) / (NW * WIDE), id = blockIdx.x, run = a.spread ? id >> 3 : id;
+        tn = run % nt;
+        if (!tile_of(a, a.tile0 + (a.spread ? (run / nt) * 8 + (id & 7) : run / nt), TM, e, r0, rows)) return;
+    }
+    const int cols = a.w.cols, groups = cols / G, steps = (cols + 127) / 128;
+    const int first = (tn * NW + nw) * WIDE, n0 = first + col, top = min(first, a.w.rows - 1);
+    const int last_block = (cols - 32 - q * 32) >= 0 ? (cols - 32 - q * 32) / 128 : 0;
+    const size_t row0 = (size_t)e * a.w.rows + top;
+    uint32_t code[P];
+#pragma unroll
+    for (int p = 0; p < P; p++)
+        code[p] = (min(n0 + (UP ? 0 : 16 * p), a.w.rows - 1) - top) * (cols / 2) + (q * 32 < cols ? q * 16 : 0);
+
+    v4u codes[2][P];
+    auto fetch_w = [&](auto at, int step) {
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
+            const uint8_t *const from = static_cast<const uint8_t *>(m.codes) + row0 * (cols / 2);
+            codes[decltype(at)::value][p] = *reinterpret_cast<const v4u *>(from + (code[p] + min(step, last_block) * 64));
+        }
+    };
+    // the wave's copies: lane l of a copy brings piece (l % 16) ^ row of row l / 16
+    const uint8_t *const x0 = static_cast<const uint8_t *>(a.x) + (size_t)r0 * cols * 2;
+    uint32_t src[CH];
+#pragma unroll
+    for (int j = 0; j < CH; j++) src[j] = (uint32_t)min((nw * CH + j) * 4 + q, rows - 1) * (uint32_t)cols * 2;
+    const int piece = col ^ q;  // of rows 0..3 of 16; rows 4 j on differ in bits 2 and 3
+    auto fetch_x = [&](int buffer, int step) {
+#pragma unroll
+        for (int j = 0; j < CH; j++)
+            if ((nw * CH + j) * 4 < rows)
+                dma_lanes_at(lds[buffer] + (nw * CH + j) * 1024, x0,
+                             src[j] + 2 * min(step * 128 + (piece ^ (((nw * CH + j) & 3) * 4)) * 8, cols - 8));
+    };
+    auto stage_scales = [&](int chunk) {
+        const int row = tid / (SC / SI), g0 = (tid % (SC / SI)) * SI, p = row / (16 * NW), in = row % (16 * NW);
+        const int n = tn * NW * WIDE + (UP ? in : (in / 16) * WIDE + p * 16 + in % 16);
+        const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
+        const size_t from = ((size_t)e * a.w.rows + min(n, a.w.rows - 1)) * groups;
+#pragma unroll
+        for (int g = 0; g < SI; g++) {
+            const int at = min(chunk * SC + g0 + g, groups - 1);
+            scale[row][g0 + g] = scale_of(m.scale_type, raw_scale(m, from, at));
+            zero[row][g0 + g] = kInOrderBias<T> + (m.zeros ? (float)m.zeros[from + at] : 8.0f);
+        }
+    };
+
+    v4f acc[P][MT];
+#pragma unroll
+    for (int p = 0; p < P; p++)
+#pragma unroll
+        for (int t = 0; t < MT; t++) acc[p][t] = (v4f)(0.0f);
+    const v4u ones = (v4u)(kOnes<T>);
+    auto body = [&](auto at, int step) {
+        constexpr int B = decltype(at)::value;
+        if (step % SPC == 0) {
+            if (step) __syncthreads();
+            stage_scales(step / SPC);
+        }
+        // this step's codes, and with them the copies of x issued before the next step's
+        // codes: what the compiler waits for here, and the wait by itself
+#pragma unroll
+        for (int p = 0; p < P; p++) asm volatile("" : "+v"(codes[B][p]));
+        if (step + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(P) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        v4u now[P];
+#pragma unroll
+        for (int p = 0; p < P; p++) now[p] = exchange<G>(codes[B][p]);
+        if (step + 1 < steps) fetch_x(B ^ 1, step + 1);
+        if (step + 2 < steps) fetch_w(at, step + 2);
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            if (step * 128 + g * G >= cols) break;  // a group lies inside or behind the last column as a whole
+            v4u w[P][SP];
+            float sc[P], zc[P];
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                sc[p] = scale[(p * NW + nw) * 16 + col][(step % SPC) * NG + g];
+                zc[p] = zero[(p * NW + nw) * 16 + col][(step % SPC) * NG + g];
+#pragma unroll
+                for (int i = 0; i < SP; i++) w[p][i] = in_order<T>(now[p][g * SP + i]);
+            }
+#pragma unroll
+            for (int t = 0; t < MT; t++) {
+                if (t * 16 >= rows) break;
+                v4f d[P] = {}, xs = (v4f)(0.0f);
+                const uint8_t *from = lds[B] + (t * 16 + col) * 256;
+#pragma unroll
+                for (int i = 0; i < SP; i++) {
+                    const v4u x = *reinterpret_cast<const v4u *>(from + (((column_of<G>(g * SP + i, q) / 8) ^ col) * 16));
+                    xs = mfma_16x16x32<T>(x, ones, xs);
+#pragma unroll
+                    for (int p = 0; p < P; p++) d[p] = mfma_16x16x32<T>(x, w[p][i], d[p]);
+                }
+#pragma unroll
+                for (int p = 0; p < P; p++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        acc[p][t][i] = fmaf(sc[p], fmaf(-zc[p], xs[i], d[p][i]), acc[p][t][i]);
+            }
+        }
+    };
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> odd{};
+    fetch_w(even, 0);
+    fetch_x(0, 0);
+    if (steps > 1) fetch_w(odd, 1);
+    for (int step = 0; step < steps; step += 2) {
+        body(even, step);
+        if (step + 1 < steps) body(odd, step + 1);
+    }
+    T *y = static_cast<T *>(a.y) + (size_t)r0 * a.w.rows;
+#pragma unroll
+    for (int p = 0; p < (UP ? 1 : P); p++) {
+        const int n = n0 + 16 * p;
+        if (n >= a.w.rows) continue;
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = t * 16 + 4 * q + i;
+                if (row >= rows) continue;
+                float v = acc[p][t][i];
+                if constexpr (UP) v = silu_mul(v, acc[1][t][i]);
+                y[(size_t)row * a.w.rows + n] = (T)v;
+            }
+    }
+}
+
+// f(tile, grid) over the launches that cover the call's tiles.
+template <int TM, int TN, typename F>
+hipError_t over_tiles(const Q4Args &a, F launch) {
     int64_t tiles = ((int64_t)a.n_rows + TM - 1) / TM;
     if (a.mode == kQ4Sorted) tiles = a.n_rows / TM + (a.n_rows < a.w.n_mat ? a.n_rows : a.w.n_mat);
     const int64_t nt = (a.w.rows + TN - 1) / TN, most = std::max<int64_t>(8, ((1 << 22) / nt) & ~7);  // tiles of a launch
     Q4Args part = a;
     part.spread = tiles >= 32;
     for (part.tile0 = 0; part.tile0 < tiles; part.tile0 += most) {
-        const int64_t now = std::min(most, tiles - part.tile0), grid = nt * (part.spread ? (now + 7) / 8 * 8 : now);
-        q4_tiles_kernel<T, G, UP, P, MT, NW, KS, KB, MW><<<(unsigned)grid, 64 * NW * KS, 0, s>>>(part);
+        const int64_t now = std::min(most, tiles - part.tile0);
+        launch(part, (unsigned)(nt * (part.spread ? (now + 7) / 8 * 8 : now)));
         const hipError_t rc = hipGetLastError();
         if (rc != hipSuccess) return rc;
     }
     return hipSuccess;
+}
+
+template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB, int MW>
+hipError_t launch_tiles_of(const Q4Args &a, hipStream_t s) {
+    return over_tiles<16 * MT, NW *(UP ? 16 : 16 * P)>(a, [&](const Q4Args &part, unsigned grid) {
+        q4_tiles_kernel<T, G, UP, P, MT, NW, KS, KB, MW><<<grid, 64 * NW * KS, 0, s>>>(part);
+    });
+}
+template <typename T, int G, bool UP, int MT, int NW, int MW>
+hipError_t launch_flow_of(const Q4Args &a, hipStream_t s) {
+    return over_tiles<16 * MT, NW *(UP ? 16 : 32)>(a, [&](const Q4Args &part, unsigned grid) {
+        q4_flow_kernel<T, G, UP, MT, NW, MW><<<grid, 64 * NW, 0, s>>>(part);
+    });
 }
 
 template <typename T, int G, bool UP>
@@ -396,8 +562,12 @@ hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
     constexpr bool WIDE = sizeof(T) == 4;  // three planes of x
     const int per = a.mode == kQ4Sorted ? (a.n_rows + a.w.n_mat - 1) / a.w.n_mat : a.n_rows;
     if (per <= 16) return launch_tiles_of<T, G, UP, UP ? 2 : 1, 1, 1, WIDE ? 4 : 8, 1, 2>(a, s);
-    if (per <= 24 || WIDE) return launch_tiles_of<T, G, UP, 2, 2, 4, 1, WIDE ? 1 : 2, 2>(a, s);
-    return launch_tiles_of<T, G, UP, 2, 4, 4, 1, 1, 3>(a, s);
+    if constexpr (WIDE) {
+        return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 1, 2>(a, s);
+    } else {
+        if (per <= 24) return launch_flow_of<T, G, UP, 2, 4, 3>(a, s);
+        return launch_flow_of<T, G, UP, 4, 4, 3>(a, s);
+    }
 }
 
 template <typename T>
