@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256) void q4_rows_kernel(Q4Args a, int lanes_log) {
                     if (lk == j) mine[p] = v;
                 }
             if (lk < NR && n0 + lk < a.w.rows && r0 + r < a.n_rows) {
-                float v = UP ? silu_mul(mine[0], mine[P - 1]) : mine[0];
+                float v = UP ? silu_mul<T>(mine[0], mine[P - 1]) : mine[0];
                 if (e < 0) v = __builtin_nanf("");
                 static_cast<T *>(a.y)[(size_t)(r0 + r) * a.w.rows + n0 + lk] = (T)v;
             }

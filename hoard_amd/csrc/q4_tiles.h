@@ -77,6 +77,28 @@ __device__ __forceinline__ int column_of(int step, int q) {
     return q * 32 + step * 8;
 }
 
+// N scales of a row from index `from` on, and its zero points plus `bias`, into LDS.
+template <int N>
+__device__ __forceinline__ void load_scales(const hoard_q4_matrix &m, size_t from, float *scale, float *zero, float bias) {
+    if (m.scale_type == HOARD_TYPE_F32) {
+        float v[N];
+        __builtin_memcpy(v, static_cast<const float *>(m.scales) + from, sizeof v);
+#pragma unroll
+        for (int g = 0; g < N; g++) scale[g] = v[g];
+    } else {
+        uint16_t v[N];
+        __builtin_memcpy(v, static_cast<const uint16_t *>(m.scales) + from, sizeof v);
+        const bool half = m.scale_type == HOARD_TYPE_F16;
+#pragma unroll
+        for (int g = 0; g < N; g++)
+            scale[g] = half ? (float)__builtin_bit_cast(f16, v[g]) : __uint_as_float((uint32_t)v[g] << 16);
+    }
+    uint8_t z[N];
+    if (m.zeros) __builtin_memcpy(z, m.zeros + from, sizeof z);
+#pragma unroll
+    for (int g = 0; g < N; g++) zero[g] = bias + (m.zeros ? (float)z[g] : 8.0f);
+}
+
 // Eight values of a row of x as they are fetched.
 template <typename T>
 struct Piece {
@@ -96,33 +118,41 @@ __device__ __forceinline__ bool tile_of(const Q4Args &a, int64_t t, int tm, int 
     }
     const int lane = threadIdx.x & 63, n = a.w.n_mat, per = (n + 63) / 64, e0 = lane * per, e1 = min(n, e0 + per);
     auto at = [&](int i) { return max(0, min(a.n_rows, a.sel[i])); };
-    int mine = 0;
+    // whole tiles and the rest of a matrix's rows: the whole ones of all matrices come
+    // first, so that the launch does not end on the longest work
+    int whole = 0, rest = 0;
     if (e0 < e1) {
         int lo = at(e0);
         for (int i = e0; i < e1; i++) {
-            const int hi = at(i + 1);
-            mine += max(0, hi - lo + tm - 1) / tm;
+            const int hi = at(i + 1), c = max(0, hi - lo);
+            whole += c / tm;
+            rest += c % tm != 0;
             lo = hi;
         }
     }
-    int incl = mine;
+    int incl_w = whole, incl_r = rest;
     for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(incl, d);
-        if (lane >= d) incl += v;
+        const int v = __shfl_up(incl_w, d), u = __shfl_up(incl_r, d);
+        if (lane >= d) incl_w += v, incl_r += u;
     }
+    const int all = __builtin_amdgcn_readlane(incl_w, 63);
+    const bool first = t < all;
+    if (!first) t -= all;
+    const int incl = first ? incl_w : incl_r, mine = first ? whole : rest;
     const uint64_t past = __ballot(incl > t);
     if (!past) return false;
     const int who = __ffsll((unsigned long long)past) - 1;
     int left = (int)t - __builtin_amdgcn_readlane(incl - mine, who), lo = 0, hi = 0;
     for (e = who * per;; e++) {  // ends at the matrix whose tile it is, within the lane's run
         lo = at(e);
-        hi = at(e + 1);
-        const int tiles = max(0, hi - lo + tm - 1) / tm;
+        hi = max(lo, at(e + 1));
+        const int tiles = first ? (hi - lo) / tm : (hi - lo) % tm != 0;
         if (left < tiles || e + 1 >= n) break;
         left -= tiles;
     }
+    const int from = first ? left * tm : (hi - lo) / tm * tm;
     e = __builtin_amdgcn_readfirstlane(e);
-    r0 = __builtin_amdgcn_readfirstlane(lo + left * tm);
+    r0 = __builtin_amdgcn_readfirstlane(lo + from);
     rows = __builtin_amdgcn_readfirstlane(min(tm, hi - r0));
     return rows > 0;
 }
@@ -202,11 +232,13 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
         const int n = tn * NW * WIDE + (UP ? in : (in / 16) * WIDE + p * 16 + in % 16);
         const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
         const size_t from = ((size_t)e * a.w.rows + min(n, a.w.rows - 1)) * groups;
+        const int g1 = chunk * SC + g0;
+        if (g1 + SI <= groups) {
+            load_scales<SI>(m, from + g1, scale[row] + g0, zero[row] + g0, 16.0f);
+        } else {
 #pragma unroll
-        for (int g = 0; g < SI; g++) {
-            const int at = min(chunk * SC + g0 + g, groups - 1);
-            scale[row][g0 + g] = scale_of(m.scale_type, raw_scale(m, from, at));
-            zero[row][g0 + g] = m.zeros ? 16.0f + (float)m.zeros[from + at] : 24.0f;
+            for (int g = 0; g < SI; g++)
+                load_scales<1>(m, from + min(g1 + g, groups - 1), scale[row] + g0 + g, zero[row] + g0 + g, 16.0f);
         }
     };
     const int xrow = tid / (COLS / 8), xcol = (tid % (COLS / 8)) * 8;
@@ -369,7 +401,7 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
                 const int row = t * 16 + 4 * q + i;
                 if (row >= rows) continue;
                 float v = acc[p][t][i];
-                if constexpr (UP) v = silu_mul(v, acc[1][t][i]);
+                if constexpr (UP) v = silu_mul<T>(v, acc[1][t][i]);
                 y[(size_t)row * a.w.rows + n] = (T)v;
             }
     }
@@ -383,11 +415,11 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
 //
 // A row of x is 256 bytes of a buffer, its 16-byte pieces exchanged by the row's
 // number (piece ^ row % 16), so that 16 rows' pieces fall on all the banks.
-template <typename T, int G, bool UP, int MT, int NW, int MW>
+template <typename T, int G, bool UP, int MT, int NW, int SC, int MW>
 __global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
     constexpr int TM = 16 * MT, THREADS = 64 * NW, P = 2, NG = 128 / G, SP = 4 / NG;
     constexpr int CH = TM / 4 / NW;                        // copies of 1 KB a wave and step
-    constexpr int RW = 16 * NW * P, SC = 16, SPC = SC / NG, SI = RW * SC / THREADS;
+    constexpr int RW = 16 * NW * P, SPC = SC / NG, SI = RW * SC / THREADS;
     constexpr int WIDE = UP ? 16 : 32;
     static_assert(CH * NW * 4 == TM && SI * THREADS == RW * SC && SC % SI == 0, "whole shares");
     __shared__ __align__(16) uint8_t lds[2][TM * 256];
@@ -436,11 +468,13 @@ __global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
         const int n = tn * NW * WIDE + (UP ? in : (in / 16) * WIDE + p * 16 + in % 16);
         const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
         const size_t from = ((size_t)e * a.w.rows + min(n, a.w.rows - 1)) * groups;
+        const int g1 = chunk * SC + g0;
+        if (g1 + SI <= groups) {
+            load_scales<SI>(m, from + g1, scale[row] + g0, zero[row] + g0, kInOrderBias<T>);
+        } else {
 #pragma unroll
-        for (int g = 0; g < SI; g++) {
-            const int at = min(chunk * SC + g0 + g, groups - 1);
-            scale[row][g0 + g] = scale_of(m.scale_type, raw_scale(m, from, at));
-            zero[row][g0 + g] = kInOrderBias<T> + (m.zeros ? (float)m.zeros[from + at] : 8.0f);
+            for (int g = 0; g < SI; g++)
+                load_scales<1>(m, from + min(g1 + g, groups - 1), scale[row] + g0 + g, zero[row] + g0 + g, kInOrderBias<T>);
         }
     };
 
@@ -521,7 +555,7 @@ __global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
                 const int row = t * 16 + 4 * q + i;
                 if (row >= rows) continue;
                 float v = acc[p][t][i];
-                if constexpr (UP) v = silu_mul(v, acc[1][t][i]);
+                if constexpr (UP) v = silu_mul<T>(v, acc[1][t][i]);
                 y[(size_t)row * a.w.rows + n] = (T)v;
             }
     }
@@ -550,10 +584,10 @@ hipError_t launch_tiles_of(const Q4Args &a, hipStream_t s) {
         q4_tiles_kernel<T, G, UP, P, MT, NW, KS, KB, MW><<<grid, 64 * NW * KS, 0, s>>>(part);
     });
 }
-template <typename T, int G, bool UP, int MT, int NW, int MW>
+template <typename T, int G, bool UP, int MT, int NW, int SC, int MW>
 hipError_t launch_flow_of(const Q4Args &a, hipStream_t s) {
     return over_tiles<16 * MT, NW *(UP ? 16 : 32)>(a, [&](const Q4Args &part, unsigned grid) {
-        q4_flow_kernel<T, G, UP, MT, NW, MW><<<grid, 64 * NW, 0, s>>>(part);
+        q4_flow_kernel<T, G, UP, MT, NW, SC, MW><<<grid, 64 * NW, 0, s>>>(part);
     });
 }
 
@@ -565,8 +599,8 @@ hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
     if constexpr (WIDE) {
         return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 1, 2>(a, s);
     } else {
-        if (per <= 24) return launch_flow_of<T, G, UP, 2, 4, 3>(a, s);
-        return launch_flow_of<T, G, UP, 4, 4, 3>(a, s);
+        if (per <= 24) return launch_flow_of<T, G, UP, 2, 4, 16, 3>(a, s);
+        return launch_flow_of<T, G, UP, 4, 4, 16, 3>(a, s);
     }
 }
 
