@@ -54,7 +54,9 @@ __global__ __launch_bounds__(kBlockPairs) void place_kernel(PairsArgs a, int64_t
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = a.n_expert, blocks = gridDim.x;
     const int64_t p = (int64_t)blockIdx.x * kBlockPairs + tid;
     const int key = key_of(a, p, pairs);
-    for (int i = tid; i < kWaves * (kMaxExperts + 1); i += kBlockPairs) (&of_wave[0][0])[i] = 0;
+    for (int e = tid; e <= E; e += kBlockPairs)
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) of_wave[w][e] = 0;
     __syncthreads();
     const uint64_t same = same_key(key, bits), before = same & ((1ull << lane) - 1ull);
     const int rank = __popcll(before);
@@ -71,6 +73,7 @@ __global__ __launch_bounds__(kBlockPairs) void place_kernel(PairsArgs a, int64_t
         if (blocks == 1) {
             total = mine;
         } else {
+#pragma unroll 8
             for (int b = 0; b < blocks; b++) {
                 const int c = a.work[(size_t)b * E + tid];
                 if (b < (int)blockIdx.x) earlier += c;
@@ -110,12 +113,31 @@ __global__ __launch_bounds__(kBlockPairs) void place_kernel(PairsArgs a, int64_t
 
 // -- rows ---------------------------------------------------------------------
 
-// An item is 8 columns of a token; a wave's items are consecutive.
+// Gather and combine are bound by memory: an item is 8 columns of a token, a wave's
+// items are consecutive, and an item's places and rows are fetched kAhead slots at a
+// time, so that their latencies overlap.
+constexpr int kAhead = 8;
+
 __device__ __forceinline__ bool item_of(const RowsArgs &a, int64_t i, int per_row, int64_t &t, int &at, int &some) {
     t = i / per_row;
     at = (int)(i - t * per_row) * 8;
     some = min(8, a.n - at);
     return t < a.n_tokens;
+}
+// The sorted rows of slots j0 .. j0 + kAhead - 1 of token t, -1 for a dropped pair.
+__device__ __forceinline__ void rows_of(const RowsArgs &a, int64_t t, int j0, int64_t pairs, int row[kAhead],
+                                        float w[kAhead]) {
+    const int32_t *const place = a.place + t * a.k;
+    const float *const weight = a.w + t * a.k;
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+        const int j = min(j0 + u, a.k - 1);
+        row[u] = place[j];
+        w[u] = a.w ? weight[j] : 1.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; u++)
+        if (j0 + u >= a.k || row[u] >= pairs) row[u] = -1;
 }
 
 template <typename T>
@@ -126,15 +148,18 @@ __global__ __launch_bounds__(256) void gather_kernel(RowsArgs a) {
         int64_t t;
         int at, some;
         if (!item_of(a, i, per_row, t, at, some)) return;
-        float x[8], o[8];
+        float x[8], o[8], w[kAhead];
+        int row[kAhead];
         load_some(static_cast<const T *>(a.x) + t * a.n + at, some, x);
-        for (int j = 0; j < a.k; j++) {
-            const int row = a.place[t * a.k + j];
-            if (row < 0 || row >= pairs) continue;
-            const float w = a.w ? a.w[t * a.k + j] : 1.0f;
+        for (int j = 0; j < a.k; j += kAhead) {
+            rows_of(a, t, j, pairs, row, w);
 #pragma unroll
-            for (int c = 0; c < 8; c++) o[c] = a.w ? w * x[c] : x[c];
-            store_some(static_cast<T *>(a.out) + (int64_t)row * a.n + at, some, o);
+            for (int u = 0; u < kAhead; u++) {
+                if (row[u] < 0) continue;
+#pragma unroll
+                for (int c = 0; c < 8; c++) o[c] = a.w ? w[u] * x[c] : x[c];
+                store_some(static_cast<T *>(a.out) + (int64_t)row[u] * a.n + at, some, o);
+            }
         }
     }
 }
@@ -147,46 +172,76 @@ __global__ __launch_bounds__(256) void combine_kernel(RowsArgs a) {
         int64_t t;
         int at, some;
         if (!item_of(a, i, per_row, t, at, some)) return;
-        float s[8] = {}, y[8];
+        float s[8] = {}, w[kAhead];
+        int row[kAhead];
         if (a.res) load_some(static_cast<const T *>(a.res) + t * a.n + at, some, s);
-        for (int j = 0; j < a.k; j++) {
-            const int row = a.place[t * a.k + j];
-            if (row < 0 || row >= pairs) continue;
-            const float w = a.w ? a.w[t * a.k + j] : 1.0f;
-            load_some(static_cast<const T *>(a.x) + (int64_t)row * a.n + at, some, y);
+        for (int j = 0; j < a.k; j += kAhead) {
+            rows_of(a, t, j, pairs, row, w);
+            float y[kAhead][8];
 #pragma unroll
-            for (int c = 0; c < 8; c++) s[c] = fmaf(w, y[c], s[c]);
+            for (int u = 0; u < kAhead; u++)
+                if (row[u] >= 0) load_some(static_cast<const T *>(a.x) + (int64_t)row[u] * a.n + at, some, y[u]);
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) {
+                if (row[u] < 0) continue;
+#pragma unroll
+                for (int c = 0; c < 8; c++) s[c] = fmaf(w[u], y[u][c], s[c]);
+            }
         }
         store_some(static_cast<T *>(a.out) + t * a.n + at, some, s);
     }
 }
 
-// A wave takes a pair.
+// A wave takes a pair, kChunks * 512 columns at a time; ROUND: n is a multiple of 8.
+constexpr int kChunks = 4;
+template <typename T, bool ROUND>
+__device__ __forceinline__ float grad_row(const T *d, const T *y, T *dy, float w, int n) {
+    const int lane = threadIdx.x & 63;
+    float s = 0.0f;
+    for (int at0 = lane * 8; at0 < n; at0 += kChunks * 512) {
+        float dv[kChunks][8], yv[kChunks][8];
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            const int at = at0 + c * 512;
+            if (ROUND) {  // behind the end: the last columns again, without weight
+                load8(d + min(at, n - 8), dv[c]);
+                load8(y + min(at, n - 8), yv[c]);
+            } else {
+                load_some(d + at, n - at, dv[c]);
+                load_some(y + at, n - at, yv[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            const int at = at0 + c * 512;
+            if (ROUND && at >= n) continue;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                s = fmaf(dv[c][i], yv[c][i], s);
+                dv[c][i] *= w;
+            }
+            if (!dy) continue;
+            if (ROUND) store8(dy + at, dv[c]);
+            else store_some(dy + at, n - at, dv[c]);
+        }
+    }
+    return s;
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void combine_grad_kernel(RowsArgs a) {
     const int64_t pairs = (int64_t)a.n_tokens * a.k;
-    const int lane = threadIdx.x & 63;
     for (int64_t p = (int64_t)blockIdx.x * 4 + wave_index(); p < pairs; p += (int64_t)gridDim.x * 4) {
         const int row = a.place[p];
         float s = 0.0f;
         if (row >= 0 && row < pairs) {
-            const int64_t t = p / a.k;
-            const float w = a.w[p];
-            for (int at = lane * 8; at < a.n; at += 512) {
-                const int some = min(8, a.n - at);
-                float d[8], y[8];
-                load_some(static_cast<const T *>(a.res) + t * a.n + at, some, d);
-                load_some(static_cast<const T *>(a.x) + (int64_t)row * a.n + at, some, y);
-#pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    s = fmaf(d[c], y[c], s);
-                    d[c] *= w;
-                }
-                if (a.out) store_some(static_cast<T *>(a.out) + (int64_t)row * a.n + at, some, d);
-            }
+            const T *const d = static_cast<const T *>(a.res) + p / a.k * a.n;
+            const T *const y = static_cast<const T *>(a.x) + (int64_t)row * a.n;
+            T *const dy = a.out ? static_cast<T *>(a.out) + (int64_t)row * a.n : nullptr;
+            s = a.n % 8 == 0 ? grad_row<T, true>(d, y, dy, a.w[p], a.n) : grad_row<T, false>(d, y, dy, a.w[p], a.n);
         }
         s = wave_sum_f(s);
-        if (lane == 0) a.dw[p] = s;
+        if ((threadIdx.x & 63) == 0) a.dw[p] = s;
     }
 }
 
