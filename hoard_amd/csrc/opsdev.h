@@ -12,37 +12,48 @@ namespace hoard {
 typedef _Float16 f16;
 typedef __bf16 bf16;
 
-// Eight values of T at p as floats.  p is aligned to T only: gfx950 loads 16
-// bytes from any address, so rows of an odd length take the same path.
-template <typename T>
-struct Pack8 {
-    T v[8];
-};
-template <typename T>
+// Sixteen bytes at any 2-byte aligned address: gfx950 loads and stores them from
+// there, so rows of an odd length take the same path.
+typedef uint32_t u128 __attribute__((ext_vector_type(4), aligned(2)));
+
+// Eight values of T at p as floats.  NT: with the non-temporal policy, for what is
+// read or written once and would only push other data out of the caches.
+template <bool NT = false, typename T>
 __device__ __forceinline__ void load8(const T *p, float o[8]) {
-    Pack8<T> t;
-    __builtin_memcpy(&t, p, sizeof t);
+    T v[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = (float)t.v[i];
+    for (int i = 0; i < (int)sizeof v / 16; i++) {
+        const u128 *from = reinterpret_cast<const u128 *>(p) + i;
+        const u128 w = NT ? __builtin_nontemporal_load(from) : *from;
+        __builtin_memcpy(reinterpret_cast<char *>(v) + 16 * i, &w, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = (float)v[i];
 }
 // Stored values are rounded to nearest, ties to even, once.
-template <typename T>
+template <bool NT = false, typename T>
 __device__ __forceinline__ void store8(T *p, const float o[8]) {
-    Pack8<T> t;
+    T v[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) t.v[i] = (T)o[i];
-    __builtin_memcpy(p, &t, sizeof t);
+    for (int i = 0; i < 8; i++) v[i] = (T)o[i];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof v / 16; i++) {
+        u128 w, *to = reinterpret_cast<u128 *>(p) + i;
+        __builtin_memcpy(&w, reinterpret_cast<const char *>(v) + 16 * i, 16);
+        if (NT) __builtin_nontemporal_store(w, to);
+        else *to = w;
+    }
 }
 // The first `some` of them; the rest of o is zero.
-template <typename T>
+template <bool NT = false, typename T>
 __device__ __forceinline__ void load_some(const T *p, int some, float o[8]) {
-    if (some >= 8) return load8(p, o);
+    if (some >= 8) return load8<NT>(p, o);
 #pragma unroll
     for (int i = 0; i < 8; i++) o[i] = i < some ? (float)p[i] : 0.0f;
 }
-template <typename T>
+template <bool NT = false, typename T>
 __device__ __forceinline__ void store_some(T *p, int some, const float o[8]) {
-    if (some >= 8) return store8(p, o);
+    if (some >= 8) return store8<NT>(p, o);
 #pragma unroll
     for (int i = 0; i < 8; i++)
         if (i < some) p[i] = (T)o[i];
