@@ -21,82 +21,127 @@ namespace {
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
 
-// The gate of eight values as it is stored.
+// The gate of eight columns as it is stored: 32-bit values of a channel gate, those of
+// a full one, or the row's in the first word.
+struct Gate {
+    u128 w[2];
+};
 template <typename T>
-__device__ __forceinline__ void load_gate(const hoard_norm_args &a, size_t row, int at, int some, float g[8]) {
+__device__ __forceinline__ Gate fetch_gate(const hoard_norm_args &a, size_t row, Cols c) {
+    Gate g;
     if (a.gate_kind == HOARD_GATE_CHANNEL) {
-        load_some(static_cast<const float *>(a.gate) + at, some, g);
+        const Raw<float> r = fetch(static_cast<const float *>(a.gate), c, a.n);
+        __builtin_memcpy(&g, &r, sizeof r);
     } else if (a.gate_kind == HOARD_GATE_FULL) {
-        load_some(static_cast<const T *>(a.gate) + row * a.n + at, some, g);
+        const Raw<T> r = fetch(static_cast<const T *>(a.gate) + row * a.n, c, a.n);
+        __builtin_memcpy(&g, &r, sizeof r);
     } else {
-        const float t = a.gate_kind == HOARD_GATE_TOKEN ? static_cast<const float *>(a.gate)[row] : 1.0f;
+        g.w[0][0] = static_cast<const uint32_t *>(a.gate)[row];
+    }
+    return g;
+}
+template <typename T>
+__device__ __forceinline__ void gate_of(const hoard_norm_args &a, const Gate &g, float o[8]) {
+    if (a.gate_kind == HOARD_GATE_CHANNEL) {
+        Raw<float> r;
+        __builtin_memcpy(&r, &g, sizeof r);
+        widen(r, o);
+    } else if (a.gate_kind == HOARD_GATE_FULL) {
+        Raw<T> r;
+        __builtin_memcpy(&r, &g, sizeof r);
+        widen(r, o);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) g[i] = t;
+        for (int i = 0; i < 8; i++) o[i] = __uint_as_float(g.w[0][0]);
     }
 }
 
 // A workgroup of BS threads takes a row at a time; NV chunks of BS * 8 values cover it.
+// Everything that the row needs is fetched before the first sum, but in workgroups of
+// 1024, whose 128 registers do not hold it: there the gate and the weights come late.
 template <typename T, typename R, int BS, int NV>
 __global__ __launch_bounds__(BS) void norm_kernel(hoard_norm_args a) {
+    constexpr bool EARLY = BS <= 256;
     __shared__ float part[2][2][BS / 64];
     const float inv_n = 1.0f / (float)a.n;
-    int at[NV], some[NV];
+    Cols c[NV];
 #pragma unroll
-    for (int c = 0; c < NV; c++) {
-        at[c] = (c * BS + (int)threadIdx.x) * 8;
-        some[c] = max(0, min(8, a.n - at[c]));
-    }
+    for (int k = 0; k < NV; k++) c[k] = cols_of((k * BS + (int)threadIdx.x) * 8, a.n);
     int turn = 0;
     for (size_t row = blockIdx.x; row < (size_t)a.n_rows; row += gridDim.x, turn ^= 1) {
         const size_t base = row * a.n;
-        float v[NV][8], b[NV][8];
+        Raw<R> r[NV];
+        Raw<T> br[NV];
+        Raw<float> wp[NV], wq[NV];
+        Gate gate[NV];
 #pragma unroll
-        for (int c = 0; c < NV; c++) {
-            load_some(static_cast<const R *>(a.r) + base + at[c], some[c], v[c]);
-            if (a.b) load_some(static_cast<const T *>(a.b) + base + at[c], some[c], b[c]);
+        for (int k = 0; k < NV; k++) {
+            if (a.b) br[k] = fetch(static_cast<const T *>(a.b) + base, c[k], a.n);
+            r[k] = fetch(static_cast<const R *>(a.r) + base, c[k], a.n);
         }
-        float rho_b = 1.0f, rho_v = 1.0f;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            if (EARLY && a.w_post) wp[k] = fetch(a.w_post, c[k], a.n);
+            if (EARLY && a.gate) gate[k] = fetch_gate<T>(a, row, c[k]);
+            if (EARLY && a.h) wq[k] = fetch(a.w_pre, c[k], a.n);
+        }
+        float rho_b = 1.0f, rho_v = 1.0f, v[NV][8];
         if (a.b) {
             if (a.w_post) {
                 float s = 0.0f;
 #pragma unroll
-                for (int c = 0; c < NV; c++)
+                for (int k = 0; k < NV; k++) {
+                    float b[8];
+                    widen(br[k], b);
+                    mask_cols(c[k], b);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) s = fmaf(b[c][i], b[c][i], s);
+                    for (int i = 0; i < 8; i++) s = fmaf(b[i], b[i], s);
+                }
                 s = group_sum<BS / 64>(s, part[turn][0]);
                 rho_b = 1.0f / sqrtf(fmaf(s, inv_n, a.eps));
             }
 #pragma unroll
-            for (int c = 0; c < NV; c++) {
-                float g[8], w[8] = {};
-                load_gate<T>(a, row, at[c], some[c], g);
-                if (a.w_post) load_some(a.w_post + at[c], some[c], w);
+            for (int k = 0; k < NV; k++) {
+                float b[8], g[8], w[8];
+                widen(r[k], v[k]);
+                widen(br[k], b);
+                if (a.w_post) {
+                    widen(EARLY ? wp[k] : fetch(a.w_post, c[k], a.n), w);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (a.gate_sigmoid) g[i] = sigmoid(g[i]);
-                    const float cc = a.w_post ? b[c][i] * rho_b * (a.w_offset + w[i]) : b[c][i];
-                    // rounded here: the norm that follows is the stored stream's, as whoever reads it
-                    // (the gradient, the next layer) sees it
-                    v[c][i] = i < some[c] ? (float)(R)fmaf(a.scale * g[i], cc, v[c][i]) : 0.0f;
+                    for (int i = 0; i < 8; i++) b[i] = b[i] * rho_b * (a.w_offset + w[i]);
                 }
-                store_some(static_cast<R *>(a.r_out) + base + at[c], some[c], v[c]);
+                if (a.gate) {
+                    gate_of<T>(a, EARLY ? gate[k] : fetch_gate<T>(a, row, c[k]), g);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) g[i] = a.scale * (a.gate_sigmoid ? sigmoid(g[i]) : g[i]);
+                }
+                // rounded here: the norm that follows is the stored stream's, as whoever reads it
+                // (the gradient, the next layer) sees it
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[k][i] = (float)(R)fmaf(a.gate ? g[i] : a.scale, b[i], v[k][i]);
+                if (c[k].lo < 8) put(static_cast<R *>(a.r_out) + base, c[k], a.n, v[k]);
             }
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; k++) widen(r[k], v[k]);
         }
         if (a.h) {
             float s = 0.0f;
 #pragma unroll
-            for (int c = 0; c < NV; c++)
+            for (int k = 0; k < NV; k++) {
+                mask_cols(c[k], v[k]);
 #pragma unroll
-                for (int i = 0; i < 8; i++) s = fmaf(v[c][i], v[c][i], s);
+                for (int i = 0; i < 8; i++) s = fmaf(v[k][i], v[k][i], s);
+            }
             s = group_sum<BS / 64>(s, part[turn][1]);
             rho_v = 1.0f / sqrtf(fmaf(s, inv_n, a.eps));
 #pragma unroll
-            for (int c = 0; c < NV; c++) {
+            for (int k = 0; k < NV; k++) {
                 float w[8];
-                load_some(a.w_pre + at[c], some[c], w);
+                widen(EARLY ? wq[k] : fetch(a.w_pre, c[k], a.n), w);
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = v[c][i] * rho_v * (a.w_offset + w[i]);
-                store_some(static_cast<T *>(a.h) + base + at[c], some[c], w);
+                for (int i = 0; i < 8; i++) w[i] = v[k][i] * rho_v * (a.w_offset + w[i]);
+                if (c[k].lo < 8) put(static_cast<T *>(a.h) + base, c[k], a.n, w);
             }
         }
         if (a.stats && threadIdx.x == 0) {
@@ -106,115 +151,171 @@ __global__ __launch_bounds__(BS) void norm_kernel(hoard_norm_args a) {
     }
 }
 
+// A row's inputs of the backward pass.
+template <typename T, typename R, int NV>
+struct GradIn {
+    Raw<R> v[NV], dr[NV];
+    Raw<T> dh[NV], b[NV];
+    Gate gate[NV];
+    float rho_b, rho_v;
+};
+
 // Group blockIdx.x takes the rows blockIdx.x, + gridDim.x, ...: the sums over its
 // rows stay in registers and go to its rows of the workspace, one per wanted
-// parameter ([parameter][group][n]).
+// parameter ([parameter][group][n]).  Where the registers hold them (AHEAD) the next
+// row's inputs are fetched before this row's sums, whose two barriers would leave the
+// memory idle, and the weights stay.
 template <typename T, typename R, int BS, int NV>
 __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_norm_grads g, float *work) {
+    constexpr bool AHEAD = BS <= 256 && NV * (2 * sizeof(R) + 2 * sizeof(T)) <= 16;
     __shared__ float part[2][3][BS / 64];
     const float inv_n = 1.0f / (float)a.n;
     float s_pre[NV][8] = {}, s_post[NV][8] = {}, s_gate[NV][8] = {};
-    int at[NV], some[NV];
+    Cols c[NV];
+    Raw<float> wp[NV], wq[NV];
+    auto fetch_weights = [&]() {
 #pragma unroll
-    for (int c = 0; c < NV; c++) {
-        at[c] = (c * BS + (int)threadIdx.x) * 8;
-        some[c] = max(0, min(8, a.n - at[c]));
-    }
+        for (int k = 0; k < NV; k++) {
+            if (a.w_post) wp[k] = fetch(a.w_post, c[k], a.n);
+            if (g.dh) wq[k] = fetch(a.w_pre, c[k], a.n);
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < NV; k++) c[k] = cols_of((k * BS + (int)threadIdx.x) * 8, a.n);
     const bool block = g.db || g.dgate || g.dw_post;
-    int turn = 0;
-    for (size_t row = blockIdx.x; row < (size_t)a.n_rows; row += gridDim.x, turn ^= 1) {
+    auto fetch_row = [&](GradIn<T, R, NV> &in, size_t row) {
         const size_t base = row * a.n;
-        const float rho_b = a.stats[2 * row], rho_v = a.stats[2 * row + 1];
+        in.rho_b = a.stats[2 * row];
+        in.rho_v = a.stats[2 * row + 1];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            if (g.dh) {
+                in.v[k] = fetch(static_cast<const R *>(a.r_out) + base, c[k], a.n);
+                in.dh[k] = fetch(static_cast<const T *>(g.dh) + base, c[k], a.n);
+            }
+            if (g.dr_out) in.dr[k] = fetch(static_cast<const R *>(g.dr_out) + base, c[k], a.n);
+            if (block) {
+                in.b[k] = fetch(static_cast<const T *>(a.b) + base, c[k], a.n);
+                if (AHEAD && a.gate) in.gate[k] = fetch_gate<T>(a, row, c[k]);
+            }
+        }
+    };
+    int turn = 0;
+    auto one = [&](const GradIn<T, R, NV> &in, size_t row) {
+        const size_t base = row * a.n;
         float dv[NV][8];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            if (g.dr_out) {
+                widen(in.dr[k], dv[k]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) dv[k][i] = 0.0f;
+            }
+        }
         if (g.dh) {
             float v[NV][8], u[NV][8], s = 0.0f;
 #pragma unroll
-            for (int c = 0; c < NV; c++) {
+            for (int k = 0; k < NV; k++) {
                 float w[8];
-                load_some(static_cast<const R *>(a.r_out) + base + at[c], some[c], v[c]);
-                load_some(static_cast<const T *>(g.dh) + base + at[c], some[c], u[c]);
-                load_some(a.w_pre + at[c], some[c], w);
+                widen(in.v[k], v[k]);
+                widen(in.dh[k], u[k]);
+                widen(AHEAD ? wq[k] : fetch(a.w_pre, c[k], a.n), w);
+                mask_cols(c[k], u[k]);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    s_pre[c][i] = fmaf(u[c][i], v[c][i] * rho_v, s_pre[c][i]);
-                    u[c][i] *= a.w_offset + w[i];
-                    s = fmaf(u[c][i], v[c][i], s);
+                    s_pre[k][i] = fmaf(u[k][i], v[k][i] * in.rho_v, s_pre[k][i]);
+                    u[k][i] *= a.w_offset + w[i];
+                    s = fmaf(u[k][i], v[k][i], s);
                 }
             }
-            s = group_sum<BS / 64>(s, part[turn][0]) * inv_n * rho_v * rho_v;
+            s = group_sum<BS / 64>(s, part[turn][0]) * inv_n * in.rho_v * in.rho_v;
 #pragma unroll
-            for (int c = 0; c < NV; c++) {
-                if (g.dr_out) {
-                    load_some(static_cast<const R *>(g.dr_out) + base + at[c], some[c], dv[c]);
-                } else {
+            for (int k = 0; k < NV; k++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) dv[c][i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; i++) dv[c][i] += rho_v * (u[c][i] - v[c][i] * s);
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < NV; c++) load_some(static_cast<const R *>(g.dr_out) + base + at[c], some[c], dv[c]);
+                for (int i = 0; i < 8; i++) dv[k][i] += in.rho_v * (u[k][i] - v[k][i] * s);
         }
         if (g.dr) {
 #pragma unroll
-            for (int c = 0; c < NV; c++) store_some(static_cast<R *>(g.dr) + base + at[c], some[c], dv[c]);
+            for (int k = 0; k < NV; k++)
+                if (c[k].lo < 8) put(static_cast<R *>(g.dr) + base, c[k], a.n, dv[k]);
         }
-        if (!block) continue;
+        if (!block) return;
         float b[NV][8], s_b = 0.0f, s_g = 0.0f;
 #pragma unroll
-        for (int c = 0; c < NV; c++) {
+        for (int k = 0; k < NV; k++) {
             float q[8], w[8], dg[8];
-            load_some(static_cast<const T *>(a.b) + base + at[c], some[c], b[c]);
-            load_gate<T>(a, row, at[c], some[c], q);
-            if (a.w_post) load_some(a.w_post + at[c], some[c], w);
+            widen(in.b[k], b[k]);
+            mask_cols(c[k], dv[k]);
+            if (a.gate) gate_of<T>(a, AHEAD ? in.gate[k] : fetch_gate<T>(a, row, c[k]), q);
+            if (a.w_post) widen(AHEAD ? wp[k] : fetch(a.w_post, c[k], a.n), w);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float t = a.gate_sigmoid ? sigmoid(q[i]) : q[i];
+                const float t = !a.gate ? 1.0f : a.gate_sigmoid ? sigmoid(q[i]) : q[i];
                 const float slope = a.gate_sigmoid ? t * (1.0f - t) : 1.0f;
-                const float wp = a.w_post ? a.w_offset + w[i] : 1.0f;
-                const float d = a.scale * dv[c][i];  // of g c
-                const float nb = b[c][i] * rho_b;    // rho_b is 1 without a norm
-                dg[i] = d * nb * wp * slope;
-                s_gate[c][i] += dg[i];
+                const float wo = a.w_post ? a.w_offset + w[i] : 1.0f;
+                const float d = a.scale * dv[k][i];   // of g c
+                const float nb = b[k][i] * in.rho_b;  // rho_b is 1 without a norm
+                dg[i] = d * nb * wo * slope;
+                s_gate[k][i] += dg[i];
                 s_g += dg[i];
-                s_post[c][i] = fmaf(d * t, nb, s_post[c][i]);
-                dv[c][i] = d * t * wp;  // u2 from here on
-                s_b = fmaf(dv[c][i], b[c][i], s_b);
+                s_post[k][i] = fmaf(d * t, nb, s_post[k][i]);
+                dv[k][i] = d * t * wo;  // u2 from here on
+                s_b = fmaf(dv[k][i], b[k][i], s_b);
             }
-            if (a.gate_kind == HOARD_GATE_FULL && g.dgate)
-                store_some(static_cast<T *>(g.dgate) + base + at[c], some[c], dg);
+            if (a.gate_kind == HOARD_GATE_FULL && g.dgate && c[k].lo < 8)
+                put(static_cast<T *>(g.dgate) + base, c[k], a.n, dg);
         }
         if (a.gate_kind == HOARD_GATE_TOKEN && g.dgate) {
             s_g = group_sum<BS / 64>(s_g, part[turn][2]);
             if (threadIdx.x == 0) static_cast<float *>(g.dgate)[row] = s_g;
         }
-        if (!g.db) continue;
+        if (!g.db) return;
         if (a.w_post) {
-            s_b = group_sum<BS / 64>(s_b, part[turn][1]) * inv_n * rho_b * rho_b;
+            s_b = group_sum<BS / 64>(s_b, part[turn][1]) * inv_n * in.rho_b * in.rho_b;
 #pragma unroll
-            for (int c = 0; c < NV; c++)
+            for (int k = 0; k < NV; k++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) dv[c][i] = rho_b * (dv[c][i] - b[c][i] * s_b);
+                for (int i = 0; i < 8; i++) dv[k][i] = in.rho_b * (dv[k][i] - b[k][i] * s_b);
         }
 #pragma unroll
-        for (int c = 0; c < NV; c++) store_some(static_cast<T *>(g.db) + base + at[c], some[c], dv[c]);
+        for (int k = 0; k < NV; k++)
+            if (c[k].lo < 8) put(static_cast<T *>(g.db) + base, c[k], a.n, dv[k]);
+    };
+    if constexpr (AHEAD) {
+        GradIn<T, R, NV> in[2];
+        const size_t rows = a.n_rows, by = gridDim.x;
+        fetch_weights();
+        fetch_row(in[0], blockIdx.x);  // there are no more groups than rows
+        for (size_t row = blockIdx.x; row < rows; row += 2 * by, turn = 0) {
+            fetch_row(in[1], min(row + by, rows - 1));
+            one(in[0], row);
+            if (row + by >= rows) break;
+            turn = 1;
+            fetch_row(in[0], min(row + 2 * by, rows - 1));
+            one(in[1], row + by);
+        }
+    } else {
+        for (size_t row = blockIdx.x; row < (size_t)a.n_rows; row += gridDim.x, turn ^= 1) {
+            GradIn<T, R, NV> in;
+            fetch_row(in, row);
+            one(in, row);
+        }
     }
     const size_t mine = (size_t)blockIdx.x * a.n, all = (size_t)gridDim.x * a.n;
-    float *to = work;
 #pragma unroll
-    for (int c = 0; c < NV; c++) {
-        float *p = to;
+    for (int k = 0; k < NV; k++) {
+        float *p = work + mine;
+        if (c[k].lo == 8) continue;
         if (g.dw_pre) {
-            store_some(p + mine + at[c], some[c], s_pre[c]);
+            put(p, c[k], a.n, s_pre[k]);
             p += all;
         }
         if (g.dw_post) {
-            store_some(p + mine + at[c], some[c], s_post[c]);
+            put(p, c[k], a.n, s_post[k]);
             p += all;
         }
-        if (g.dgate && a.gate_kind == HOARD_GATE_CHANNEL) store_some(p + mine + at[c], some[c], s_gate[c]);
+        if (g.dgate && a.gate_kind == HOARD_GATE_CHANNEL) put(p, c[k], a.n, s_gate[k]);
     }
 }
 
@@ -272,9 +373,14 @@ void grad_of(const hoard_norm_args &a, const hoard_norm_grads &g, float *work, h
 
 }  // namespace
 
+// As many groups as the chip holds at once (by their registers: 3 of 256 threads a CU,
+// 1 of 1024; of 64 threads as many as the partial sums are worth), with equal shares
+// of the rows.  4096 x 2048, bf16: 29.4 us with 768 groups, 33.0 with 512, 37.7 with 1024.
 int norm_groups(int n_rows, int n) {
-    (void)n;
-    return n_rows < 512 ? n_rows : 512;
+    const int most = n <= 1024 ? 1024 : n <= 4096 ? 768 : 256;
+    if (n_rows <= most) return n_rows;
+    const int share = (n_rows + most - 1) / most;
+    return (n_rows + share - 1) / share;
 }
 
 hipError_t launch_norm(const hoard_norm_args &a, hipStream_t s) {

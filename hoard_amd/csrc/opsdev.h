@@ -16,47 +16,73 @@ typedef __bf16 bf16;
 // there, so rows of an odd length take the same path.
 typedef uint32_t u128 __attribute__((ext_vector_type(4), aligned(2)));
 
-// Eight values of T at p as floats.  NT: with the non-temporal policy, for what is
-// read or written once and would only push other data out of the caches.
+// Eight columns of a row of n, at .. at + 7, of which those from at + lo on are the
+// thread's.  A row whose length is no multiple of 8 ends in columns that overlap the
+// ones before (lo > 0); a thread behind the end has none (lo 8).  So no load stands
+// under a condition: loads of many rows and arrays are in flight together.
+struct Cols {
+    int at, lo;
+};
+__device__ __forceinline__ Cols cols_of(int first, int n) {
+    const int last = max(n - 8, 0);
+    return first < n ? Cols{min(first, last), first - min(first, last)} : Cols{last, 8};
+}
+
+// Eight values as they lie in memory.
+template <typename T>
+struct Raw {
+    u128 w[sizeof(T) / 2];
+};
+// NT: with the non-temporal policy, for what is read or written once and would only
+// push other data out of the caches.
 template <bool NT = false, typename T>
-__device__ __forceinline__ void load8(const T *p, float o[8]) {
-    T v[8];
+__device__ __forceinline__ Raw<T> fetch(const T *row, Cols c, int n) {
+    Raw<T> r;
+    if (n >= 8) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof v / 16; i++) {
-        const u128 *from = reinterpret_cast<const u128 *>(p) + i;
-        const u128 w = NT ? __builtin_nontemporal_load(from) : *from;
-        __builtin_memcpy(reinterpret_cast<char *>(v) + 16 * i, &w, 16);
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            const u128 *from = reinterpret_cast<const u128 *>(row + c.at) + i;
+            r.w[i] = NT ? __builtin_nontemporal_load(from) : *from;
+        }
+    } else {
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = i < n ? row[i] : (T)0.0f;
+        __builtin_memcpy(&r, v, sizeof r);
     }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Raw<T> &r, float o[8]) {
+    T v[8];
+    __builtin_memcpy(v, &r, sizeof v);
 #pragma unroll
     for (int i = 0; i < 8; i++) o[i] = (float)v[i];
 }
-// Stored values are rounded to nearest, ties to even, once.
+// Zero in the columns that are not the thread's, for sums.
+__device__ __forceinline__ void mask_cols(Cols c, float o[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = i >= c.lo ? o[i] : 0.0f;
+}
+// The thread's columns, rounded to nearest, ties to even, once.
 template <bool NT = false, typename T>
-__device__ __forceinline__ void store8(T *p, const float o[8]) {
+__device__ __forceinline__ void put(T *row, Cols c, int n, const float o[8]) {
     T v[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = (T)o[i];
+    if (c.lo == 0 && n >= 8) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof v / 16; i++) {
-        u128 w, *to = reinterpret_cast<u128 *>(p) + i;
-        __builtin_memcpy(&w, reinterpret_cast<const char *>(v) + 16 * i, 16);
-        if (NT) __builtin_nontemporal_store(w, to);
-        else *to = w;
+        for (int i = 0; i < (int)sizeof v / 16; i++) {
+            u128 w, *to = reinterpret_cast<u128 *>(row + c.at) + i;
+            __builtin_memcpy(&w, reinterpret_cast<const char *>(v) + 16 * i, 16);
+            if (NT) __builtin_nontemporal_store(w, to);
+            else *to = w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i >= c.lo && i < n) row[c.at + i] = v[i];
     }
-}
-// The first `some` of them; the rest of o is zero.
-template <bool NT = false, typename T>
-__device__ __forceinline__ void load_some(const T *p, int some, float o[8]) {
-    if (some >= 8) return load8<NT>(p, o);
-#pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = i < some ? (float)p[i] : 0.0f;
-}
-template <bool NT = false, typename T>
-__device__ __forceinline__ void store_some(T *p, int some, const float o[8]) {
-    if (some >= 8) return store8<NT>(p, o);
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (i < some) p[i] = (T)o[i];
 }
 
 // Sum over the wave's 64 lanes, in every lane, in a fixed order.

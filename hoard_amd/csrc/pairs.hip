@@ -118,10 +118,9 @@ __global__ __launch_bounds__(kBlockPairs) void place_kernel(PairsArgs a, int64_t
 // time, so that their latencies overlap.
 constexpr int kAhead = 8;
 
-__device__ __forceinline__ bool item_of(const RowsArgs &a, int64_t i, int per_row, int64_t &t, int &at, int &some) {
+__device__ __forceinline__ bool item_of(const RowsArgs &a, int64_t i, int per_row, int64_t &t, Cols &c) {
     t = i / per_row;
-    at = (int)(i - t * per_row) * 8;
-    some = min(8, a.n - at);
+    c = cols_of((int)(i - t * per_row) * 8, a.n);
     return t < a.n_tokens;
 }
 // The sorted rows of slots j0 .. j0 + kAhead - 1 of token t, -1 for a dropped pair.
@@ -146,19 +145,19 @@ __global__ __launch_bounds__(256) void gather_kernel(RowsArgs a) {
     const int64_t pairs = (int64_t)a.n_tokens * a.k;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;; i += (int64_t)gridDim.x * 256) {
         int64_t t;
-        int at, some;
-        if (!item_of(a, i, per_row, t, at, some)) return;
+        Cols c;
+        if (!item_of(a, i, per_row, t, c)) return;
         float x[8], o[8], w[kAhead];
         int row[kAhead];
-        load_some(static_cast<const T *>(a.x) + t * a.n + at, some, x);
+        widen(fetch(static_cast<const T *>(a.x) + t * a.n, c, a.n), x);
         for (int j = 0; j < a.k; j += kAhead) {
             rows_of(a, t, j, pairs, row, w);
 #pragma unroll
             for (int u = 0; u < kAhead; u++) {
                 if (row[u] < 0) continue;
 #pragma unroll
-                for (int c = 0; c < 8; c++) o[c] = a.w ? w[u] * x[c] : x[c];
-                store_some<NT>(static_cast<T *>(a.out) + (int64_t)row[u] * a.n + at, some, o);
+                for (int v = 0; v < 8; v++) o[v] = a.w ? w[u] * x[v] : x[v];
+                put<NT>(static_cast<T *>(a.out) + (int64_t)row[u] * a.n, c, a.n, o);
             }
         }
     }
@@ -170,59 +169,54 @@ __global__ __launch_bounds__(256) void combine_kernel(RowsArgs a) {
     const int64_t pairs = (int64_t)a.n_tokens * a.k;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;; i += (int64_t)gridDim.x * 256) {
         int64_t t;
-        int at, some;
-        if (!item_of(a, i, per_row, t, at, some)) return;
-        float s[8] = {}, w[kAhead];
+        Cols c;
+        if (!item_of(a, i, per_row, t, c)) return;
+        float s[8] = {}, w[kAhead], v[8];
         int row[kAhead];
-        if (a.res) load_some(static_cast<const T *>(a.res) + t * a.n + at, some, s);
+        if (a.res) widen(fetch(static_cast<const T *>(a.res) + t * a.n, c, a.n), s);
         for (int j = 0; j < a.k; j += kAhead) {
             rows_of(a, t, j, pairs, row, w);
-            float y[kAhead][8];
+            Raw<T> y[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; u++)
-                if (row[u] >= 0) load_some<NT>(static_cast<const T *>(a.x) + (int64_t)row[u] * a.n + at, some, y[u]);
+            for (int u = 0; u < kAhead; u++)  // a dropped pair's place is row 0's, and not added
+                y[u] = fetch<NT>(static_cast<const T *>(a.x) + (int64_t)max(row[u], 0) * a.n, c, a.n);
 #pragma unroll
             for (int u = 0; u < kAhead; u++) {
-                if (row[u] < 0) continue;
+                widen(y[u], v);
 #pragma unroll
-                for (int c = 0; c < 8; c++) s[c] = fmaf(w[u], y[u][c], s[c]);
+                for (int i = 0; i < 8; i++) s[i] = row[u] >= 0 ? fmaf(w[u], v[i], s[i]) : s[i];
             }
         }
-        store_some<NT>(static_cast<T *>(a.out) + t * a.n + at, some, s);
+        put<NT>(static_cast<T *>(a.out) + t * a.n, c, a.n, s);
     }
 }
 
-// A wave takes a pair, kChunks * 512 columns at a time; ROUND: n is a multiple of 8.
+// A wave takes a pair, kChunks * 512 columns at a time.
 constexpr int kChunks = 4;
-template <typename T, bool ROUND, bool NT>
+template <typename T, bool NT>
 __device__ __forceinline__ float grad_row(const T *d, const T *y, T *dy, float w, int n) {
     const int lane = threadIdx.x & 63;
     float s = 0.0f;
-    for (int at0 = lane * 8; at0 < n; at0 += kChunks * 512) {
-        float dv[kChunks][8], yv[kChunks][8];
+    for (int at = lane * 8; at - lane * 8 < n; at += kChunks * 512) {
+        Raw<T> dr[kChunks], yr[kChunks];
+        Cols c[kChunks];
 #pragma unroll
-        for (int c = 0; c < kChunks; c++) {
-            const int at = at0 + c * 512;
-            if (ROUND) {  // behind the end: the last columns again, without weight
-                load8(d + min(at, n - 8), dv[c]);
-                load8<NT>(y + min(at, n - 8), yv[c]);
-            } else {
-                load_some(d + at, n - at, dv[c]);
-                load_some<NT>(y + at, n - at, yv[c]);
-            }
+        for (int u = 0; u < kChunks; u++) {
+            c[u] = cols_of(at + u * 512, n);
+            dr[u] = fetch(d, c[u], n);
+            yr[u] = fetch<NT>(y, c[u], n);
         }
 #pragma unroll
-        for (int c = 0; c < kChunks; c++) {
-            const int at = at0 + c * 512;
-            if (ROUND && at >= n) continue;
+        for (int u = 0; u < kChunks; u++) {
+            float dv[8], yv[8];
+            widen(dr[u], dv);
+            widen(yr[u], yv);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                s = fmaf(dv[c][i], yv[c][i], s);
-                dv[c][i] *= w;
+                s = i >= c[u].lo ? fmaf(dv[i], yv[i], s) : s;
+                dv[i] *= w;
             }
-            if (!dy) continue;
-            if (ROUND) store8<NT>(dy + at, dv[c]);
-            else store_some<NT>(dy + at, n - at, dv[c]);
+            if (dy && c[u].lo < 8) put<NT>(dy, c[u], n, dv);
         }
     }
     return s;
@@ -238,7 +232,7 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(RowsArgs a) {
             const T *const d = static_cast<const T *>(a.res) + p / a.k * a.n;
             const T *const y = static_cast<const T *>(a.x) + (int64_t)row * a.n;
             T *const dy = a.out ? static_cast<T *>(a.out) + (int64_t)row * a.n : nullptr;
-            s = a.n % 8 == 0 ? grad_row<T, true, NT>(d, y, dy, a.w[p], a.n) : grad_row<T, false, NT>(d, y, dy, a.w[p], a.n);
+            s = grad_row<T, NT>(d, y, dy, a.w[p], a.n);
         }
         s = wave_sum_f(s);
         if ((threadIdx.x & 63) == 0) a.dw[p] = s;
