@@ -404,11 +404,12 @@ void grad_of(const hoard_norm_args &a, const hoard_norm_grads &g, float *work, h
 
 }  // namespace
 
-// As many groups as the chip holds at once (by their registers: 3 of 256 threads a CU,
-// 1 of 1024; of 64 threads as many as the partial sums are worth), with equal shares
-// of the rows.  4096 x 2048, bf16: 29.4 us with 768 groups, 33.0 with 512, 37.7 with 1024.
+// As many groups as the chip holds at once (by their registers 3 of 256 threads a CU,
+// 1 of more; of 64 threads as many as the partial sums are worth), with equal shares
+// of the rows.  4096 x 2048, bf16: 29.4 us with 768 groups, 33.0 with 512, 37.7 with
+// 1024; 4096 x 4096: 62.5 with 256, 64.3 with 512, 74.0 with 768.
 int norm_groups(int n_rows, int n) {
-    const int most = n <= 1024 ? 1024 : n <= 4096 ? 768 : 256;
+    const int most = n <= 1024 ? 1024 : n <= 2048 ? 768 : 256;
     if (n_rows <= most) return n_rows;
     const int share = (n_rows + most - 1) / most;
     return (n_rows + share - 1) / share;
