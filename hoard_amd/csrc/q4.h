@@ -84,10 +84,10 @@ __device__ __forceinline__ float dot2(uint32_t w, uint32_t x, float s) {
 template <typename T>
 constexpr uint32_t kOnes = __is_same(T, bf16) ? 0x3f803f80u : 0x3c003c00u;
 
-// A scale as it is stored (scale `i` from `base` on), and its value.
-__device__ __forceinline__ uint32_t raw_scale(const hoard_q4_matrix &m, size_t base, uint32_t i) {
-    if (m.scale_type == HOARD_TYPE_F32) return (static_cast<const uint32_t *>(m.scales) + base)[i];
-    return (static_cast<const uint16_t *>(m.scales) + base)[i];
+// A scale as it is stored, and its value.
+__device__ __forceinline__ uint32_t raw_scale(const hoard_q4_matrix &m, size_t i) {
+    if (m.scale_type == HOARD_TYPE_F32) return static_cast<const uint32_t *>(m.scales)[i];
+    return static_cast<const uint16_t *>(m.scales)[i];
 }
 __device__ __forceinline__ float scale_of(int type, uint32_t raw) {
     if (type == HOARD_TYPE_F32) return __uint_as_float(raw);
@@ -95,21 +95,11 @@ __device__ __forceinline__ float scale_of(int type, uint32_t raw) {
     return (float)__builtin_bit_cast(f16, (uint16_t)raw);
 }
 
-// The matrix of row r, or -1.
+// The matrix of row r of a call without offsets, or -1.
 __device__ __forceinline__ int matrix_of(const Q4Args &a, int r) {
     if (a.mode == kQ4One) return 0;
-    if (a.mode == kQ4Ids) {
-        const int e = a.sel[r];
-        return e < 0 || e >= a.w.n_mat ? -1 : e;
-    }
-    // the last e with sel[e] <= r
-    int lo = 0, hi = a.w.n_mat;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.sel[mid] <= r) lo = mid;
-        else hi = mid;
-    }
-    return a.sel[lo] <= r && r < a.sel[lo + 1] ? lo : -1;
+    const int e = a.sel[r];
+    return e < 0 || e >= a.w.n_mat ? -1 : e;
 }
 
 // g / (1 + e^-g) * u.  Where the result is rounded to 16 bits, with the exponential of
