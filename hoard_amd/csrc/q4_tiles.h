@@ -415,24 +415,26 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
 //
 // A row of x is 256 bytes of a buffer, its 16-byte pieces exchanged by the row's
 // number (piece ^ row % 16), so that 16 rows' pieces fall on all the banks.
-template <typename T, int G, bool UP, int MT, int NW, int SC, int MW>
-__global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
-    constexpr int TM = 16 * MT, THREADS = 64 * NW, P = 2, NG = 128 / G, SP = 4 / NG;
+template <typename T, int G, bool UP, int MT, int NW, int KS, int MW>
+__global__ __launch_bounds__(64 * NW * KS, MW) void q4_flow_kernel(Q4Args a) {
+    constexpr int TM = 16 * MT, THREADS = 64 * NW * KS, P = 2, NG = 128 / G, SP = 4 / NG;
     constexpr int CH = TM / 4 / NW;                        // copies of 1 KB a wave and step
-    constexpr int RW = 16 * NW * P, SPC = SC / NG, SI = RW * SC / THREADS;
+    constexpr int RW = 16 * NW * P, XS = KS * NG, SC = XS > 16 ? XS : 16, SPC = SC / XS, SI = RW * SC / THREADS;
     constexpr int WIDE = UP ? 16 : 32;
     static_assert(CH * NW * 4 == TM && SI * THREADS == RW * SC && SC % SI == 0, "whole shares");
-    __shared__ __align__(16) uint8_t lds[2][TM * 256];
+    static_assert((KS - 1) * NW * P * MT * 1024 <= KS * 2 * TM * 256, "the partial sums take the place of x");
+    __shared__ __align__(16) uint8_t lds[KS][2][TM * 256];
     __shared__ float scale[RW][SC + 1], zero[RW][SC + 1];
 
-    const int tid = threadIdx.x, lane = tid & 63, nw = wave_index(), col = lane & 15, q = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), nw = wave % NW, ks = wave / NW;
+    const int col = lane & 15, q = lane >> 4;
     int e, r0, rows, tn;
     {
         const int nt = (a.w.rows + NW * WIDE - 1) / (NW * WIDE), id = blockIdx.x, run = a.spread ? id >> 3 : id;
         tn = run % nt;
         if (!tile_of(a, a.tile0 + (a.spread ? (run / nt) * 8 + (id & 7) : run / nt), TM, e, r0, rows)) return;
     }
-    const int cols = a.w.cols, groups = cols / G, steps = (cols + 127) / 128;
+    const int cols = a.w.cols, groups = cols / G, blocks = (cols + 127) / 128, steps = (blocks + KS - 1) / KS;
     const int first = (tn * NW + nw) * WIDE, n0 = first + col, top = min(first, a.w.rows - 1);
     const int last_block = (cols - 32 - q * 32) >= 0 ? (cols - 32 - q * 32) / 128 : 0;
     const size_t row0 = (size_t)e * a.w.rows + top;
@@ -447,7 +449,7 @@ __global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
         for (int p = 0; p < P; p++) {
             const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
             const uint8_t *const from = static_cast<const uint8_t *>(m.codes) + row0 * (cols / 2);
-            codes[decltype(at)::value][p] = *reinterpret_cast<const v4u *>(from + (code[p] + min(step, last_block) * 64));
+            codes[decltype(at)::value][p] = *reinterpret_cast<const v4u *>(from + (code[p] + min(step * KS + ks, last_block) * 64));
         }
     };
     // the wave's copies: lane l of a copy brings piece (l % 16) ^ row of row l / 16
@@ -460,8 +462,8 @@ __global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
 #pragma unroll
         for (int j = 0; j < CH; j++)
             if ((nw * CH + j) * 4 < rows)
-                dma_lanes_at(lds[buffer] + (nw * CH + j) * 1024, x0,
-                             src[j] + 2 * min(step * 128 + (piece ^ (((nw * CH + j) & 3) * 4)) * 8, cols - 8));
+                dma_lanes_at(lds[ks][buffer] + (nw * CH + j) * 1024, x0,
+                             src[j] + 2 * min((step * KS + ks) * 128 + (piece ^ (((nw * CH + j) & 3) * 4)) * 8, cols - 8));
     };
     auto stage_scales = [&](int chunk) {
         const int row = tid / (SC / SI), g0 = (tid % (SC / SI)) * SI, p = row / (16 * NW), in = row % (16 * NW);
@@ -504,13 +506,13 @@ __global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
         if (step + 2 < steps) fetch_w(at, step + 2);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            if (step * 128 + g * G >= cols) break;  // a group lies inside or behind the last column as a whole
+            if ((step * KS + ks) * 128 + g * G >= cols) break;  // a group lies inside or behind the last column as a whole
             v4u w[P][SP];
             float sc[P], zc[P];
 #pragma unroll
             for (int p = 0; p < P; p++) {
-                sc[p] = scale[(p * NW + nw) * 16 + col][(step % SPC) * NG + g];
-                zc[p] = zero[(p * NW + nw) * 16 + col][(step % SPC) * NG + g];
+                sc[p] = scale[(p * NW + nw) * 16 + col][(step % SPC) * XS + ks * NG + g];
+                zc[p] = zero[(p * NW + nw) * 16 + col][(step % SPC) * XS + ks * NG + g];
 #pragma unroll
                 for (int i = 0; i < SP; i++) w[p][i] = in_order<T>(now[p][g * SP + i]);
             }
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
             for (int t = 0; t < MT; t++) {
                 if (t * 16 >= rows) break;
                 v4f d[P] = {}, xs = (v4f)(0.0f);
-                const uint8_t *from = lds[B] + (t * 16 + col) * 256;
+                const uint8_t *from = lds[ks][B] + (t * 16 + col) * 256;
 #pragma unroll
                 for (int i = 0; i < SP; i++) {
                     const v4u x = *reinterpret_cast<const v4u *>(from + (((column_of<G>(g * SP + i, q) / 8) ^ col) * 16));
@@ -542,6 +544,23 @@ __global__ __launch_bounds__(64 * NW, MW) void q4_flow_kernel(Q4Args a) {
     for (int step = 0; step < steps; step += 2) {
         body(even, step);
         if (step + 1 < steps) body(odd, step + 1);
+    }
+    if constexpr (KS > 1) {
+        __syncthreads();
+        v4f *meet = reinterpret_cast<v4f *>(&lds[0][0][0]);
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+                if (ks) meet[((((ks - 1) * NW + nw) * P + p) * MT + t) * 64 + lane] = acc[p][t];
+        __syncthreads();
+        if (ks) return;
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int c = 1; c < KS; c++) acc[p][t] += meet[((((c - 1) * NW + nw) * P + p) * MT + t) * 64 + lane];
     }
     T *y = static_cast<T *>(a.y) + (size_t)r0 * a.w.rows;
 #pragma unroll
@@ -584,10 +603,10 @@ hipError_t launch_tiles_of(const Q4Args &a, hipStream_t s) {
         q4_tiles_kernel<T, G, UP, P, MT, NW, KS, KB, MW><<<grid, 64 * NW * KS, 0, s>>>(part);
     });
 }
-template <typename T, int G, bool UP, int MT, int NW, int SC, int MW>
+template <typename T, int G, bool UP, int MT, int NW, int KS, int MW>
 hipError_t launch_flow_of(const Q4Args &a, hipStream_t s) {
     return over_tiles<16 * MT, NW *(UP ? 16 : 32)>(a, [&](const Q4Args &part, unsigned grid) {
-        q4_flow_kernel<T, G, UP, MT, NW, SC, MW><<<grid, 64 * NW, 0, s>>>(part);
+        q4_flow_kernel<T, G, UP, MT, NW, KS, MW><<<grid, 64 * NW * KS, 0, s>>>(part);
     });
 }
 
@@ -599,8 +618,8 @@ hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
     if constexpr (WIDE) {
         return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 1, 2>(a, s);
     } else {
-        if (per <= 24) return launch_flow_of<T, G, UP, 2, 4, 16, 3>(a, s);
-        return launch_flow_of<T, G, UP, 4, 4, 16, 3>(a, s);
+        if (per <= 24) return launch_flow_of<T, G, UP, 2, 4, 1, 3>(a, s);
+        return launch_flow_of<T, G, UP, 4, 4, 1, 3>(a, s);
     }
 }
 
