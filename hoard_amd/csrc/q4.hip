@@ -72,18 +72,19 @@ __device__ __forceinline__ float dots(v4u codes, float zero, const Slice<T> &x) 
     return d;
 }
 
-// A row of x at a time.  A wave takes kRowsOfW rows of W per run of 2^lanes_log lanes;
-// the run's lanes split the columns, 32 consecutive ones (16 bytes of codes) at a time.
+// A row of x at a time.  A wave takes NR rows of W per run of 2^lanes_log lanes; the
+// run's lanes split the columns, 32 consecutive ones (16 bytes of codes) at a time.
 //
 // Bound by memory, and below a few MB of codes by its latency: two rows of W a wave
-// keep enough waves in flight (16384 x 8192: 15.9 us with 2 rows, 18.1 with 4, 19.3
-// with 8, 21.5 with 1; 8 experts' 768 x 2048 twice in fp32: 8.4 with 2, 9.2 with 4, 9.9
-// with 1).  x goes from the caches to registers: through LDS, shared by the four waves,
-// the same took 18.1 and 10.3.
-constexpr int kRowsOfW = 2;
-template <typename T, bool UP>
+// keep enough waves in flight (16384 x 8192 in bf16: 15.9 us with 2 rows, 18.1 with 4,
+// 19.3 with 8, 21.5 with 1; 8 experts' 768 x 2048 twice in fp32: 8.4 with 2, 9.2 with 4,
+// 9.9 with 1).  In fp32 a row of x is four times its codes, and from 4096 rows of W on
+// four rows a wave that share it are faster (8192 x 8192: 13.8 against 18.6; 512 x 2048:
+// 5.2 against 4.4).  x goes from the caches to registers: through LDS, shared by the
+// four waves, 16384 x 8192 took 18.1 and the 8 experts 10.3.
+template <typename T, bool UP, int NR>
 __global__ __launch_bounds__(256) void q4_rows_kernel(Q4Args a, int lanes_log) {
-    constexpr int P = UP ? 2 : 1, NR = kRowsOfW;
+    constexpr int P = UP ? 2 : 1;
     const int lane = threadIdx.x & 63, run = lane >> lanes_log, lk = lane & ((1 << lanes_log) - 1);
     const int64_t at = (((int64_t)blockIdx.x * 4 + wave_index()) << (6 - lanes_log)) * NR + run * NR;
     const int n0 = (int)min(at, (int64_t)a.w.rows);
@@ -144,15 +145,20 @@ __global__ __launch_bounds__(256) void q4_rows_kernel(Q4Args a, int lanes_log) {
     }
 }
 
-template <typename T>
-hipError_t launch_rows(const Q4Args &a, hipStream_t s) {
+template <typename T, bool UP, int NR>
+hipError_t launch_rows_of(const Q4Args &a, hipStream_t s) {
     int lanes_log = 3;
     while (lanes_log < 6 && (32 << lanes_log) < a.w.cols) lanes_log++;
-    const int64_t per = (int64_t)4 * kRowsOfW << (6 - lanes_log);
+    const int64_t per = (int64_t)4 * NR << (6 - lanes_log);
     const dim3 grid((unsigned)((a.w.rows + per - 1) / per), (unsigned)(a.n_rows < 65535 ? a.n_rows : 65535));
-    if (a.up.codes) q4_rows_kernel<T, true><<<grid, 256, 0, s>>>(a, lanes_log);
-    else q4_rows_kernel<T, false><<<grid, 256, 0, s>>>(a, lanes_log);
+    q4_rows_kernel<T, UP, NR><<<grid, 256, 0, s>>>(a, lanes_log);
     return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_rows(const Q4Args &a, hipStream_t s) {
+    if (a.up.codes) return launch_rows_of<T, true, 2>(a, s);
+    if (sizeof(T) == 4 && (int64_t)a.w.rows * a.n_rows >= 4096) return launch_rows_of<T, false, 4>(a, s);
+    return launch_rows_of<T, false, 2>(a, s);
 }
 
 }  // namespace

@@ -180,7 +180,8 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
     __shared__ __align__(16) float sums[XS][TM];
     __shared__ float scale[RW][SC + 1], zero[RW][SC + 1];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), nw = wave % NW, ks = wave / NW;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
+    const int nw = KS > 1 ? wave % NW : wave, ks = KS > 1 ? wave / NW : 0;
     const int col = lane & 15, q = lane >> 4;
     int e, r0, rows;
     // a tile of x in all its tiles of W: next to each other, or (a.spread) on one XCD,
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
         const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
         const size_t from = ((size_t)e * a.w.rows + min(n, a.w.rows - 1)) * groups;
         const int g1 = chunk * SC + g0;
-        if (g1 + SI <= groups) {
+        if (SI > 1 && g1 + SI <= groups) {
             load_scales<SI>(m, from + g1, scale[row] + g0, zero[row] + g0, 16.0f);
         } else {
 #pragma unroll
@@ -426,7 +427,8 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_flow_kernel(Q4Args a) {
     __shared__ __align__(16) uint8_t lds[KS][2][TM * 256];
     __shared__ float scale[RW][SC + 1], zero[RW][SC + 1];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), nw = wave % NW, ks = wave / NW;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
+    const int nw = KS > 1 ? wave % NW : wave, ks = KS > 1 ? wave / NW : 0;
     const int col = lane & 15, q = lane >> 4;
     int e, r0, rows, tn;
     {
@@ -471,7 +473,7 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_flow_kernel(Q4Args a) {
         const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
         const size_t from = ((size_t)e * a.w.rows + min(n, a.w.rows - 1)) * groups;
         const int g1 = chunk * SC + g0;
-        if (g1 + SI <= groups) {
+        if (SI > 1 && g1 + SI <= groups) {
             load_scales<SI>(m, from + g1, scale[row] + g0, zero[row] + g0, kInOrderBias<T>);
         } else {
 #pragma unroll
@@ -580,11 +582,16 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_flow_kernel(Q4Args a) {
     }
 }
 
-// f(tile, grid) over the launches that cover the call's tiles.
+// Tiles of tm rows of x; with offsets, which the host does not see, at most so many.
+inline int64_t tiles_of(const Q4Args &a, int tm) {
+    if (a.mode == kQ4Sorted) return a.n_rows / tm + (a.n_rows < a.w.n_mat ? a.n_rows : a.w.n_mat);
+    return ((int64_t)a.n_rows + tm - 1) / tm;
+}
+
+// launch(part, grid) over the launches that cover the call's tiles.
 template <int TM, int TN, typename F>
 hipError_t over_tiles(const Q4Args &a, F launch) {
-    int64_t tiles = ((int64_t)a.n_rows + TM - 1) / TM;
-    if (a.mode == kQ4Sorted) tiles = a.n_rows / TM + (a.n_rows < a.w.n_mat ? a.n_rows : a.w.n_mat);
+    const int64_t tiles = tiles_of(a, TM);
     const int64_t nt = (a.w.rows + TN - 1) / TN, most = std::max<int64_t>(8, ((1 << 22) / nt) & ~7);  // tiles of a launch
     Q4Args part = a;
     part.spread = tiles >= 32;
@@ -610,15 +617,65 @@ hipError_t launch_flow_of(const Q4Args &a, hipStream_t s) {
     });
 }
 
+// The form of a call, by the workgroups it makes.  A workgroup's steps follow one
+// another at a latency of 0.7 us or so, whatever the tile's size, so while there are
+// fewer workgroups than the 256 CUs hold, smaller tiles and columns split over more
+// waves are faster; above that, larger tiles read x and unpack the codes less often.
+// Measured on bf16 (us):
+//   4096 x 4096, rows of x   16    20    32    64   128   256   512
+//     tiles 16, columns / 8  7.8
+//     tiles 32, columns / 8        9.4  11.9  26.6  50.9
+//     flow 16, columns / 4  13.8  14.1  14.0  14.9  15.8  28.8  59.6
+//     flow 32, columns / 4  14.7  17.7  18.0  18.4  18.8  20.1  37.6
+//     flow 64, columns / 2              20.5  28.6  29.0  29.7  31.6
+//     flow 64               22.0  27.0  27.2  42.0  42.3  42.4  43.8 (8192 rows of W:
+//                                               59.5 at 512, where flow 64 / 2 takes 60.8)
+//   16384 x 8192, 16 rows: 24.5 by tiles 16 / 4 two wide, 34.3 by tiles 16 / 8.
+//   Sorted, 10 of 512 experts of 512 x 2048 twice, tokens   1     4    16    64   384
+//     tiles 16, columns / 4, two wide                     10.9  18.0  47.7   119   219
+//     flow 16, columns / 2                                14.4  17.0  36.1  79.5   156
+//     flow 32                                             20.0  21.5  32.3  61.5   118
+//   8 of 128 experts of 768 x 2048 twice, 512 tokens: 79 by flow 64, 92 by flow 32.
+// fp32 (us): 4096 x 4096, 64 rows 27 by tiles 32 / 4 two wide, 56 by tiles 32 four wide;
+// 8 of 128 experts, 128 tokens: 65 by tiles 16 four wide, 76 by tiles 32, 139 by tiles
+// 16 / 4; 4 tokens: 19 by tiles 16 / 2 two wide, 25 by tiles 16 four wide; 1 token 10.1
+// by tiles 16 / 4, 12.9 by tiles 16 / 2 two wide.
+constexpr int64_t kCUs = 256;
+
 template <typename T, int G, bool UP>
 hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
-    constexpr bool WIDE = sizeof(T) == 4;  // three planes of x
-    const int per = a.mode == kQ4Sorted ? (a.n_rows + a.w.n_mat - 1) / a.w.n_mat : a.n_rows;
-    if (per <= 16) return launch_tiles_of<T, G, UP, UP ? 2 : 1, 1, 1, WIDE ? 4 : 8, 1, 2>(a, s);
-    if constexpr (WIDE) {
+    constexpr int P = UP ? 2 : 1;
+    const bool sorted = a.mode == kQ4Sorted;
+    const int per = sorted ? (a.n_rows + a.w.n_mat - 1) / a.w.n_mat : a.n_rows;  // rows of x of a matrix
+    // workgroups with tiles of tm rows of x and tn of W
+    auto groups = [&](int tm, int tn) { return (int64_t)((a.w.rows + tn - 1) / tn) * tiles_of(a, tm); };
+    constexpr int TN = UP ? 64 : 128;  // rows of W of a workgroup four wide
+    if constexpr (sizeof(T) == 4) {
+        if (sorted) {
+            if (groups(16, TN) <= kCUs / 2) return launch_tiles_of<T, G, UP, 2, 1, 1, 4, 1, 2>(a, s);
+            if (groups(16, TN) <= 2 * kCUs) return launch_tiles_of<T, G, UP, 2, 1, 2, 2, 1, 2>(a, s);
+            if (per <= 16) return launch_tiles_of<T, G, UP, 2, 1, 4, 1, 1, 2>(a, s);
+            return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 1, 2>(a, s);
+        }
+        if (per <= 16)
+            return groups(16, 16) <= 3 * kCUs ? launch_tiles_of<T, G, UP, 2, 1, 1, 8, 1, 2>(a, s)
+                                              : launch_tiles_of<T, G, UP, 2, 1, 1, 4, 1, 2>(a, s);
+        if (groups(32, 32) <= kCUs) return launch_tiles_of<T, G, UP, P, 2, 2, 4, 1, 2>(a, s);
+        if (groups(32, TN) <= kCUs) return launch_tiles_of<T, G, UP, 2, 2, 4, 2, 1, 2>(a, s);
         return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 1, 2>(a, s);
     } else {
-        if (per <= 24) return launch_flow_of<T, G, UP, 2, 4, 1, 3>(a, s);
+        if (sorted) {
+            if (groups(16, TN) <= kCUs / 2) return launch_tiles_of<T, G, UP, P, 1, 2, 4, 1, 2>(a, s);
+            if (groups(16, TN) <= 2 * kCUs) return launch_flow_of<T, G, UP, 1, 4, 2, 4>(a, s);
+            return per <= 24 ? launch_flow_of<T, G, UP, 2, 4, 1, 4>(a, s) : launch_flow_of<T, G, UP, 4, 4, 1, 3>(a, s);
+        }
+        if (per <= 16)
+            return groups(16, 16) <= 3 * kCUs ? launch_tiles_of<T, G, UP, P, 1, 1, 8, 1, 2>(a, s)
+                                              : launch_tiles_of<T, G, UP, P, 1, 2, 4, 1, 2>(a, s);
+        if (groups(32, 16) <= kCUs) return launch_tiles_of<T, G, UP, P, 2, 1, 8, 1, 2>(a, s);
+        if (groups(16, TN) <= kCUs) return launch_flow_of<T, G, UP, 1, 4, 4, 4>(a, s);
+        if (groups(32, TN) <= kCUs) return launch_flow_of<T, G, UP, 2, 4, 4, 4>(a, s);
+        if (groups(64, TN) <= kCUs) return launch_flow_of<T, G, UP, 4, 4, 2, 2>(a, s);
         return launch_flow_of<T, G, UP, 4, 4, 1, 3>(a, s);
     }
 }
