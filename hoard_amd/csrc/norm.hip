@@ -322,20 +322,23 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
             one(in, row);
         }
     }
+    // the group's rows of the workspace, or the result itself where it is the only row
     const size_t mine = (size_t)blockIdx.x * a.n, all = (size_t)gridDim.x * a.n;
+    const bool alone = a.n_rows == 1;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         float *p = work + mine;
         if (c[k].lo == 8) continue;
         if (g.dw_pre) {
-            put(p, c[k], a.n, s_pre[k]);
+            put(alone ? g.dw_pre : p, c[k], a.n, s_pre[k]);
             p += all;
         }
         if (g.dw_post) {
-            put(p, c[k], a.n, s_post[k]);
+            put(alone ? g.dw_post : p, c[k], a.n, s_post[k]);
             p += all;
         }
-        if (g.dgate && a.gate_kind == HOARD_GATE_CHANNEL) put(p, c[k], a.n, s_gate[k]);
+        if (g.dgate && a.gate_kind == HOARD_GATE_CHANNEL)
+            put(alone ? static_cast<float *>(g.dgate) : p, c[k], a.n, s_gate[k]);
     }
 }
 
@@ -422,17 +425,17 @@ hipError_t launch_norm(const hoard_norm_args &a, hipStream_t s) {
 }
 
 hipError_t launch_norm_grad(const hoard_norm_args &a, const hoard_norm_grads &g, float *work, hipStream_t s) {
-    if (a.n_rows) {
-        HOARD_NORM_TYPES(grad_of, a, g, work, s);
-        const hipError_t rc = hipGetLastError();
-        if (rc != hipSuccess) return rc;
-    }
     SumOut o{};
     int params = 0;
     if (g.dw_pre) o.out[params++] = g.dw_pre;
     if (g.dw_post) o.out[params++] = g.dw_post;
     if (g.dgate && a.gate_kind == HOARD_GATE_CHANNEL) o.out[params++] = static_cast<float *>(g.dgate);
-    if (!params) return hipSuccess;
+    if (a.n_rows) {
+        HOARD_NORM_TYPES(grad_of, a, g, work, s);
+        const hipError_t rc = hipGetLastError();
+        if (rc != hipSuccess) return rc;
+    }
+    if (!params || a.n_rows == 1) return hipSuccess;  // one row's sums were written in place
     norm_sum_kernel<<<dim3((a.n + 63) / 64, params), 1024, 0, s>>>(work, norm_groups(a.n_rows, a.n), a.n, o);
     return hipGetLastError();
 }

@@ -14,6 +14,7 @@ bool activation_type(int t) { return t == HOARD_TYPE_F32 || t == HOARD_TYPE_F16 
 size_t type_size(int t) { return t == HOARD_TYPE_F32 ? 4 : 2; }
 bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+constexpr int kMaxRows = 1 << 22;  // a launch's workgroups of 16 rows by 8 tiles of x within its 2^32 threads
 constexpr int kMaxCols = 1 << 20;  // 64 rows of x lie within the kernels' 32-bit offsets
 
 int launched(const char *what, hipError_t rc) {
@@ -28,6 +29,7 @@ int check_matrix(const char *what, const hoard_q4_matrix &m) {
     if (!m.codes || !m.scales) return fail_fmt(HOARD_ERR_INVALID, "%s: null codes or scales", what);
     if (!aligned(m.codes, 16)) return fail_fmt(HOARD_ERR_INVALID, "%s: codes are not 16-byte aligned", what);
     if (m.rows <= 0 || m.n_mat <= 0) return fail_fmt(HOARD_ERR_INVALID, "%s: rows %d, n_mat %d", what, m.rows, m.n_mat);
+    if (m.rows > kMaxRows) return fail_fmt(HOARD_ERR_UNSUPPORTED, "%s: rows %d above %d", what, m.rows, kMaxRows);
     if (m.group != 32 && m.group != 64 && m.group != 128)
         return fail_fmt(HOARD_ERR_UNSUPPORTED, "%s: group %d is not 32, 64 or 128", what, m.group);
     if (m.cols <= 0 || m.cols % m.group)

@@ -5,8 +5,9 @@
 // experts, plus those of its own expert in earlier blocks, plus its rank among
 // its own block's.  The rank within a wave comes from ballots over the bits of
 // the expert id, the one across the block's waves from their counts in LDS.
-// Up to one block of pairs that is one launch; above it a launch of counts
-// comes first, and each block adds up what precedes it.
+// One block of pairs is one launch; above it a launch of counts comes first.  Up to
+// kAddBlocks each block adds up what precedes it, which is one launch less; above, the
+// counts are summed along the blocks by a launch between the two.
 #include "ops.h"
 #include "opsdev.h"
 
@@ -17,6 +18,7 @@ namespace {
 constexpr int kBlockPairs = 1024;
 constexpr int kMaxExperts = 1024;
 constexpr int kWaves = kBlockPairs / 64;
+constexpr int kAddBlocks = 64;
 
 // The lanes of the wave that hold the same key (of `bits` bits), as a mask.
 __device__ __forceinline__ uint64_t same_key(int key, int bits) {
@@ -46,7 +48,30 @@ __global__ __launch_bounds__(kBlockPairs) void count_kernel(PairsArgs a, int64_t
     for (int e = threadIdx.x; e < a.n_expert; e += kBlockPairs) a.work[(size_t)blockIdx.x * a.n_expert + e] = cnt[e];
 }
 
-// blocks > 1: a.work holds every block's counts.
+// a.work[b][e]: the counts of blocks 0..b.  A workgroup takes 64 experts, its 16 waves
+// a sixteenth of the blocks each: their sums first, then the running ones.
+__global__ __launch_bounds__(1024) void scan_kernel(PairsArgs a, int blocks) {
+    __shared__ int sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+    const int per = (blocks + 15) / 16, b0 = min(blocks, wave * per), b1 = min(blocks, b0 + per);
+    int s = 0;
+    if (e < a.n_expert) {
+#pragma unroll 8
+        for (int b = b0; b < b1; b++) s += a.work[(size_t)b * a.n_expert + e];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (e >= a.n_expert) return;
+    s = 0;
+    for (int w = 0; w < wave; w++) s += sums[w][lane];
+#pragma unroll 8
+    for (int b = b0; b < b1; b++) {
+        s += a.work[(size_t)b * a.n_expert + e];
+        a.work[(size_t)b * a.n_expert + e] = s;
+    }
+}
+
+// blocks > 1: a.work holds every block's counts, or their running sums (above kAddBlocks).
 __global__ __launch_bounds__(kBlockPairs) void place_kernel(PairsArgs a, int64_t pairs, int bits) {
     __shared__ uint16_t of_wave[kWaves][kMaxExperts + 1];  // pairs of each expert in each wave, then before it
     __shared__ int base[kMaxExperts + 1];                  // the block's first row of each expert
@@ -72,6 +97,9 @@ __global__ __launch_bounds__(kBlockPairs) void place_kernel(PairsArgs a, int64_t
         }
         if (blocks == 1) {
             total = mine;
+        } else if (blocks > kAddBlocks) {
+            total = a.work[(size_t)(blocks - 1) * E + tid];
+            earlier = blockIdx.x ? a.work[(size_t)(blockIdx.x - 1) * E + tid] : 0;
         } else {
 #pragma unroll 8
             for (int b = 0; b < blocks; b++) {
@@ -279,6 +307,11 @@ hipError_t launch_sort_pairs(const PairsArgs &a, hipStream_t s) {
     while ((1 << bits) <= a.n_expert) bits++;  // keys 0..n_expert
     if (blocks > 1) {
         count_kernel<<<blocks, kBlockPairs, 0, s>>>(a, pairs);
+        const hipError_t rc = hipGetLastError();
+        if (rc != hipSuccess) return rc;
+    }
+    if (blocks > kAddBlocks) {
+        scan_kernel<<<(a.n_expert + 63) / 64, 1024, 0, s>>>(a, blocks);
         const hipError_t rc = hipGetLastError();
         if (rc != hipSuccess) return rc;
     }

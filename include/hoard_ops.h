@@ -42,7 +42,7 @@ extern "C" {
 
 /* n_mat matrices of rows x cols weights, row r of matrix e at index e*rows + r:
    weight k = scale[k / group] * (code[k] - zero[k / group]), zero 8 without
-   zeros.  cols is a multiple of group, at most 2^20. */
+   zeros.  rows is at most 2^22; cols is a multiple of group, at most 2^20. */
 typedef struct hoard_q4_matrix {
     const void *codes;    /* [n_mat*rows][cols/2] bytes, 16-byte aligned: byte j holds code 2j in
                              its low half and code 2j+1 in its high half */
@@ -57,9 +57,11 @@ typedef struct hoard_q4_matrix {
 /* y[r] = W x[r] for n_rows rows: x [n_rows][cols] and y [n_rows][rows] of `type`,
    x 16-byte aligned.  With `up` (same rows, cols, group and n_mat; its zeros and
    scale type may differ) y[r] = silu(W x[r]) * (W_up x[r]).  W has n_mat 1.  The
-   products are formed with the activations as given, not quantised.  A row of x
-   that holds an infinity or a NaN gives a row of y without a defined value
-   (infinities and NaN); other rows are not touched by it. */
+   products are formed with the activations as given, not quantised; their sums are
+   of codes plus an offset of up to 1024 and are corrected, so they overflow where the
+   sum of |x| over a group reaches 2^117.  A row of x that holds an infinity or a NaN
+   gives a row of y without a defined value (infinities and NaN); other rows are not
+   touched by it. */
 int hoard_q4_matmul(const hoard_q4_matrix *w, const hoard_q4_matrix *up, int type, int n_rows, const void *x,
                     void *y, void *stream);
 

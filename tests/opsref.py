@@ -43,12 +43,18 @@ def dense(codes, scales, zeros):
 def product(x, m, e):
     """(value, bound before storing) of x [r, cols] times matrix e of m = (codes, scales, zeros).
 
-    The kernel may form a group's sum of (16 + q) x less (16 + z) times the sum of x: the terms' magnitudes are then at
-    most (32 + z) |x| and the two sums, their difference and its use add a few roundings to those of the sum itself."""
+    The kernels may form a group's sum of (B + q) x less (B + z) times the sum of x, B up to 16 for fp32 activations
+    (split into three parts, so three terms a column), 128 for bf16 and 1024 for f16: both sums, of magnitudes up to
+    (B + q) |x| and (B + z) |x|, round once a term and a few times more, their difference is scaled, and the groups'
+    sums, now of magnitudes |q - z| |s| |x|, are added."""
     w, q, z, s = (t[e] for t in dense(*m)) if m[0].dim() == 3 else dense(*m)
+    groups = m[1].shape[-1]
+    group = q.shape[-1] // groups
+    bias, terms = {torch.float32: (16, 3), torch.bfloat16: (128, 1), torch.float16: (1024, 1)}[x.dtype]
     x = x.cpu().to(torch.float64)
-    mag = x.abs() @ ((q + z + 32.0) * s.abs()).t()
-    return x @ w.t(), mag * (x.shape[1] + 8) * U32
+    inner = x.abs() @ ((2 * bias + q + z) * s.abs()).t()
+    outer = x.abs() @ w.abs().t()
+    return x @ w.t(), ((terms * group + 8) * inner + (groups + 16) * outer) * U32
 
 
 def swiglu(g, bg, up, bu):

@@ -81,6 +81,10 @@ CASES = [
     dict(m=4, n=300, dtype=BF16, res=F32, block=False), dict(m=4, n=300, dtype=F32, res=F32, block=False, offset=1.0),
     dict(m=4, n=300, dtype=BF16, res=BF16, post=False, pre=False), dict(m=4, n=300, dtype=F16, res=F16, post=False, gate="token"),
     dict(m=4, n=300, dtype=BF16, res=F32, pre=False, gate="channel", sigmoid=True), dict(m=4, n=2048, dtype=F32, res=F32, post=False),
+    # one row, whose sums over the rows need none
+    dict(m=1, n=1500, dtype=F32, res=F32, gate="channel"), dict(m=1, n=9001, dtype=BF16, res=F32, gate="channel", sigmoid=True),
+    # more rows than groups
+    dict(m=3000, n=24, dtype=F32, res=F32, gate="channel"), dict(m=1600, n=1100, dtype=BF16, res=BF16, gate="channel"),
     # rows of zeros
     dict(m=6, n=320, dtype=BF16, res=F32, gate="channel", zero_row=True),
 ]

@@ -24,7 +24,7 @@ def make_ids(seed, tokens, k, experts, drop=0.0, skew=False):
 
 SORTS = [(0, 8, 4, 0.0), (1, 1, 1, 0.0), (1, 8, 128, 0.0), (1, 64, 3, 0.1), (5, 3, 1024, 0.0), (16, 8, 128, 0.3),
          (127, 8, 64, 0.0), (128, 8, 64, 0.0), (129, 8, 64, 0.0), (341, 3, 1000, 0.2), (512, 10, 512, 0.0),
-         (700, 7, 2, 0.5), (2048, 8, 127, 0.0), (5001, 8, 1024, 0.1), (20000, 4, 60, 0.0), (40000, 5, 256, 1.0)]
+         (700, 7, 2, 0.5), (2048, 8, 127, 0.0), (8192, 8, 1000, 0.1), (8193, 8, 3, 0.0), (66000, 1, 65, 0.2), (5001, 8, 1024, 0.1), (20000, 4, 60, 0.0), (40000, 5, 256, 1.0)]
 
 
 @pytest.mark.parametrize("tokens,k,experts,drop", SORTS)

@@ -182,6 +182,61 @@ def test_rows_apart(n, dtype):
     assert torch.equal(y[3:], clean[3:])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tokens,k,experts,rows,cols,group,up", [
+    (3, 2, 40, 96, 256, 64, False), (40, 4, 16, 200, 384, 128, True), (300, 2, 5, 130, 256, 32, True),
+    (64, 3, 200, 64, 160, 32, False), (1200, 1, 6, 256, 128, 64, False)])
+def test_sorted_routed(tokens, k, experts, rows, cols, group, up, dtype):
+    """The sizes at which a sorted call takes another form: few rows, many small runs, long runs, many matrices."""
+    from hoard_amd.ops import q4_matmul, sort_pairs
+    w = weights(91, experts, rows, cols, group, BF16, True)
+    u = weights(92, experts, rows, cols, group, F16) if up else None
+    s = sort_pairs(routing(93, tokens, k, experts).cuda(), experts)
+    x = rows_of(94, tokens * k, cols, dtype)
+    y = q4_matmul(x, op(w), op(u) if up else None, offsets=s.offsets)
+    off = s.offsets.tolist()
+    for e in range(experts):
+        if off[e + 1] > off[e]:
+            R.close(y[off[e]:off[e + 1]], *expect(x[off[e]:off[e + 1]], w, u, e), f"expert {e}")
+
+
+@pytest.mark.parametrize("n,rows,cols,group,dtype", [
+    (16, 12400, 128, 64, BF16), (9, 12400, 128, 64, F32), (30, 4200, 160, 32, BF16), (48, 2100, 256, 128, F16),
+    (150, 700, 256, 64, BF16), (300, 600, 384, 128, F16), (600, 520, 128, 32, BF16), (700, 3000, 64, 32, F32),
+    (1, 4100, 96, 32, F32), (90, 1100, 224, 32, F32), (1100, 2050, 64, 64, F16)])
+def test_dense_forms(n, rows, cols, group, dtype):
+    """The sizes at which a dense call takes another form, and odd ones beside them."""
+    from hoard_amd.ops import q4_matmul
+    w = weights(95, 0, rows, cols, group, F32, True)
+    x = rows_of(96, n, cols, dtype)
+    R.close(q4_matmul(x, op(w)), *expect(x, w, None), "y")
+
+
+def test_graphs():
+    """Three forms captured and replayed with eager work between, each replay the eager result."""
+    from hoard_amd.ops import q4_matmul
+    w, many = op(weights(97, 0, 300, 512, 128)), op(weights(98, 4, 300, 512, 128))
+    ids = torch.tensor([[3, 1], [0, 2]], dtype=torch.int32).cuda()
+    offsets = torch.tensor([0, 5, 5, 80, 99], dtype=torch.int32).cuda()
+    x = {n: rows_of(99 + n, n, 512, BF16) for n in (1, 2, 30, 99)}
+    calls = [lambda: q4_matmul(x[1], w), lambda: q4_matmul(x[30], w), lambda: q4_matmul(x[2], many, ids=ids),
+             lambda: q4_matmul(x[99], many, many, offsets=offsets)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = [c() for c in calls]
+    for r in range(4):
+        for t in got:
+            t.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), r
+        calls[r]()
+        torch.empty(1 << 16, device="cuda").normal_().sum().item()
+
+
 def test_deterministic_and_streams():
     from hoard_amd.ops import q4_matmul
     w, u = op(weights(61, 0, 300, 1024, 128)), op(weights(62, 0, 300, 1024, 128))

@@ -23,7 +23,7 @@ def refused(rc, code, *words):
 @pytest.mark.parametrize("field,value,code,word", [
     ("codes", None, H.ERR_INVALID, "null"), ("codes", A + 8, H.ERR_INVALID, "16-byte"),
     ("scales", None, H.ERR_INVALID, "null"), ("scales", A + 1, H.ERR_INVALID, "aligned"),
-    ("rows", 0, H.ERR_INVALID, "rows"), ("rows", -4, H.ERR_INVALID, "rows"),
+    ("rows", (1 << 22) + 1, H.ERR_UNSUPPORTED, "rows"), ("rows", 0, H.ERR_INVALID, "rows"), ("rows", -4, H.ERR_INVALID, "rows"),
     ("cols", 0, H.ERR_INVALID, "cols"), ("cols", 192, H.ERR_INVALID, "cols"), ("cols", 100, H.ERR_INVALID, "cols"),
     ("cols", (1 << 20) + 128, H.ERR_UNSUPPORTED, "cols"), ("group", 16, H.ERR_UNSUPPORTED, "group"), ("group", 0, H.ERR_UNSUPPORTED, "group"),
     ("group", 256, H.ERR_UNSUPPORTED, "group"), ("n_mat", 0, H.ERR_INVALID, "n_mat"),
