@@ -191,7 +191,7 @@ def sort_combine(y, place, w=None, res=None, *, out=None):
 
 
 def sort_combine_grad(dout, y, place, w, *, dy=None):
-    """(dy, dw) of sort_combine; rows of dy that no pair names are left as they are (zero in a new tensor)."""
+    """(dy, dw) of sort_combine; rows of dy that no pair names are left as they are (zero in a new tensor); dy may be y."""
     dt, m, k, n = _rows("y", y, place, w, lambda m, k: m * k)
     _need(w is not None, "w: wanted")
     _tensor("dout", dout, (m, n), y.dtype, y.device)

@@ -110,7 +110,7 @@ int hoard_sort_combine(int type, int n_tokens, int k, int n, const void *y, cons
 /* Gradients of hoard_sort_combine given dout [n_tokens][n] (that of res is dout
    itself): dy[place[t][j]] = w[t][j] * dout[t] and dw[t][j] = <dout[t],
    y[place[t][j]]>; dw is 0 for a dropped pair, and rows of dy that no pair names
-   are left as they are.  dy may be NULL (not wanted). */
+   are left as they are.  dy may be NULL (not wanted), or y. */
 int hoard_sort_combine_grad(int type, int n_tokens, int k, int n, const void *dout, const void *y,
                             const int32_t *place, const float *w, void *dy, float *dw, void *stream);
 

@@ -142,6 +142,19 @@ def test_combine_grad(tokens, k, experts, n, dtype, drop, off):
     R.close(dw.reshape(-1), ww, wb, "dw")
 
 
+@pytest.mark.parametrize("n", [5, 64, 2047, 2049, 5003])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_combine_grad_in_place(n, dtype):
+    """dy over y."""
+    from hoard_amd.ops import sort_combine_grad, sort_pairs
+    tokens, k = 30, 5
+    s = sort_pairs(make_ids(50, tokens, k, 9, 0.1).cuda(), 9)
+    y, w, dout = data(51, tokens * k, n, dtype=dtype), data(52, tokens, k, dtype=F32), data(53, tokens, n, dtype=dtype)
+    dy, dw = sort_combine_grad(dout, y, s.place, w, dy=y.clone())
+    got, dw2 = sort_combine_grad(dout, y, s.place, w, dy=y)
+    assert got is y and torch.equal(got, dy) and torch.equal(dw, dw2)
+
+
 def test_gather_and_combine_are_adjoint():
     """<gather(x), g> = <x, combine(g)>, the gradient of each by the other, and dw against differences."""
     from hoard_amd.ops import sort_combine, sort_combine_grad, sort_gather, sort_pairs
