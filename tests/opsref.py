@@ -47,7 +47,9 @@ def product(x, m, e):
     (split into three parts, so three terms a column), 128 for bf16 and 1024 for f16: both sums, of magnitudes up to
     (B + q) |x| and (B + z) |x|, round once a term and a few times more, their difference is scaled, and the groups'
     sums, now of magnitudes |q - z| |s| |x|, are added."""
-    w, q, z, s = (t[e] for t in dense(*m)) if m[0].dim() == 3 else dense(*m)
+    if m[0].dim() == 3:
+        m = tuple(t[e] if t is not None else None for t in m)
+    w, q, z, s = dense(*m)
     groups = m[1].shape[-1]
     group = q.shape[-1] // groups
     bias, terms = {torch.float32: (16, 3), torch.bfloat16: (128, 1), torch.float16: (1024, 1)}[x.dtype]

@@ -185,7 +185,9 @@ def test_rows_apart(n, dtype):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("tokens,k,experts,rows,cols,group,up", [
     (3, 2, 40, 96, 256, 64, False), (40, 4, 16, 200, 384, 128, True), (300, 2, 5, 130, 256, 32, True),
-    (64, 3, 200, 64, 160, 32, False), (1200, 1, 6, 256, 128, 64, False)])
+    (64, 3, 200, 64, 160, 32, False), (1200, 1, 6, 256, 128, 64, False), (200, 4, 100, 600, 128, 64, False),
+    (900, 4, 20, 1000, 96, 32, False), (100, 4, 20, 2000, 128, 128, False), (130, 4, 60, 500, 224, 32, True),
+    (500, 4, 10, 520, 128, 128, True)])
 def test_sorted_routed(tokens, k, experts, rows, cols, group, up, dtype):
     """The sizes at which a sorted call takes another form: few rows, many small runs, long runs, many matrices."""
     from hoard_amd.ops import q4_matmul, sort_pairs
@@ -200,16 +202,19 @@ def test_sorted_routed(tokens, k, experts, rows, cols, group, up, dtype):
             R.close(y[off[e]:off[e + 1]], *expect(x[off[e]:off[e + 1]], w, u, e), f"expert {e}")
 
 
+@pytest.mark.parametrize("up", [False, True])
 @pytest.mark.parametrize("n,rows,cols,group,dtype", [
     (16, 12400, 128, 64, BF16), (9, 12400, 128, 64, F32), (30, 4200, 160, 32, BF16), (48, 2100, 256, 128, F16),
     (150, 700, 256, 64, BF16), (300, 600, 384, 128, F16), (600, 520, 128, 32, BF16), (700, 3000, 64, 32, F32),
-    (1, 4100, 96, 32, F32), (90, 1100, 224, 32, F32), (1100, 2050, 64, 64, F16)])
-def test_dense_forms(n, rows, cols, group, dtype):
+    (1, 4100, 96, 32, F32), (90, 1100, 224, 32, F32), (1100, 2050, 64, 64, F16), (600, 1100, 352, 32, BF16),
+    (800, 2050, 320, 64, F16), (300, 1000, 288, 32, F32), (300, 560, 1152, 128, BF16)])
+def test_dense_forms(n, rows, cols, group, dtype, up):
     """The sizes at which a dense call takes another form, and odd ones beside them."""
     from hoard_amd.ops import q4_matmul
     w = weights(95, 0, rows, cols, group, F32, True)
+    u = weights(90, 0, rows, cols, group, F16) if up else None
     x = rows_of(96, n, cols, dtype)
-    R.close(q4_matmul(x, op(w)), *expect(x, w, None), "y")
+    R.close(q4_matmul(x, op(w), op(u) if up else None), *expect(x, w, u), "y")
 
 
 def test_graphs():
