@@ -48,6 +48,32 @@ __device__ __forceinline__ v4f mfma_16x16x32<f16>(v4u x, v4u w, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, w), c, 0, 0, 0);
 }
 
+// Waits out the last matrix instruction before its result is read (8 wait states).  The
+// compiler counts them itself, but not over a branch: with the rows' early exit between
+// the product and its use, it read accumulators that were not there yet.  In bf16 that
+// costs 1 to 8 % (most with groups of 32), where the compiler puts other tiles' products
+// between; there its order happens to be safe, which nothing guarantees.
+// All accumulators go through one statement, which so follows all their products.
+__device__ __forceinline__ void settle(v4f (&d)[1]) { asm volatile("s_nop 7" : "+v"(d[0])); }
+__device__ __forceinline__ void settle(v4f (&d)[2]) { asm volatile("s_nop 7" : "+v"(d[0]), "+v"(d[1])); }
+__device__ __forceinline__ void settle(v4f (&d)[2], v4f &xs) {
+    asm volatile("s_nop 7" : "+v"(d[0]), "+v"(d[1]), "+v"(xs));
+}
+
+// f16 holds code - zero exactly (11 bits, the zero point being a byte), so there the
+// offset is taken off in pairs and no sums of x are needed: 4 instructions for 8 codes
+// in place of a product with ones, or of sums formed beside x (2000 rows of x by 8192
+// x 4096 in groups of 32: 243 us against 284; 512 rows by 4096 x 4096: 29.8 against 32.2).
+template <typename E>
+constexpr bool kExact = __is_same(E, f16);
+__device__ __forceinline__ v4u less(v4u w, float offset) {
+    const f16 o = (f16)-offset;
+    const v2h pair = {o, o};
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, (uint32_t)w[i]) + pair);
+    return w;
+}
+
 // Four words of a lane rearranged among the four lanes (16 apart) of a row of W.
 template <int G>
 __device__ __forceinline__ v4u exchange(v4u c) {
@@ -177,7 +203,7 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
     constexpr int SPC = SC / XS, SI = RW * SC / THREADS;
     static_assert(SC % XS == 0 && RW * SC % THREADS == 0 && SC % SI == 0, "whole steps, whole shares");
     __shared__ __align__(16) uint8_t lds[XBYTES > MEET ? XBYTES : MEET];
-    __shared__ __align__(16) float sums[XS][TM];
+    __shared__ __align__(16) float sums[kExact<E> ? 1 : XS][kExact<E> ? 4 : TM];
     __shared__ float scale[RW][SC + 1], zero[RW][SC + 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
@@ -269,9 +295,10 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
             if constexpr (PL == 1) {
                 v4u w;
                 __builtin_memcpy(&w, &xr[j], 16);
+                *reinterpret_cast<v4u *>(to) = paired(w);
+                if (kExact<E>) continue;
 #pragma unroll
                 for (int c = 0; c < 4; c++) s = dot2<E>(w[c], kOnes<E>, s);
-                *reinterpret_cast<v4u *>(to) = paired(w);
             } else {
                 uint32_t part[3][8];
 #pragma unroll
@@ -337,16 +364,21 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
 #pragma unroll
                 for (int p = 0; p < P; p++)
 #pragma unroll
-                    for (int i = 0; i < SP; i++) w[p][i] = biased<E>(now[p][b][g * SP + i]);
+                    for (int i = 0; i < SP; i++) {
+                        w[p][i] = biased<E>(now[p][b][g * SP + i]);
+                        if (kExact<E>) w[p][i] = less(w[p][i], zc[p]);
+                    }
 #pragma unroll
                 for (int t = 0; t < MT; t++) {
                     if (t * 16 >= rows) break;
-                    const v4f xs = *reinterpret_cast<const v4f *>(&sums[(ks * KB + b) * NG + g][t * 16 + 4 * q]);
-                    v4f d[P];
+                    v4f d[P] = {};
+                    if constexpr (!kExact<E>) {
+                        const v4f xs = *reinterpret_cast<const v4f *>(&sums[(ks * KB + b) * NG + g][t * 16 + 4 * q]);
 #pragma unroll
-                    for (int p = 0; p < P; p++)
+                        for (int p = 0; p < P; p++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) d[p][i] = -zc[p] * xs[i];
+                            for (int i = 0; i < 4; i++) d[p][i] = -zc[p] * xs[i];
+                    }
                     const uint8_t *from = lds + (t * 16 + col) * RS + (ks * KB + b) * 256;
 #pragma unroll
                     for (int i = 0; i < SP; i++)
@@ -356,6 +388,7 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
 #pragma unroll
                             for (int p = 0; p < P; p++) d[p] = mfma_16x16x32<E>(x, w[p][i], d[p]);
                         }
+                    settle(d);
 #pragma unroll
                     for (int p = 0; p < P; p++)
 #pragma unroll
@@ -409,9 +442,9 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
 }
 
 // The same product for 16-bit activations and many rows of x: x goes straight from
-// memory to LDS in its own order, the codes take that order (in_order), and the sums
-// of x come from a third product with a matrix of ones, whose accumulator holds them
-// where the scaled sums need them.  A step is 128 columns; x lies in two buffers, so
+// memory to LDS in its own order, the codes take that order (in_order), and in bf16 the
+// sums of x come from a third product with a matrix of ones, whose accumulator holds
+// them where the scaled sums need them.  A step is 128 columns; x lies in two buffers, so
 // one barrier a step hands over what arrived and frees what was read.
 //
 // A row of x is 256 bytes of a buffer, its 16-byte pieces exchanged by the row's
@@ -516,7 +549,10 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_flow_kernel(Q4Args a) {
                 sc[p] = scale[(p * NW + nw) * 16 + col][(step % SPC) * XS + ks * NG + g];
                 zc[p] = zero[(p * NW + nw) * 16 + col][(step % SPC) * XS + ks * NG + g];
 #pragma unroll
-                for (int i = 0; i < SP; i++) w[p][i] = in_order<T>(now[p][g * SP + i]);
+                for (int i = 0; i < SP; i++) {
+                    w[p][i] = in_order<T>(now[p][g * SP + i]);
+                    if (kExact<T>) w[p][i] = less(w[p][i], zc[p]);
+                }
             }
 #pragma unroll
             for (int t = 0; t < MT; t++) {
@@ -526,15 +562,17 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_flow_kernel(Q4Args a) {
 #pragma unroll
                 for (int i = 0; i < SP; i++) {
                     const v4u x = *reinterpret_cast<const v4u *>(from + (((column_of<G>(g * SP + i, q) / 8) ^ col) * 16));
-                    xs = mfma_16x16x32<T>(x, ones, xs);
+                    if (!kExact<T>) xs = mfma_16x16x32<T>(x, ones, xs);
 #pragma unroll
                     for (int p = 0; p < P; p++) d[p] = mfma_16x16x32<T>(x, w[p][i], d[p]);
                 }
+                if constexpr (kExact<T>) settle(d);
+                else settle(d, xs);
 #pragma unroll
                 for (int p = 0; p < P; p++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        acc[p][t][i] = fmaf(sc[p], fmaf(-zc[p], xs[i], d[p][i]), acc[p][t][i]);
+                        acc[p][t][i] = fmaf(sc[p], kExact<T> ? d[p][i] : fmaf(-zc[p], xs[i], d[p][i]), acc[p][t][i]);
             }
         }
     };
