@@ -2,9 +2,9 @@
 //
 // A workgroup takes a tile of up to 16 MT rows of x (of one matrix) and NW * 16 P
 // rows of W (NW * 16 of both matrices with a second one).  Its waves are NW wide
-// over the rows of W and KS deep over the columns; the KS partial sums meet in
-// LDS.  Codes go from memory to registers, each read by one wave, one step of
-// KB * 128 columns ahead; x goes through LDS once per workgroup and step.
+// over the rows of W and KS deep over the columns, 128 a step; the KS partial sums
+// meet in LDS.  Codes go from memory to registers, each read by one wave, two steps
+// ahead; x goes through LDS once per workgroup and step.
 //
 // x is the A operand and W the B operand: a lane then holds one row of W, its
 // scale and zero point, and 4 rows of x in an accumulator.  A lane reads 32
@@ -183,16 +183,16 @@ __device__ __forceinline__ bool tile_of(const Q4Args &a, int64_t t, int tm, int 
     return rows > 0;
 }
 
-template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB, int MW>
+template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int MW>
 __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
     typedef typename Tiles<T>::elem E;
     constexpr int PL = Tiles<T>::planes, TM = 16 * MT, THREADS = 64 * NW * KS;
     constexpr int NG = 128 / G, SP = 4 / NG;               // groups in a block of 128 columns, steps in a group
-    constexpr int COLS = KS * KB * 128;                    // columns of a step of the workgroup
+    constexpr int COLS = KS * 128;                         // columns of a step of the workgroup
     constexpr int RS = COLS * 2 + 16;                      // bytes of a row of x in LDS: 16 off the banks' period
     constexpr int XP = TM * (COLS / 8) / THREADS;          // pieces of 8 values a thread stages
     constexpr int XROWS = THREADS / (COLS / 8);            // rows of x between them
-    constexpr int XS = KS * KB * NG;                       // groups of a step
+    constexpr int XS = KS * NG;                            // groups of a step
     constexpr int MEET = KS > 1 ? (KS - 1) * NW * P * MT * 1024 : 0;  // bytes of the partial sums
     static_assert(XROWS * (COLS / 8) == THREADS && XP * XROWS == TM, "whole pieces a thread, whole rows between them");
     static_assert(!UP || P == 2, "the second matrix is the second stream");
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
     const int tn = run % nt;
     const int64_t tx = a.tile0 + (a.spread ? (run / nt) * 8 + (id & 7) : run / nt);
     if (!tile_of(a, tx, TM, e, r0, rows)) return;
-    const int cols = a.w.cols, blocks = (cols + 127) / 128, steps = (blocks + KS * KB - 1) / (KS * KB);
+    const int cols = a.w.cols, blocks = (cols + 127) / 128, steps = (blocks + KS - 1) / KS;
     constexpr int WIDE = UP ? 16 : 16 * P;  // rows of W of a wave
     const int first = (tn * NW + nw) * WIDE, n0 = first + col;
 
@@ -239,18 +239,16 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
     // staging x waits for nothing behind it.  Nothing is loaded under a condition: what
     // lies behind the last column or row is read from a place inside instead, x is
     // zeroed behind the last column, and rows behind the last are not stored.
-    v4u codes[2][P][KB];
+    v4u codes[2][P];
     Piece<T> xr[XP];
     auto fetch_w = [&](auto at, int step) {
         constexpr int B = decltype(at)::value;
-        const int block = (step * KS + ks) * KB;
+        const int block = step * KS + ks;
 #pragma unroll
         for (int p = 0; p < P; p++) {
             const hoard_q4_matrix &m = UP && p == 1 ? a.up : a.w;
             const uint8_t *const from = static_cast<const uint8_t *>(m.codes) + row0 * (cols / 2);
-#pragma unroll
-            for (int b = 0; b < KB; b++)
-                codes[B][p][b] = *reinterpret_cast<const v4u *>(from + (code[p] + min(block + b, last_block) * 64));
+            codes[B][p] = *reinterpret_cast<const v4u *>(from + (code[p] + min(block, last_block) * 64));
         }
     };
     // the scales of SC groups into LDS: read along the rows, as they lie in memory
@@ -341,59 +339,54 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
         if (step) __syncthreads();  // the last step's x has been read
         if (step % SPC == 0) stage_scales(step / SPC);
         stage(step);
-        v4u now[P][KB];
+        v4u now[P];
 #pragma unroll
-        for (int p = 0; p < P; p++)
-#pragma unroll
-            for (int b = 0; b < KB; b++) now[p][b] = exchange<G>(codes[B][p][b]);
+        for (int p = 0; p < P; p++) now[p] = exchange<G>(codes[B][p]);
         __syncthreads();
         if (step + 1 < steps) fetch_x(step + 1);
         if (step + 2 < steps) fetch_w(at, step + 2);
 #pragma unroll
-        for (int b = 0; b < KB; b++) {
+        for (int g = 0; g < NG; g++) {
+            v4u w[P][SP];
+            float sc[P], zc[P];
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                v4u w[P][SP];
-                float sc[P], zc[P];
+            for (int p = 0; p < P; p++) {
+                const int at = (step % SPC) * XS + ks * NG + g;
+                sc[p] = scale[(p * NW + nw) * 16 + col][at];
+                zc[p] = zero[(p * NW + nw) * 16 + col][at];
+            }
 #pragma unroll
-                for (int p = 0; p < P; p++) {
-                    const int at = (step % SPC) * XS + (ks * KB + b) * NG + g;
-                    sc[p] = scale[(p * NW + nw) * 16 + col][at];
-                    zc[p] = zero[(p * NW + nw) * 16 + col][at];
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int i = 0; i < SP; i++) {
+                    w[p][i] = biased<E>(now[p][g * SP + i]);
+                    if (kExact<E>) w[p][i] = less(w[p][i], zc[p]);
                 }
 #pragma unroll
-                for (int p = 0; p < P; p++)
-#pragma unroll
-                    for (int i = 0; i < SP; i++) {
-                        w[p][i] = biased<E>(now[p][b][g * SP + i]);
-                        if (kExact<E>) w[p][i] = less(w[p][i], zc[p]);
-                    }
-#pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    if (t * 16 >= rows) break;
-                    v4f d[P] = {};
-                    if constexpr (!kExact<E>) {
-                        const v4f xs = *reinterpret_cast<const v4f *>(&sums[(ks * KB + b) * NG + g][t * 16 + 4 * q]);
-#pragma unroll
-                        for (int p = 0; p < P; p++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) d[p][i] = -zc[p] * xs[i];
-                    }
-                    const uint8_t *from = lds + (t * 16 + col) * RS + (ks * KB + b) * 256;
-#pragma unroll
-                    for (int i = 0; i < SP; i++)
-#pragma unroll
-                        for (int l = 0; l < PL; l++) {
-                            const v4u x = *reinterpret_cast<const v4u *>(from + l * TM * RS + 2 * column_of<G>(g * SP + i, q));
-#pragma unroll
-                            for (int p = 0; p < P; p++) d[p] = mfma_16x16x32<E>(x, w[p][i], d[p]);
-                        }
-                    settle(d);
+            for (int t = 0; t < MT; t++) {
+                if (t * 16 >= rows) break;
+                v4f d[P] = {};
+                if constexpr (!kExact<E>) {
+                    const v4f xs = *reinterpret_cast<const v4f *>(&sums[ks * NG + g][t * 16 + 4 * q]);
 #pragma unroll
                     for (int p = 0; p < P; p++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) acc[p][t][i] = fmaf(sc[p], d[p][i], acc[p][t][i]);
+                        for (int i = 0; i < 4; i++) d[p][i] = -zc[p] * xs[i];
                 }
+                const uint8_t *from = lds + (t * 16 + col) * RS + ks * 256;
+#pragma unroll
+                for (int i = 0; i < SP; i++)
+#pragma unroll
+                    for (int l = 0; l < PL; l++) {
+                        const v4u x = *reinterpret_cast<const v4u *>(from + l * TM * RS + 2 * column_of<G>(g * SP + i, q));
+#pragma unroll
+                        for (int p = 0; p < P; p++) d[p] = mfma_16x16x32<E>(x, w[p][i], d[p]);
+                    }
+                settle(d);
+#pragma unroll
+                for (int p = 0; p < P; p++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[p][t][i] = fmaf(sc[p], d[p][i], acc[p][t][i]);
             }
         }
     };
@@ -642,10 +635,10 @@ hipError_t over_tiles(const Q4Args &a, F launch) {
     return hipSuccess;
 }
 
-template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int KB, int MW>
+template <typename T, int G, bool UP, int P, int MT, int NW, int KS, int MW>
 hipError_t launch_tiles_of(const Q4Args &a, hipStream_t s) {
     return over_tiles<16 * MT, NW *(UP ? 16 : 16 * P)>(a, [&](const Q4Args &part, unsigned grid) {
-        q4_tiles_kernel<T, G, UP, P, MT, NW, KS, KB, MW><<<grid, 64 * NW * KS, 0, s>>>(part);
+        q4_tiles_kernel<T, G, UP, P, MT, NW, KS, MW><<<grid, 64 * NW * KS, 0, s>>>(part);
     });
 }
 template <typename T, int G, bool UP, int MT, int NW, int KS, int MW>
@@ -690,27 +683,27 @@ hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
     constexpr int TN = UP ? 64 : 128;  // rows of W of a workgroup four wide
     if constexpr (sizeof(T) == 4) {
         if (sorted) {
-            if (groups(16, TN) <= kCUs / 2) return launch_tiles_of<T, G, UP, 2, 1, 1, 4, 1, 2>(a, s);
-            if (groups(16, TN) <= 2 * kCUs) return launch_tiles_of<T, G, UP, 2, 1, 2, 2, 1, 2>(a, s);
-            if (per <= 16) return launch_tiles_of<T, G, UP, 2, 1, 4, 1, 1, 2>(a, s);
-            return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 1, 2>(a, s);
+            if (groups(16, TN) <= kCUs / 2) return launch_tiles_of<T, G, UP, 2, 1, 1, 4, 2>(a, s);
+            if (groups(16, TN) <= 2 * kCUs) return launch_tiles_of<T, G, UP, 2, 1, 2, 2, 2>(a, s);
+            if (per <= 16) return launch_tiles_of<T, G, UP, 2, 1, 4, 1, 2>(a, s);
+            return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 2>(a, s);
         }
         if (per <= 16)
-            return groups(16, 16) <= 3 * kCUs ? launch_tiles_of<T, G, UP, 2, 1, 1, 8, 1, 2>(a, s)
-                                              : launch_tiles_of<T, G, UP, 2, 1, 1, 4, 1, 2>(a, s);
-        if (groups(32, 32) <= kCUs) return launch_tiles_of<T, G, UP, P, 2, 2, 4, 1, 2>(a, s);
-        if (groups(32, TN) <= kCUs) return launch_tiles_of<T, G, UP, 2, 2, 4, 2, 1, 2>(a, s);
-        return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 1, 2>(a, s);
+            return groups(16, 16) <= 3 * kCUs ? launch_tiles_of<T, G, UP, 2, 1, 1, 8, 2>(a, s)
+                                              : launch_tiles_of<T, G, UP, 2, 1, 1, 4, 2>(a, s);
+        if (groups(32, 32) <= kCUs) return launch_tiles_of<T, G, UP, P, 2, 2, 4, 2>(a, s);
+        if (groups(32, TN) <= kCUs) return launch_tiles_of<T, G, UP, 2, 2, 4, 2, 2>(a, s);
+        return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 2>(a, s);
     } else {
         if (sorted) {
-            if (groups(16, TN) <= kCUs / 2) return launch_tiles_of<T, G, UP, P, 1, 2, 4, 1, 2>(a, s);
+            if (groups(16, TN) <= kCUs / 2) return launch_tiles_of<T, G, UP, P, 1, 2, 4, 2>(a, s);
             if (groups(16, TN) <= 2 * kCUs) return launch_flow_of<T, G, UP, 1, 4, 2, 4>(a, s);
             return per <= 24 ? launch_flow_of<T, G, UP, 2, 4, 1, 4>(a, s) : launch_flow_of<T, G, UP, 4, 4, 1, 3>(a, s);
         }
         if (per <= 16)
-            return groups(16, 16) <= 3 * kCUs ? launch_tiles_of<T, G, UP, P, 1, 1, 8, 1, 2>(a, s)
-                                              : launch_tiles_of<T, G, UP, P, 1, 2, 4, 1, 2>(a, s);
-        if (groups(32, 16) <= kCUs) return launch_tiles_of<T, G, UP, P, 2, 1, 8, 1, 2>(a, s);
+            return groups(16, 16) <= 3 * kCUs ? launch_tiles_of<T, G, UP, P, 1, 1, 8, 2>(a, s)
+                                              : launch_tiles_of<T, G, UP, P, 1, 2, 4, 2>(a, s);
+        if (groups(32, 16) <= kCUs) return launch_tiles_of<T, G, UP, P, 2, 1, 8, 2>(a, s);
         if (groups(16, TN) <= kCUs) return launch_flow_of<T, G, UP, 1, 4, 4, 4>(a, s);
         if (groups(32, TN) <= kCUs) return launch_flow_of<T, G, UP, 2, 4, 4, 4>(a, s);
         if (groups(64, TN) <= kCUs) return launch_flow_of<T, G, UP, 4, 4, 2, 2>(a, s);
