@@ -14,8 +14,12 @@
 // exchanged between the lanes of a row (v_permlane32_swap, v_permlane16_swap) so
 // that a step never spans two groups.  A group's sum is scaled once it is whole.
 //
-// fp32 activations are split into three bf16 parts of 8 bits each (exactly x,
-// where x is no smaller than the smallest normal by 2^16), each a plane of its own.
+// fp32 activations are two f16 planes: a group of a row is multiplied by the power of
+// two that brings its largest value to 2^14, rounded, and what that leaves is rounded
+// again.  Their sum is x to 2^-24 of it, as one rounding to fp32, or to 2^-39 of the
+// group's largest value, whichever is more.  With f16's exact codes (below) the sums are
+// of the terms themselves; three bf16 planes, exactly x, had to correct sums of 16 + code
+// whose terms are five times the plain ones', and were four times further off.
 #pragma once
 
 #include <algorithm>
@@ -33,8 +37,8 @@ struct Tiles {
 };
 template <>
 struct Tiles<float> {
-    typedef bf16 elem;
-    static constexpr int planes = 3;
+    typedef f16 elem;
+    static constexpr int planes = 2;
 };
 
 template <typename E>
@@ -203,7 +207,9 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
     constexpr int SPC = SC / XS, SI = RW * SC / THREADS;
     static_assert(SC % XS == 0 && RW * SC % THREADS == 0 && SC % SI == 0, "whole steps, whole shares");
     __shared__ __align__(16) uint8_t lds[XBYTES > MEET ? XBYTES : MEET];
-    __shared__ __align__(16) float sums[kExact<E> ? 1 : XS][kExact<E> ? 4 : TM];
+    // of a row of x and group: its sum in bf16; in fp32 what undoes its power of two
+    constexpr bool SUMS = !kExact<E>, POWERS = PL == 2;
+    __shared__ __align__(16) float beside[SUMS || POWERS ? XS : 1][SUMS || POWERS ? TM : 4];
     __shared__ float scale[RW][SC + 1], zero[RW][SC + 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
@@ -275,7 +281,7 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
                 xr[j] = *reinterpret_cast<const Piece<T> *>(x0 + (uint32_t)(min(xrow + j * XROWS, rows - 1) * cols + k) *
                                                                      (uint32_t)sizeof(T));
     };
-    // x into LDS, and its sums over the groups
+    // x into LDS, and what stands beside it; a group's G / 8 pieces lie in consecutive lanes
     auto stage = [&](int step) {
         if ((step + 1) * COLS > cols) {
             const bool in = step * COLS + xcol < cols;
@@ -289,42 +295,45 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
             if (j * XROWS >= rows) break;
             const int row = xrow + j * XROWS, piece = xcol / 8;
             uint8_t *to = lds + row * RS + piece * 16;
-            float s = 0.0f;
+            float value;
             if constexpr (PL == 1) {
                 v4u w;
                 __builtin_memcpy(&w, &xr[j], 16);
                 *reinterpret_cast<v4u *>(to) = paired(w);
-                if (kExact<E>) continue;
+                if constexpr (!SUMS) continue;
+                value = 0.0f;
 #pragma unroll
-                for (int c = 0; c < 4; c++) s = dot2<E>(w[c], kOnes<E>, s);
+                for (int c = 0; c < 4; c++) value = dot2<E>(w[c], kOnes<E>, value);
+                value += dpp_f<kDppQuadXor1>(value);
+                value += dpp_f<kDppQuadXor2>(value);
+                if (G >= 64) value += dpp_f<kDppRowHalfMirror>(value);
+                if (G >= 128) value += dpp_f<kDppRowMirror>(value);
             } else {
-                uint32_t part[3][8];
+                // of magnitudes (a NaN's is above them all)
+                uint32_t most = 0;
+#pragma unroll
+                for (int c = 0; c < 8; c++) most = max(most, xr[j].w[c] & 0x7fffffffu);
+                most = max(most, __float_as_uint(dpp_f<kDppQuadXor1>(__uint_as_float(most))));
+                most = max(most, __float_as_uint(dpp_f<kDppQuadXor2>(__uint_as_float(most))));
+                if (G >= 64) most = max(most, __float_as_uint(dpp_f<kDppRowHalfMirror>(__uint_as_float(most))));
+                if (G >= 128) most = max(most, __float_as_uint(dpp_f<kDppRowMirror>(__uint_as_float(most))));
+                // 2^(141 - e) for the largest value's biased exponent e, and its inverse, both normal
+                const uint32_t up = min(268u - (most >> 23), 253u);
+                const float power = __uint_as_float(up << 23);
+                value = __uint_as_float((254u - up) << 23);
+                float x[8];
+                v8h high, low;
 #pragma unroll
                 for (int c = 0; c < 8; c++) {
-                    const uint32_t w = xr[j].w[c];
-                    const float x = __uint_as_float(w);
-                    s += x;
-                    // of an infinity or a NaN the first part says it all
-                    const float x1 = __uint_as_float(w & 0xffff0000u), rest = isfinite(x) ? x - x1 : 0.0f;
-                    const float x2 = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
-                    part[0][c] = __float_as_uint(x1) | (x != x ? 0x400000u : 0u);
-                    part[1][c] = __float_as_uint(x2);
-                    part[2][c] = __float_as_uint(rest - x2);
+                    x[c] = __uint_as_float(xr[j].w[c]) * power;
+                    high[(c & 3) * 2 + (c >> 2)] = (f16)x[c];
                 }
 #pragma unroll
-                for (int l = 0; l < 3; l++) {
-                    v4u w;
-#pragma unroll
-                    for (int c = 0; c < 4; c++) w[c] = __builtin_amdgcn_perm(part[l][c + 4], part[l][c], 0x07060302u);
-                    *reinterpret_cast<v4u *>(to + l * TM * RS) = w;
-                }
+                for (int c = 0; c < 8; c++) low[(c & 3) * 2 + (c >> 2)] = (f16)(x[c] - (float)high[(c & 3) * 2 + (c >> 2)]);
+                *reinterpret_cast<v8h *>(to) = high;
+                *reinterpret_cast<v8h *>(to + TM * RS) = low;
             }
-            // a group's G / 8 pieces lie in consecutive lanes
-            s += dpp_f<kDppQuadXor1>(s);
-            s += dpp_f<kDppQuadXor2>(s);
-            if (G >= 64) s += dpp_f<kDppRowHalfMirror>(s);
-            if (G >= 128) s += dpp_f<kDppRowMirror>(s);
-            if (piece % (G / 8) == 0) sums[piece / (G / 8)][row] = s;
+            if (piece % (G / 8) == 0) beside[piece / (G / 8)][row] = value;
         }
     };
 
@@ -365,9 +374,9 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
 #pragma unroll
             for (int t = 0; t < MT; t++) {
                 if (t * 16 >= rows) break;
-                v4f d[P] = {};
-                if constexpr (!kExact<E>) {
-                    const v4f xs = *reinterpret_cast<const v4f *>(&sums[ks * NG + g][t * 16 + 4 * q]);
+                v4f d[P] = {}, xs = (v4f)(1.0f);
+                if constexpr (SUMS || POWERS) xs = *reinterpret_cast<const v4f *>(&beside[ks * NG + g][t * 16 + 4 * q]);
+                if constexpr (SUMS) {
 #pragma unroll
                     for (int p = 0; p < P; p++)
 #pragma unroll
@@ -386,7 +395,8 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
 #pragma unroll
                 for (int p = 0; p < P; p++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[p][t][i] = fmaf(sc[p], d[p][i], acc[p][t][i]);
+                    for (int i = 0; i < 4; i++)
+                        acc[p][t][i] = fmaf(sc[p], POWERS ? d[p][i] * xs[i] : d[p][i], acc[p][t][i]);
             }
         }
     };

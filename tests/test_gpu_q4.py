@@ -217,6 +217,52 @@ def test_dense_forms(n, rows, cols, group, dtype, up):
     R.close(q4_matmul(x, op(w), op(u) if up else None), *expect(x, w, u), "y")
 
 
+def near_fp32(x, m):
+    """(value, bound) of fp32 products whose terms (q - z) x are formed without an offset.
+
+    x is held to 2^-24 of itself or 2^-39 of its group's largest magnitude.  A group's sum takes two terms a column,
+    each adding at most a whole step (twice U32) of the sum of their magnitudes; its scaling, the groups' sum and the
+    parts of a split row round a few times more.  Below the normal range every term and sum rounds to 2^-149."""
+    codes, s, z = m
+    w = R.dense(codes, s, z)[0]
+    group, groups = w.shape[-1] // s.shape[-1], s.shape[-1]
+    x = x.cpu().to(torch.float64)
+    most = x.abs().view(len(x), groups, group).amax(dim=2).repeat_interleave(group, dim=1)
+    held = torch.maximum(2.0 ** -24 * x.abs(), 2.0 ** -39 * most)
+    size = x.abs() @ w.abs().t()
+    step = 2.0 ** -149 * (groups + 20 + 2 * group * s.cpu().to(torch.float64).abs().sum(-1))
+    return x @ w.t(), held @ w.abs().t() + (4 * group + groups + 24) * R.U32 * size + step
+
+
+F32_FORMS = [(1, 512, 2048, 128), (1, 4100, 256, 32), (3, 64, 640, 64), (16, 100, 1024, 32), (20, 96, 2080, 32),
+             (40, 2048, 512, 128), (70, 65, 1920, 64), (300, 1500, 384, 32)]
+
+
+@pytest.mark.parametrize("scale", [1e-40, 1e-37, 1.0, 1e34])
+@pytest.mark.parametrize("n,rows,cols,group", F32_FORMS)
+def test_f32_magnitudes(n, rows, cols, group, scale):
+    from hoard_amd.ops import q4_matmul
+    print("q4 f32 magnitudes", n, rows, cols, group, scale, flush=True)
+    w = weights(61, 0, rows, cols, group, F32, True)
+    x = (torch.randn((n, cols), generator=torch.Generator().manual_seed(62), dtype=torch.float64) * scale).to(F32)
+    x[0, :group] = 0.0  # a group of nothing
+    R.close(q4_matmul(x.cuda(), op(w)), *near_fp32(x, w), "y")
+
+
+@pytest.mark.parametrize("n,rows,cols,group", F32_FORMS)
+def test_f32_small_beside_large(n, rows, cols, group):
+    """Values 2^-25 of the group's largest, which itself meets a weight of zero, keep their digits."""
+    from hoard_amd.ops import q4_matmul
+    print("q4 f32 small beside large", n, rows, cols, group, flush=True)
+    codes, s, z = weights(63, 0, rows, cols, group, F32, False)
+    codes = codes.clone()
+    codes[:, ::group // 2] = codes[:, ::group // 2] & 0xF0 | 8  # a group's first code: the zero point
+    x = torch.randn((n, cols), generator=torch.Generator().manual_seed(64)) * 2.0 ** -25
+    x[:, ::group] = 1.9
+    w = (codes, s, z)
+    R.close(q4_matmul(x.cuda(), op(w)), *near_fp32(x, w), "y")
+
+
 def test_graphs():
     """Three forms captured and replayed with eager work between, each replay the eager result."""
     from hoard_amd.ops import q4_matmul
