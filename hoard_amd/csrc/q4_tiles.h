@@ -663,24 +663,34 @@ hipError_t launch_flow_of(const Q4Args &a, hipStream_t s) {
 // fewer workgroups than the 256 CUs hold, smaller tiles and columns split over more
 // waves are faster; above that, larger tiles read x and unpack the codes less often.
 // Measured on bf16 (us):
-//   4096 x 4096, rows of x   16    20    32    64   128   256   512
-//     tiles 16, columns / 8  7.8
-//     tiles 32, columns / 8        9.4  11.9  26.6  50.9
-//     flow 16, columns / 4  13.8  14.1  14.0  14.9  15.8  28.8  59.6
-//     flow 32, columns / 4  14.7  17.7  18.0  18.4  18.8  20.1  37.6
-//     flow 64, columns / 2              20.5  28.6  29.0  29.7  31.6
-//     flow 64               22.0  27.0  27.2  42.0  42.3  42.4  43.8 (8192 rows of W:
+//   4096 x 4096, rows of x          16    20    32    64   128   256   512
+//     tiles 16, columns / 8        7.8
+//     tiles 16, columns / 8, two wide     9.8  10.0  12.8  22.7
+//     flow 16, columns / 4        13.8  14.1  14.0  14.9  15.8  28.8  59.6
+//     flow 32, columns / 4        14.7  17.7  18.0  18.4  18.8  20.1  37.6
+//     flow 64, columns / 2                    20.5  28.6  29.0  29.7  31.6
+//     flow 64                     22.0  27.0  27.2  42.0  42.3  42.4  43.8 (8192 rows of W:
 //                                               59.5 at 512, where flow 64 / 2 takes 60.8)
+//   8192 x 4096, 20 / 64 rows: 12.8 / 25.4 by tiles 16 / 8 two wide, 17.2 / 17.7 by flow 16 / 4.
 //   16384 x 8192, 16 rows: 24.5 by tiles 16 / 4 two wide, 34.3 by tiles 16 / 8.
 //   Sorted, 10 of 512 experts of 512 x 2048 twice, tokens   1     4    16    64   384
 //     tiles 16, columns / 4, two wide                     10.9  18.0  47.7   119   219
 //     flow 16, columns / 2                                14.4  17.0  36.1  79.5   156
 //     flow 32                                             20.0  21.5  32.3  61.5   118
 //   8 of 128 experts of 768 x 2048 twice, 512 tokens: 79 by flow 64, 92 by flow 32.
-// fp32 (us): 4096 x 4096, 64 rows 27 by tiles 32 / 4 two wide, 56 by tiles 32 four wide;
-// 8 of 128 experts, 128 tokens: 65 by tiles 16 four wide, 76 by tiles 32, 139 by tiles
-// 16 / 4; 4 tokens: 19 by tiles 16 / 2 two wide, 25 by tiles 16 four wide; 1 token 10.1
-// by tiles 16 / 4, 12.9 by tiles 16 / 2 two wide.
+// On fp32, tiles two streams deep (rows of x x rows of W / columns):
+//   4096 x 4096, rows of x           20    64   128   256   512   (8192 x 4096)  20    64   128   512
+//     16 x 32 / 8                  14.4  26.1  48.6  93.7   190                23.8  52.6   100   394
+//     16 x 64 / 4                  18.9  19.7  36.4  68.2   137                20.2  29.3  53.4   202
+//     32 x 64 / 4                  25.1  29.9  30.8  58.4   114                26.5  31.1  57.6   215
+//     32 x 128 / 2                 38.5  39.7  40.1  41.9  78.9                40.2  41.5  43.5   157
+//     32 x 128                     50.1  50.5  51.2  52.6  68.1                53.4  54.4  56.0   122
+//     64 x 128                     50.6  82.7  83.6  84.4  86.2                55.0  92.9  93.3   125
+//   Sorted, 4 of 32 experts of 2048 x 2048, tokens   1     4    16    64   512
+//     16 x 32 / 4                                  9.1  12.0  22.0  39.2   176
+//     16 x 64 / 2                                 10.9  14.4  19.0  33.9   124
+//     16 x 128                                    17.2  19.9  24.3  29.5  86.9
+//     32 x 128                                    17.5  20.0  24.6  34.0  80.6
 constexpr int64_t kCUs = 256;
 
 template <typename T, int G, bool UP>
@@ -693,15 +703,14 @@ hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
     constexpr int TN = UP ? 64 : 128;  // rows of W of a workgroup four wide
     if constexpr (sizeof(T) == 4) {
         if (sorted) {
-            if (groups(16, TN) <= kCUs / 2) return launch_tiles_of<T, G, UP, 2, 1, 1, 4, 2>(a, s);
-            if (groups(16, TN) <= 2 * kCUs) return launch_tiles_of<T, G, UP, 2, 1, 2, 2, 2>(a, s);
+            if (groups(16, TN) <= 5 * kCUs / 4) return launch_tiles_of<T, G, UP, 2, 1, 1, 4, 2>(a, s);
+            if (groups(16, TN) <= 5 * kCUs / 2) return launch_tiles_of<T, G, UP, 2, 1, 2, 2, 2>(a, s);
             if (per <= 16) return launch_tiles_of<T, G, UP, 2, 1, 4, 1, 2>(a, s);
             return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 2>(a, s);
         }
-        if (per <= 16)
-            return groups(16, 16) <= 3 * kCUs ? launch_tiles_of<T, G, UP, 2, 1, 1, 8, 2>(a, s)
-                                              : launch_tiles_of<T, G, UP, 2, 1, 1, 4, 2>(a, s);
-        if (groups(32, 32) <= kCUs) return launch_tiles_of<T, G, UP, P, 2, 2, 4, 2>(a, s);
+        if (groups(16, TN / 4) <= kCUs) return launch_tiles_of<T, G, UP, 2, 1, 1, 8, 2>(a, s);
+        if (groups(16, TN / 2) <= kCUs) return launch_tiles_of<T, G, UP, 2, 1, 2, 4, 2>(a, s);
+        if (groups(32, TN / 2) <= kCUs) return launch_tiles_of<T, G, UP, 2, 2, 2, 4, 2>(a, s);
         if (groups(32, TN) <= kCUs) return launch_tiles_of<T, G, UP, 2, 2, 4, 2, 2>(a, s);
         return launch_tiles_of<T, G, UP, 2, 2, 4, 1, 2>(a, s);
     } else {
@@ -713,7 +722,7 @@ hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
         if (per <= 16)
             return groups(16, 16) <= 3 * kCUs ? launch_tiles_of<T, G, UP, P, 1, 1, 8, 2>(a, s)
                                               : launch_tiles_of<T, G, UP, P, 1, 2, 4, 2>(a, s);
-        if (groups(32, 16) <= kCUs) return launch_tiles_of<T, G, UP, P, 2, 1, 8, 2>(a, s);
+        if (groups(16, TN / 4) <= 2 * kCUs) return launch_tiles_of<T, G, UP, 2, 1, 1, 8, 2>(a, s);
         if (groups(16, TN) <= kCUs) return launch_flow_of<T, G, UP, 1, 4, 4, 4>(a, s);
         if (groups(32, TN) <= kCUs) return launch_flow_of<T, G, UP, 2, 4, 4, 4>(a, s);
         if (groups(64, TN) <= kCUs) return launch_flow_of<T, G, UP, 4, 4, 2, 2>(a, s);
