@@ -263,6 +263,21 @@ def test_f32_small_beside_large(n, rows, cols, group):
     R.close(q4_matmul(x.cuda(), op(w)), *near_fp32(x, w), "y")
 
 
+@pytest.mark.parametrize("up", [False, True])
+@pytest.mark.parametrize("n,rows,cols,group,dtype", [
+    (20, 700, 1184, 32, F32), (70, 2500, 672, 32, F32), (70, 1200, 1088, 64, F32), (130, 2500, 320, 64, F32),
+    (400, 1500, 416, 32, F32), (700, 1800, 288, 32, F32), (33, 4100, 640, 128, F32), (100, 2000, 1312, 32, BF16),
+    (50, 1300, 640, 128, F16), (17, 8200, 1216, 64, BF16)])
+def test_dense_splits(n, rows, cols, group, dtype, up):
+    """Sizes on both sides of where a dense call's columns are split over fewer waves, none a multiple of a step."""
+    from hoard_amd.ops import q4_matmul
+    print("q4 splits", n, rows, cols, group, dtype, up, flush=True)
+    w = weights(97, 0, rows, cols, group, BF16, True)
+    u = weights(98, 0, rows, cols, group, F32) if up else None
+    x = rows_of(99, n, cols, dtype)
+    R.close(q4_matmul(x, op(w), op(u) if up else None), *expect(x, w, u), "y")
+
+
 def test_graphs():
     """Three forms captured and replayed with eager work between, each replay the eager result."""
     from hoard_amd.ops import q4_matmul
