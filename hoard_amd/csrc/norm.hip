@@ -173,13 +173,26 @@ struct GradIn {
 // rows stay in registers and go to its rows of the workspace, one per wanted
 // parameter ([parameter][group][n]).  Where the registers hold them (AHEAD) the next
 // row's inputs are fetched before this row's sums, whose two barriers would leave the
-// memory idle, and the weights stay.
+// memory idle, and the weights stay.  Rows longer than 8192 (WIDE) would need 250
+// registers of the 128 that 1024 threads leave: two of the three sums lie in LDS, each
+// column in its thread's own words, and inputs are read again where they are used
+// (512 x 16384 in bf16: 48 us, 116 with the registers spilled; 1 row 12.3, 41.7).
 template <typename T, typename R, int BS, int NV, bool NT>
 __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_norm_grads g, float *work) {
     constexpr bool AHEAD = BS <= 512 && NV * (2 * sizeof(R) + 2 * sizeof(T)) <= 16;
+    constexpr bool WIDE = NV * BS * 8 > 8192;
     __shared__ float part[2][3][BS / 64];
+    __shared__ float lds[WIDE ? 2 : 1][WIDE ? NV * 8 : 1][WIDE ? BS : 1];
     const float inv_n = 1.0f / (float)a.n;
     float s_pre[NV][8] = {}, s_post[NV][8] = {}, s_gate[NV][8] = {};
+    auto add_to = [&](int which, float (&s)[NV][8], int k, int i, float x, float y) {
+        if constexpr (WIDE) lds[which][k * 8 + i][threadIdx.x] = fmaf(x, y, lds[which][k * 8 + i][threadIdx.x]);
+        else s[k][i] = fmaf(x, y, s[k][i]);
+    };
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < NV * 8; i++) lds[0][i][threadIdx.x] = lds[1][i][threadIdx.x] = 0.0f;
+    }
     Cols c[NV];
     Raw<float> wp[NV], wq[NV];
     auto fetch_weights = [&]() {
@@ -196,6 +209,7 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
         const size_t base = row * a.n;
         in.rho_b = a.stats[2 * row];
         in.rho_v = a.stats[2 * row + 1];
+        if constexpr (WIDE) return;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             if (g.dh) {
@@ -212,11 +226,26 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
     int turn = 0;
     auto one = [&](GradIn<T, R, NV> &in, size_t row) {
         const size_t base = row * a.n;
+        auto v_of = [&](int k) {
+            if constexpr (WIDE) return fetch(static_cast<const R *>(a.r_out) + base, c[k], a.n);
+            else return in.v[k];
+        };
+        auto dh_of = [&](int k) {
+            if constexpr (WIDE) return fetch(static_cast<const T *>(g.dh) + base, c[k], a.n);
+            else return in.dh[k];
+        };
+        auto b_of = [&](int k) {
+            if constexpr (WIDE) return fetch(static_cast<const T *>(a.b) + base, c[k], a.n);
+            else return in.b[k];
+        };
+        auto in_turn = [] {  // one k after another, for their registers
+            if constexpr (WIDE) asm volatile("" ::: "memory");
+        };
         float dv[NV][8];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             if (g.dr_out) {
-                widen(in.dr[k], dv[k]);
+                widen(WIDE ? fetch(static_cast<const R *>(g.dr_out) + base, c[k], a.n) : in.dr[k], dv[k]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) dv[k][i] = 0.0f;
@@ -227,13 +256,14 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 float w[8], v[8], u[8];
-                widen(in.v[k], v);
-                widen(in.dh[k], u);
+                in_turn();
+                widen(v_of(k), v);
+                widen(dh_of(k), u);
                 widen(AHEAD ? wq[k] : fetch(a.w_pre, c[k], a.n), w);
                 mask_cols(c[k], u);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    s_pre[k][i] = fmaf(u[i], v[i] * in.rho_v, s_pre[k][i]);
+                    add_to(0, s_pre, k, i, u[i], v[i] * in.rho_v);
                     s = fmaf(u[i] * (a.w_offset + w[i]), v[i], s);
                 }
             }
@@ -241,10 +271,13 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 float w[8], v[8], u[8];
-                keep(in.v[k]);
-                keep(in.dh[k]);
-                widen(in.v[k], v);
-                widen(in.dh[k], u);
+                in_turn();
+                if constexpr (!WIDE) {
+                    keep(in.v[k]);
+                    keep(in.dh[k]);
+                }
+                widen(v_of(k), v);
+                widen(dh_of(k), u);
                 widen(AHEAD ? wq[k] : fetch(a.w_pre, c[k], a.n), w);
 #pragma unroll
                 for (int i = 0; i < 8; i++)
@@ -261,7 +294,8 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             float q[8], w[8], dg[8], b[8];
-            widen(in.b[k], b);
+            in_turn();
+            widen(b_of(k), b);
             mask_cols(c[k], dv[k]);
             if (a.gate) gate_of<T>(a, AHEAD ? in.gate[k] : fetch_gate<T>(a, row, c[k]), q);
             if (a.w_post) widen(AHEAD ? wp[k] : fetch(a.w_post, c[k], a.n), w);
@@ -275,7 +309,7 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
                 dg[i] = d * nb * wo * slope;
                 s_gate[k][i] += dg[i];
                 s_g += dg[i];
-                s_post[k][i] = fmaf(d * t, nb, s_post[k][i]);
+                add_to(1, s_post, k, i, d * t, nb);
                 dv[k][i] = d * t * wo;  // u2 from here on
                 s_b = fmaf(dv[k][i], b[i], s_b);
             }
@@ -292,8 +326,8 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 float b[8];
-                keep(in.b[k]);
-                widen(in.b[k], b);
+                if constexpr (!WIDE) keep(in.b[k]);
+                widen(b_of(k), b);
 #pragma unroll
                 for (int i = 0; i < 8; i++) dv[k][i] = in.rho_b * (dv[k][i] - b[i] * s_b);
             }
@@ -328,6 +362,13 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         float *p = work + mine;
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                s_pre[k][i] = lds[0][k * 8 + i][threadIdx.x];
+                s_post[k][i] = lds[1][k * 8 + i][threadIdx.x];
+            }
+        }
         if (c[k].lo == 8) continue;
         if (g.dw_pre) {
             put(alone ? g.dw_pre : p, c[k], a.n, s_pre[k]);

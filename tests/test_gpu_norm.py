@@ -209,6 +209,15 @@ def test_backward(kw, given):
             R.close(t, out[name], bounds[name], name)
 
 
+@pytest.mark.parametrize("given", ["both", "dr_out", "dh"])
+@pytest.mark.parametrize("kw", [dict(m=600, n=8200, dtype=BF16, res=F32, gate="channel", sigmoid=True),
+                                dict(m=520, n=9003, dtype=F32, res=F32, gate="channel"),
+                                dict(m=300, n=16384, dtype=F16, res=F16, gate="token", offset=1.0)], ids=str)
+def test_backward_long_rows(kw, given):
+    """The longest rows, several of them a group."""
+    test_backward(kw, given)
+
+
 @pytest.mark.parametrize("kw", [c for c in CASES if c["dtype"] == F32], ids=[i for i, c in zip(IDS, CASES) if c["dtype"] == F32])
 def test_backward_against_differences(kw):
     """Along a random direction: the gradients' inner product against a central difference of the 64-bit forward."""
