@@ -44,7 +44,7 @@ def product(x, m, e):
     """(value, bound before storing) of x [r, cols] times matrix e of m = (codes, scales, zeros).
 
     The kernels may form a group's sum of (B + q) x less (B + z) times the sum of x, B up to 16 for fp32 activations
-    (split into three parts, so three terms a column) and f16, 128 for bf16: both sums, of magnitudes up to
+    (split into at most three parts, so three terms a column) and f16, 128 for bf16: both sums, of magnitudes up to
     (B + q) |x| and (B + z) |x|, round once a term and a few times more, their difference is scaled, and the groups'
     sums, now of magnitudes |q - z| |s| |x|, are added."""
     if m[0].dim() == 3:
