@@ -46,20 +46,34 @@ __device__ __forceinline__ v4u biased(uint32_t codes) {
     return o;
 }
 
-// Codes in their own order, words {0, 1}, {2, 3}, {4, 5}, {6, 7}, for x that is not
-// rearranged: the code in the lowest fraction bits of kInOrderBias, so that a byte
-// permute and a masked or make a word.
+// Codes plus kInOrderBias in their own order, words {0, 1}, {2, 3}, {4, 5}, {6, 7}, for x
+// that is not rearranged.  f16: the code in the lowest fraction bits of 1024, so that a
+// byte permute and a masked or make a word; the sum is taken off exactly (less).  bf16:
+// half a byte is the 8-bit float (4 exponent bits, the lowest of which the code's fourth
+// bit is) of code * 2^-9, which one conversion to bf16 takes two at a time: no offset,
+// whose sums 32 bits would round at 128 + code for what a code of some 8 less its zero
+// point is worth (0.36 % of a prompt's results then fell to the other side of their
+// bf16 rounding).
 template <typename T>
-constexpr float kInOrderBias = __is_same(T, bf16) ? 128.0f : 1024.0f;
+constexpr float kInOrderBias = __is_same(T, bf16) ? 0.0f : 1024.0f;
 template <typename T>
 __device__ __forceinline__ v4u in_order(uint32_t codes) {
-    uint32_t base = __is_same(T, bf16) ? 0x43004300u : 0x64006400u;
-    asm("" : "+v"(base));
     const uint32_t high = codes >> 4;
     v4u o;
+    if constexpr (__is_same(T, bf16)) {
+        const uint32_t front = __builtin_amdgcn_perm(high, codes, 0x05010400u) & 0x0f0f0f0fu;
+        const uint32_t back = __builtin_amdgcn_perm(high, codes, 0x07030602u) & 0x0f0f0f0fu;
+        o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(front, 512.0f, false));
+        o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(front, 512.0f, true));
+        o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(back, 512.0f, false));
+        o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(back, 512.0f, true));
+    } else {
+        uint32_t base = 0x64006400u;
+        asm("" : "+v"(base));
 #pragma unroll
-    for (int j = 0; j < 4; j++)  // byte j of both into the two halves; the upper nibbles are masked off
-        o[j] = (__builtin_amdgcn_perm(high, codes, 0x0c040c00u + 0x00010001u * j) & 0x000f000fu) | base;
+        for (int j = 0; j < 4; j++)  // byte j of both into the two halves; the upper nibbles are masked off
+            o[j] = (__builtin_amdgcn_perm(high, codes, 0x0c040c00u + 0x00010001u * j) & 0x000f000fu) | base;
+    }
     return o;
 }
 

@@ -446,8 +446,8 @@ __global__ __launch_bounds__(64 * NW * KS, MW) void q4_tiles_kernel(Q4Args a) {
 
 // The same product for 16-bit activations and many rows of x: x goes straight from
 // memory to LDS in its own order, the codes take that order (in_order), and in bf16 the
-// sums of x come from a third product with a matrix of ones, whose accumulator holds
-// them where the scaled sums need them.  A step is 128 columns; x lies in two buffers, so
+// sums of x, which the zero points multiply, come from a third product with a matrix of
+// ones, whose accumulator holds them where the scaled sums need them.  A step is 128 columns; x lies in two buffers, so
 // one barrier a step hands over what arrived and frees what was read.
 //
 // A row of x is 256 bytes of a buffer, its 16-byte pieces exchanged by the row's

@@ -59,8 +59,8 @@ typedef struct hoard_q4_matrix {
    scale type may differ) y[r] = silu(W x[r]) * (W_up x[r]).  W has n_mat 1.  The
    products are formed with the activations as given (fp32: to 2^-24 of a value, or to
    2^-39 of its group's largest), not quantised.  A group's sum is formed before its
-   scale, for bf16 of codes plus an offset of up to 128 that is then corrected, so it
-   overflows where the sum of |x| over the group reaches 2^120.  A row of x that holds an infinity or a NaN
+   scale, in 16 bits also of codes with an offset of up to 16 that is then corrected, so
+   it overflows where the sum of |x| over the group reaches 2^119.  A row of x that holds an infinity or a NaN
    gives a row of y without a defined value (infinities and NaN); other rows are not
    touched by it. */
 int hoard_q4_matmul(const hoard_q4_matrix *w, const hoard_q4_matrix *up, int type, int n_rows, const void *x,

@@ -1,0 +1,53 @@
+"""How often a 16-bit result of a 4-bit product is not the rounded 64-bit one."""
+import pytest
+
+import opsbounds as B
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def matrix(seed, lead, rows, cols, group):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 256, (*lead, rows, cols // 2), generator=g, dtype=torch.uint8)
+    return codes.cuda(), (torch.rand((*lead, rows, cols // group), generator=g) * 0.01).to(BF16).cuda(), None
+
+
+# prompts: the sizes of each form that takes x in its own order, by rows of x and of W
+PROMPTS = [(128, 4096, 128), (130, 4096, 32), (256, 4096, 64), (512, 4096, 128), (700, 4096, 128), (700, 2080, 32)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n,rows,group", PROMPTS)
+def test_prompt(n, rows, group, dtype):
+    from hoard_amd.ops import Q4Weight, q4_matmul
+    print("q4 rounding", n, rows, group, dtype, flush=True)
+    m = matrix(1, (), rows, 2048, group)
+    x = torch.randn((n, 2048), generator=torch.Generator().manual_seed(2)).to(dtype)
+    value, expected = B.expected_over_border(x, m, dtype)
+    over = B.over_border(q4_matmul(x.cuda(), Q4Weight(*m)), value)
+    print("over a border", over, "expected", expected, "of", value.numel(), flush=True)
+    assert over <= B.allowed(expected)
+
+
+@pytest.mark.parametrize("tokens,k,experts,rows,group", [(16, 8, 64, 512, 128), (120, 4, 20, 768, 64), (512, 4, 20, 768, 128)])
+def test_sorted(tokens, k, experts, rows, group):
+    from hoard_amd.ops import Q4Weight, q4_matmul, sort_pairs
+    g = torch.Generator().manual_seed(3)
+    ids = torch.stack([torch.randperm(experts, generator=g)[:k] for _ in range(tokens)]).to(torch.int32).cuda()
+    s = sort_pairs(ids, experts)
+    m = matrix(4, (experts,), rows, 2048, group)
+    x = torch.randn((tokens * k, 2048), generator=g).to(BF16)
+    y = q4_matmul(x.cuda(), Q4Weight(*m), offsets=s.offsets)
+    off, over, expected = s.offsets.tolist(), 0, 0.0
+    for e in range(experts):
+        a, b = off[e], off[e + 1]
+        if b > a:
+            value, more = B.expected_over_border(x[a:b], (m[0][e], m[1][e], None), BF16)
+            over += B.over_border(y[a:b], value)
+            expected += more
+    print("over a border", over, "expected", expected, "of", y.numel(), flush=True)
+    assert over <= B.allowed(expected)

@@ -1,0 +1,38 @@
+"""The bounds of the 4-bit products' tests refuse what they are there to refuse: mistakes planted in a model, on the CPU."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import opsbounds as B  # noqa: E402
+
+
+def model(x, m, bias):
+    """A product as the matrix tiles form it, codes plus `bias`: 32 columns an instruction, each result rounded to 32 bits."""
+    codes, scales, _ = m
+    q = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2).to(torch.float64) + bias
+    groups = scales.shape[-1]
+    group = q.shape[-1] // groups
+    x, s = x.to(torch.float64), scales.to(torch.float64)
+    f32 = lambda t: t.to(torch.float32).to(torch.float64)  # noqa: E731
+    acc = torch.zeros((x.shape[0], q.shape[0]), dtype=torch.float64)
+    for g in range(groups):
+        d, sums = torch.zeros_like(acc), torch.zeros((x.shape[0], 1), dtype=torch.float64)
+        for c in range(g * group, (g + 1) * group, 32):
+            d = f32(d + x[:, c:c + 32] @ q[:, c:c + 32].t())
+            sums = f32(sums + x[:, c:c + 32].sum(1, keepdim=True))
+        acc = f32(acc + s[:, g] * f32(d - (8 + bias) * sums))
+    return acc
+
+
+def matrix(seed, rows, cols, group):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 256, (rows, cols // 2), generator=g, dtype=torch.uint8)
+    return codes, (torch.rand((rows, cols // group), generator=g) * 0.01).to(torch.bfloat16), None
+
+
+def test_offset_of_128_is_refused():
+    m = matrix(1, 512, 2048, 128)
+    x = torch.randn((128, 2048), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    value, expected = B.expected_over_border(x, m, torch.bfloat16)
+    over = {bias: B.over_border(model(x, m, bias).to(torch.bfloat16), value) for bias in (0, 128)}
+    assert over[0] <= B.allowed(expected) < over[128], (over, expected)
