@@ -16,8 +16,9 @@
 //
 // fp32 activations are two f16 planes: a group of a row is multiplied by the power of
 // two that brings its largest value to 2^14, rounded, and what that leaves is rounded
-// again.  Their sum is x to 2^-24 of it, as one rounding to fp32, or to 2^-39 of the
-// group's largest value, whichever is more.  With f16's exact codes (below) the sums are
+// again.  Their sum is x to 2^-23 of it (the first leaves up to 2^12 steps of x's last
+// place, of which the second's 11 bits hold no odd number above 2^11), or to 2^-39 of
+// the group's largest value, whichever is more.  With f16's exact codes (below) the sums are
 // of the terms themselves; three bf16 planes, exactly x, had to correct sums of 16 + code
 // whose terms are five times the plain ones', and were four times further off.
 #pragma once

@@ -57,12 +57,13 @@ typedef struct hoard_q4_matrix {
 /* y[r] = W x[r] for n_rows rows: x [n_rows][cols] and y [n_rows][rows] of `type`,
    x 16-byte aligned.  With `up` (same rows, cols, group and n_mat; its zeros and
    scale type may differ) y[r] = silu(W x[r]) * (W_up x[r]).  W has n_mat 1.  The
-   products are formed with the activations as given (fp32: to 2^-24 of a value, or to
-   2^-39 of its group's largest), not quantised.  A group's sum is formed before its
-   scale, in 16 bits also of codes with an offset of up to 16 that is then corrected, so
-   it overflows where the sum of |x| over the group reaches 2^119.  A row of x that holds an infinity or a NaN
-   gives a row of y without a defined value (infinities and NaN); other rows are not
-   touched by it. */
+   products are formed with the activations as given, not quantised; fp32 ones are
+   held, for more than one row and by offsets, to 2^-23 of a value or to 2^-39 of its
+   group's largest.  A group's sum is formed before its scale, in 16 bits also of codes
+   with an offset of up to 16 that is then corrected, so it overflows where the sum of
+   |x| over the group reaches 2^119.  A row of x that holds an infinity or a NaN gives a
+   row of y without a defined value (infinities and NaN); other rows are not touched by
+   it. */
 int hoard_q4_matmul(const hoard_q4_matrix *w, const hoard_q4_matrix *up, int type, int n_rows, const void *x,
                     void *y, void *stream);
 

@@ -36,3 +36,20 @@ def test_offset_of_128_is_refused():
     value, expected = B.expected_over_border(x, m, torch.bfloat16)
     over = {bias: B.over_border(model(x, m, bias).to(torch.bfloat16), value) for bias in (0, 128)}
     assert over[0] <= B.allowed(expected) < over[128], (over, expected)
+
+
+def planes(x, group, low=True):
+    """fp32 x as the matrix tiles hold it: two f16 planes of x times a power of two a group."""
+    most = x.abs().view(len(x), -1, group).amax(dim=2, keepdim=True)
+    power = torch.exp2(14 - torch.floor(torch.log2(most.to(torch.float64))))
+    v = x.to(torch.float64).view(len(x), -1, group) * power
+    high = v.to(torch.float16).to(torch.float64)
+    held = high + (v - high).to(torch.float16).to(torch.float64) if low else high
+    return (held / power).view(x.shape)
+
+
+def test_two_planes_hold_23_bits():
+    x = torch.randn((4096, 128), generator=torch.Generator().manual_seed(3))
+    off = ((planes(x, 128) - x.to(torch.float64)).abs() / x.to(torch.float64).abs())
+    near = x.abs() >= 2.0 ** -15 * x.abs().amax(dim=1, keepdim=True)
+    assert 2.0 ** -24 < off[near].max() <= 2.0 ** -23
