@@ -33,6 +33,20 @@ def test_prompt(n, rows, group, dtype):
     assert over <= B.allowed(expected)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n,rows,group", [(1, 4096, 128), (13, 2048, 32), (20, 2048, 64), (60, 2048, 128)])
+def test_few_rows(n, rows, group, dtype):
+    """Dots and the tiles of few rows sum codes with an offset of 16 (f16 tiles none)."""
+    from hoard_amd.ops import Q4Weight, q4_matmul
+    print("q4 rounding", n, rows, group, dtype, flush=True)
+    m = matrix(5, (), rows, 2048, group)
+    x = torch.randn((n, 2048), generator=torch.Generator().manual_seed(6)).to(dtype)
+    value, expected = B.expected_over_border(x, m, dtype, 0 if dtype == F16 and n > 1 else 16)
+    over = B.over_border(q4_matmul(x.cuda(), Q4Weight(*m)), value)
+    print("over a border", over, "expected", expected, "of", value.numel(), flush=True)
+    assert over <= B.allowed(expected)
+
+
 @pytest.mark.parametrize("tokens,k,experts,rows,group", [(16, 8, 64, 512, 128), (120, 4, 20, 768, 64), (512, 4, 20, 768, 128)])
 def test_sorted(tokens, k, experts, rows, group):
     from hoard_amd.ops import Q4Weight, q4_matmul, sort_pairs

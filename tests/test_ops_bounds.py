@@ -53,3 +53,17 @@ def test_two_planes_hold_23_bits():
     off = ((planes(x, 128) - x.to(torch.float64)).abs() / x.to(torch.float64).abs())
     near = x.abs() >= 2.0 ** -15 * x.abs().amax(dim=1, keepdim=True)
     assert 2.0 ** -24 < off[near].max() <= 2.0 ** -23
+
+
+@pytest.mark.parametrize("tokens,rows,cols,group", [(8, 96, 512, 128), (33, 48, 320, 64), (4, 40, 96, 32), (64, 64, 4096, 128)])
+def test_one_plane_is_refused(tokens, rows, cols, group):
+    """fp32 products with x in f16 stay far outside what the two planes may be off, with a second matrix too."""
+    m, up = matrix(4, rows, cols, group), matrix(5, rows, cols, group)
+    x = torch.randn((tokens, cols), generator=torch.Generator().manual_seed(6))
+    (g, vg), (u, vu) = B.fp32_product(x, m), B.fp32_product(x, up)
+    both, v = B.fp32_swiglu(g, vg, u, vu)
+    for low in (True, False):
+        held = planes(x, group, low)
+        g1, u1 = B.fp32_product(held, m)[0], B.fp32_product(held, up)[0]
+        for ratio in (B.rms_ratio(g1, g, vg), B.rms_ratio(g1 / (1 + torch.exp(-g1)) * u1, both, v)):
+            assert ratio <= 1.0 if low else ratio > 10.0, (low, ratio)
