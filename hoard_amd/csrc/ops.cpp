@@ -16,6 +16,7 @@ bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) 
 
 constexpr int kMaxRows = 1 << 22;  // a launch's workgroups of 16 rows by 8 tiles of x within its 2^32 threads
 constexpr int kMaxCols = 1 << 20;  // 64 rows of x lie within the kernels' 32-bit offsets
+constexpr int kMaxN = 1 << 30;     // columns of the pairs' rows: a wave's step of 2048 past the last stays within 32 bits
 
 int launched(const char *what, hipError_t rc) {
     if (rc == hipSuccess) {
@@ -80,7 +81,7 @@ int check_sort(int n_tokens, int k, int n_expert) {
 
 int check_rows(int type, int n_tokens, int k, int n) {
     if (!activation_type(type)) return fail_fmt(HOARD_ERR_UNSUPPORTED, "activation type %d", type);
-    if (n <= 0) return fail_fmt(HOARD_ERR_INVALID, "n %d", n);
+    if (n < 1 || n > kMaxN) return fail_fmt(HOARD_ERR_INVALID, "n %d outside 1..%d", n, kMaxN);
     return check_pairs(n_tokens, k);
 }
 

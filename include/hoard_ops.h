@@ -96,7 +96,7 @@ int hoard_sort_pairs(int n_tokens, int k, int n_expert, const int32_t *ids, int3
 int hoard_sort_workspace(int n_tokens, int k, int n_expert, size_t *bytes);
 
 /* xs[place[t][j]] = w[t][j] * x[t] (w NULL: 1): the tokens' rows [n_tokens][n]
-   laid out by sorted row, xs [n_tokens*k][n].  In these calls a place outside
+   laid out by sorted row, xs [n_tokens*k][n], 1 <= n <= 2^30.  In these calls a place outside
    [0, n_tokens*k) drops its pair, and the places that are not dropped must be
    distinct; rows of xs that no pair names are left as they are. */
 int hoard_sort_gather(int type, int n_tokens, int k, int n, const void *x, const int32_t *place, const float *w,
