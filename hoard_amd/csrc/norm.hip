@@ -455,8 +455,8 @@ void grad_of(const hoard_norm_args &a, const hoard_norm_grads &g, float *work, h
 int norm_groups(int n_rows, int n) {
     const int most = n <= 1024 ? 1024 : n <= 2048 ? 768 : 256;
     if (n_rows <= most) return n_rows;
-    const int share = (n_rows + most - 1) / most;
-    return (n_rows + share - 1) / share;
+    const int64_t share = ((int64_t)n_rows + most - 1) / most;
+    return (int)((n_rows + share - 1) / share);
 }
 
 hipError_t launch_norm(const hoard_norm_args &a, hipStream_t s) {
