@@ -85,11 +85,11 @@ __global__ __launch_bounds__(256) void q4_rows_kernel(Q4Args a, int lanes_log) {
     const int64_t at = (((int64_t)blockIdx.x * 4 + wave_index()) << (6 - lanes_log)) * NR + run * NR;
     const int n0 = (int)min(at, (int64_t)a.w.rows);
     const int cols = a.w.cols, groups = cols / a.w.group, group_log = __ffs(a.w.group) - 1;
-    for (int r = blockIdx.y; r < a.n_rows; r += gridDim.y) {
-        const int e = matrix_of(a, r);
+    for (int64_t r = blockIdx.y; r < a.n_rows; r += gridDim.y) {
+        const int e = matrix_of(a, (int)r);
         float acc[P][NR] = {};
         if (e >= 0) {
-            const T *x = static_cast<const T *>(a.x) + (size_t)(r / a.x_share) * cols;
+            const T *x = static_cast<const T *>(a.x) + (size_t)((int)r / a.x_share) * cols;
             size_t row[NR];  // clamped: what lies behind the last row is not stored
 #pragma unroll
             for (int j = 0; j < NR; j++) row[j] = (size_t)e * a.w.rows + min(n0 + j, a.w.rows - 1);

@@ -698,7 +698,7 @@ template <typename T, int G, bool UP>
 hipError_t launch_tiles_sized(const Q4Args &a, hipStream_t s) {
     constexpr int P = UP ? 2 : 1;
     const bool sorted = a.mode == kQ4Sorted;
-    const int per = sorted ? (a.n_rows + a.w.n_mat - 1) / a.w.n_mat : a.n_rows;  // rows of x of a matrix
+    const int64_t per = sorted ? ((int64_t)a.n_rows + a.w.n_mat - 1) / a.w.n_mat : a.n_rows;  // rows of x of a matrix
     // workgroups with tiles of tm rows of x and tn of W
     auto groups = [&](int tm, int tn) { return (int64_t)((a.w.rows + tn - 1) / tn) * tiles_of(a, tm); };
     constexpr int TN = UP ? 64 : 128;  // rows of W of a workgroup four wide
