@@ -4,7 +4,7 @@
 // h = v rho_v (o + w_pre),  rho_x = (mean x^2 + eps)^(-1/2).
 // Backward, with u = dh (o + w_pre):
 //   dv     = dr_out + rho_v (u - v rho_v^2 mean(u v)),      dr = dv
-//   dgate  = s dv c (times g (1 - g) behind a sigmoid; summed over the rows for
+//   dgate  = s dv c (times the sigmoid's derivative behind one; summed over the rows for
 //            a channel's gate, over the columns for a row's)
 //   u2     = s g dv (o + w_post),  db = rho_b (u2 - b rho_b^2 mean(u2 b))
 //   dw_pre = sum over rows of dh v rho_v,  dw_post = sum over rows of s g dv b rho_b.
@@ -20,6 +20,13 @@ namespace hoard {
 namespace {
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+// The sigmoid and its derivative e / (1 + e)^2, e = exp(-|x|): as s (1 - s) it would keep
+// none of its digits where s is close to 1.
+__device__ __forceinline__ float sigmoid_slope(float x, float &slope) {
+    const float e = expf(-fabsf(x)), r = 1.0f / (1.0f + e);
+    slope = e * r * r;
+    return x < 0.0f ? e * r : r;
+}
 
 // The gate of eight columns as it is stored: 32-bit values of a channel gate, those of
 // a full one, or the row's in the first word.
@@ -301,8 +308,8 @@ __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_
             if (a.w_post) widen(AHEAD ? wp[k] : fetch(a.w_post, c[k], a.n), w);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float t = !a.gate ? 1.0f : a.gate_sigmoid ? sigmoid(q[i]) : q[i];
-                const float slope = a.gate_sigmoid ? t * (1.0f - t) : 1.0f;
+                float slope = 1.0f;
+                const float t = !a.gate ? 1.0f : a.gate_sigmoid ? sigmoid_slope(q[i], slope) : q[i];
                 const float wo = a.w_post ? a.w_offset + w[i] : 1.0f;
                 const float d = a.scale * dv[k][i];   // of g c
                 const float nb = b[i] * in.rho_b;  // rho_b is 1 without a norm
