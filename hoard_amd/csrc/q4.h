@@ -118,10 +118,15 @@ __device__ __forceinline__ int matrix_of(const Q4Args &a, int r) {
 
 // g / (1 + e^-g) * u.  Where the result is rounded to 16 bits, with the exponential of
 // 2 and the reciprocal of one instruction each (1 step of 32 bits; the product with
-// log2 e adds at most 2^-24 |g| of it, g being at most some 100 where e^-g counts).
+// log2 e adds at most 2^-24 |g| of it, g being at most some 100 where e^-g counts).  The
+// reciprocal has no subnormal results, and 1 + e^-g goes up to 2^128: it is taken of a
+// sixteenth.
 template <typename T>
 __device__ __forceinline__ float silu_mul(float g, float u) {
-    if constexpr (sizeof(T) == 2) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
+    if constexpr (sizeof(T) == 2) {
+        const float e = __builtin_amdgcn_exp2f(g * -1.44269504f);
+        return g * (__builtin_amdgcn_rcpf((1.0f + e) * 0.0625f) * 0.0625f) * u;
+    }
     return g / (1.0f + expf(-g)) * u;
 }
 

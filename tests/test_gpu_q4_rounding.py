@@ -1,4 +1,4 @@
-"""How often a 16-bit result of a 4-bit product is not the rounded 64-bit one."""
+"""How often a 16-bit result of a 4-bit product is not the rounded 64-bit one, and silu far below zero."""
 import pytest
 
 import opsbounds as B
@@ -65,3 +65,23 @@ def test_sorted(tokens, k, experts, rows, group):
             expected += more
     print("over a border", over, "expected", expected, "of", y.numel(), flush=True)
     assert over <= B.allowed(expected)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("n", [1, 20, 400])
+def test_silu_of_far_negatives(n, dtype):
+    """silu(g) down to g = -88, where 1 / (1 + e^-g) is below the normal range, times an u that brings it back."""
+    from hoard_amd.ops import Q4Weight, q4_matmul
+    rows = 4096
+    ones = torch.full((rows, 16), 0x99, dtype=torch.uint8, device="cuda")  # codes of 9: weights of one scale
+    scale = torch.linspace(0.25, 1.0, rows).to(BF16).to(torch.float32).view(rows, 1)
+    w, u = Q4Weight(ones, scale.cuda()), Q4Weight(ones, torch.full((rows, 1), 1e34, device="cuda"))
+    x = torch.full((n, 32), -2.75, dtype=dtype, device="cuda")
+    y = q4_matmul(x, w, u)
+    g = -88.0 * scale.double().view(1, rows)
+    want = (g / (1 + torch.exp(-g)) * (-88.0 * float(torch.tensor(1e34)))).expand(n, rows)
+    # g rounds once as a product of its scale, u once; e^-g is off by that of g and 2^-24 |g| of its exponent's product;
+    # the exponential, the sum, the reciprocal and the products 8 more; half a step of the type
+    bound = want.abs() * (2.0 ** -24 * (3 * g.abs() + 16) + torch.finfo(dtype).eps / 2)
+    off = (y.cpu().double() - want).abs()
+    assert (off <= bound).all(), float((off / bound).max())
