@@ -18,7 +18,9 @@ A layer whose experts are 4-bit codes, M tokens, k of E experts each:
 
 Gradients: sort_combine(dxs, place) is sort_gather's, sort_combine_grad and
 norm_backward are those of sort_combine and norm_forward.  The 4-bit products
-have none (their weights are constants, and they serve inference).
+have none (their weights are constants, and they serve inference).  No call records
+itself for autograd: where gradients are recorded, a tensor that wants one is refused
+(detach it, or call under torch.no_grad(), and run the backward calls yourself).
 """
 from __future__ import annotations
 
@@ -40,6 +42,7 @@ def _need(ok: bool, what: str) -> None:
 
 def _tensor(name: str, t, shape=None, dtype=None, device=None) -> None:
     _need(isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous(), f"{name}: not a dense device tensor")
+    _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name}: wants a gradient, which this call does not record")
     _need(shape is None or tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, wanted {shape}")
     _need(dtype is None or t.dtype == dtype, f"{name}: {t.dtype}, wanted {dtype}")
     _need(device is None or t.device == device, f"{name}: on {t.device}, wanted {device}")
