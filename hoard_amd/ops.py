@@ -48,6 +48,13 @@ def _tensor(name: str, t, shape=None, dtype=None, device=None) -> None:
     _need(device is None or t.device == device, f"{name}: on {t.device}, wanted {device}")
 
 
+def _given(name: str, t, shape, dtype, device) -> None:
+    """Checks of a tensor to write to, whose version then counts the write: autograd refuses a gradient that needs what
+    it held."""
+    _tensor(name, t, shape, dtype, device)
+    torch.autograd.graph.increment_version(t)
+
+
 def _type(name: str, t) -> int:
     _need(t.dtype in _TYPES, f"{name}: {t.dtype} is no activation type")
     return _TYPES[t.dtype]
@@ -117,7 +124,7 @@ def q4_matmul(x, w: Q4Weight, up: Q4Weight | None = None, *, ids=None, offsets=N
     if out is None:
         out = torch.empty((n_rows, w.rows), dtype=x.dtype, device=x.device)
     else:
-        _tensor("out", out, (n_rows, w.rows), x.dtype, x.device)
+        _given("out", out, (n_rows, w.rows), x.dtype, x.device)
     lib, a, b = load_library(), ctypes.byref(w.desc), ctypes.byref(up.desc) if up is not None else None
     with _On(x.device) as stream:
         if ids is not None:
@@ -173,7 +180,7 @@ def sort_gather(x, place, w=None, *, out=None):
     if out is None:
         out = torch.empty((m * k, n), dtype=x.dtype, device=x.device)
     else:
-        _tensor("out", out, (m * k, n), x.dtype, x.device)
+        _given("out", out, (m * k, n), x.dtype, x.device)
     with _On(x.device) as stream:
         check(load_library().hoard_sort_gather(dt, m, k, n, _p(x), _p(place), _p(w), _p(out), stream))
     return out
@@ -187,7 +194,7 @@ def sort_combine(y, place, w=None, res=None, *, out=None):
     if out is None:
         out = torch.empty((m, n), dtype=y.dtype, device=y.device)
     else:
-        _tensor("out", out, (m, n), y.dtype, y.device)
+        _given("out", out, (m, n), y.dtype, y.device)
     with _On(y.device) as stream:
         check(load_library().hoard_sort_combine(dt, m, k, n, _p(y), _p(place), _p(w), _p(res), _p(out), stream))
     return out
@@ -201,7 +208,7 @@ def sort_combine_grad(dout, y, place, w, *, dy=None):
     if dy is None:
         dy = torch.zeros_like(y)
     else:
-        _tensor("dy", dy, y.shape, y.dtype, y.device)
+        _given("dy", dy, y.shape, y.dtype, y.device)
     dw = torch.empty_like(w)
     with _On(y.device) as stream:
         check(load_library().hoard_sort_combine_grad(dt, m, k, n, _p(dout), _p(y), _p(place), _p(w), _p(dy), _p(dw),
@@ -266,7 +273,7 @@ def norm_forward(r, b=None, w_post=None, gate=None, w_pre=None, *, eps: float, s
     elif r_out is None:
         r_out = new(r.shape, r.dtype)
     else:
-        _tensor("r_out", r_out, r.shape, r.dtype, r.device)
+        _given("r_out", r_out, r.shape, r.dtype, r.device)
     h = new(r.shape, dtype) if w_pre is not None else None
     stats = new((r.shape[0], 2), torch.float32) if want_stats else None
     a = _norm_args(r, b, gate, w_post, w_pre, r_out, h, stats, dtype, eps, scale, w_offset, gate_sigmoid)

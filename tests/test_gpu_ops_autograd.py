@@ -49,3 +49,16 @@ def test_a_wanted_gradient_is_refused(calls, name):
         call({k: v.detach() for k, v in t.items()})
     with torch.inference_mode():
         call({k: v.clone() for k, v in tensors.items()})
+
+
+@pytest.mark.parametrize("name,out", [("q4_matmul", "out"), ("sort_gather", "out"), ("sort_combine", "out"), ("sort_combine_grad", "dy"),
+                                      ("norm_forward", "r_out")])
+def test_a_write_counts(calls, name, out):
+    """A tensor that autograd keeps for a gradient and a call then writes over: backward refuses it."""
+    call, tensors = calls[name]
+    t = {k: v.clone() for k, v in tensors.items()}
+    factor = torch.ones_like(t[out], requires_grad=True)
+    product = (factor * t[out]).sum()
+    call(t)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
