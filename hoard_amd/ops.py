@@ -2,9 +2,10 @@
 
 torch allocates the outputs and workspaces and hands over its current stream on
 the tensors' device; every computation is a call into libhoard_moe.so.  Calls are
-asynchronous on that stream.  Tensors are dense device tensors of one device
-(anything else raises HoardError); a tensor made on another stream is the
-caller's to order, as with any torch operator.
+asynchronous on that stream.  Tensors are dense device tensors of one device, and
+one given to write to lies apart from the inputs except where said (anything else
+raises HoardError); a tensor made on another stream is the caller's to order, as
+with any torch operator.
 
 A layer whose experts are 4-bit codes, M tokens, k of E experts each:
 
@@ -48,10 +49,15 @@ def _tensor(name: str, t, shape=None, dtype=None, device=None) -> None:
     _need(device is None or t.device == device, f"{name}: on {t.device}, wanted {device}")
 
 
-def _given(name: str, t, shape, dtype, device) -> None:
-    """Checks of a tensor to write to, whose version then counts the write: autograd refuses a gradient that needs what
-    it held."""
+def _given(name: str, t, shape, dtype, device, inputs=(), or_same=None) -> None:
+    """Checks of a tensor to write to: apart from the call's inputs, or all of `or_same`.  Its version counts the write:
+    autograd refuses a gradient that needs what it held."""
     _tensor(name, t, shape, dtype, device)
+    first, last = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+    for i in (*inputs, or_same):
+        if i is None or (i is or_same and i.data_ptr() == first):
+            continue
+        _need(last <= i.data_ptr() or i.data_ptr() + i.numel() * i.element_size() <= first, f"{name}: overlaps an input")
     torch.autograd.graph.increment_version(t)
 
 
@@ -124,7 +130,7 @@ def q4_matmul(x, w: Q4Weight, up: Q4Weight | None = None, *, ids=None, offsets=N
     if out is None:
         out = torch.empty((n_rows, w.rows), dtype=x.dtype, device=x.device)
     else:
-        _given("out", out, (n_rows, w.rows), x.dtype, x.device)
+        _given("out", out, (n_rows, w.rows), x.dtype, x.device, (x, ids, offsets))
     lib, a, b = load_library(), ctypes.byref(w.desc), ctypes.byref(up.desc) if up is not None else None
     with _On(x.device) as stream:
         if ids is not None:
@@ -180,7 +186,7 @@ def sort_gather(x, place, w=None, *, out=None):
     if out is None:
         out = torch.empty((m * k, n), dtype=x.dtype, device=x.device)
     else:
-        _given("out", out, (m * k, n), x.dtype, x.device)
+        _given("out", out, (m * k, n), x.dtype, x.device, (x, place, w))
     with _On(x.device) as stream:
         check(load_library().hoard_sort_gather(dt, m, k, n, _p(x), _p(place), _p(w), _p(out), stream))
     return out
@@ -194,7 +200,7 @@ def sort_combine(y, place, w=None, res=None, *, out=None):
     if out is None:
         out = torch.empty((m, n), dtype=y.dtype, device=y.device)
     else:
-        _given("out", out, (m, n), y.dtype, y.device)
+        _given("out", out, (m, n), y.dtype, y.device, (y, place, w), res)
     with _On(y.device) as stream:
         check(load_library().hoard_sort_combine(dt, m, k, n, _p(y), _p(place), _p(w), _p(res), _p(out), stream))
     return out
@@ -208,7 +214,7 @@ def sort_combine_grad(dout, y, place, w, *, dy=None):
     if dy is None:
         dy = torch.zeros_like(y)
     else:
-        _given("dy", dy, y.shape, y.dtype, y.device)
+        _given("dy", dy, y.shape, y.dtype, y.device, (dout, place, w), y)
     dw = torch.empty_like(w)
     with _On(y.device) as stream:
         check(load_library().hoard_sort_combine_grad(dt, m, k, n, _p(dout), _p(y), _p(place), _p(w), _p(dy), _p(dw),
@@ -273,7 +279,7 @@ def norm_forward(r, b=None, w_post=None, gate=None, w_pre=None, *, eps: float, s
     elif r_out is None:
         r_out = new(r.shape, r.dtype)
     else:
-        _given("r_out", r_out, r.shape, r.dtype, r.device)
+        _given("r_out", r_out, r.shape, r.dtype, r.device, (b, gate, w_post, w_pre), r)
     h = new(r.shape, dtype) if w_pre is not None else None
     stats = new((r.shape[0], 2), torch.float32) if want_stats else None
     a = _norm_args(r, b, gate, w_post, w_pre, r_out, h, stats, dtype, eps, scale, w_offset, gate_sigmoid)
