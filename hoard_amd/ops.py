@@ -10,7 +10,7 @@ with any torch operator.
 A layer whose experts are 4-bit codes, M tokens, k of E experts each:
 
     st = norm_forward(r, w_pre=w, eps=eps)                  # h = norm(r)
-    s = sort_pairs(ids, E)                                  # ids, w from the router
+    s = sort_pairs(ids, E)                                  # ids, w from the caller's router
     xs = sort_gather(st.h, s.place)
     hid = q4_matmul(xs, gate, up=up, offsets=s.offsets)     # silu(gate x) * (up x)
     y = q4_matmul(hid, down, offsets=s.offsets)
@@ -19,7 +19,8 @@ A layer whose experts are 4-bit codes, M tokens, k of E experts each:
 
 Gradients: sort_combine(dxs, place) is sort_gather's, sort_combine_grad and
 norm_backward are those of sort_combine and norm_forward.  The 4-bit products
-have none (their weights are constants, and they serve inference).  No call records
+have none (their weights are constants, and they serve inference), nor has the
+stage: a chain through the experts takes the caller's own gradient there.  No call records
 itself for autograd: where gradients are recorded, a tensor that wants one is refused
 (detach it, or call under torch.no_grad(), and run the backward calls yourself).
 """
