@@ -183,7 +183,8 @@ struct GradIn {
 // memory idle, and the weights stay.  Rows longer than 8192 (WIDE) would need 250
 // registers of the 128 that 1024 threads leave: two of the three sums lie in LDS, each
 // column in its thread's own words, and inputs are read again where they are used
-// (512 x 16384 in bf16: 48 us, 116 with the registers spilled; 1 row 12.3, 41.7).
+// (512 x 16384 in bf16: 48 us, 116 with all of it in registers, 215 to 360 of which
+// spilled; 1 row 12.3, 41.7).  6 registers a lane still do.
 template <typename T, typename R, int BS, int NV, bool NT>
 __global__ __launch_bounds__(BS) void norm_grad_kernel(hoard_norm_args a, hoard_norm_grads g, float *work) {
     constexpr bool AHEAD = BS <= 512 && NV * (2 * sizeof(R) + 2 * sizeof(T)) <= 16;
@@ -457,8 +458,8 @@ void grad_of(const hoard_norm_args &a, const hoard_norm_grads &g, float *work, h
 
 // As many groups as the chip holds at once (by their registers 3 of 256 threads a CU,
 // 1 of more; of 64 threads as many as the partial sums are worth), with equal shares
-// of the rows.  4096 x 2048, bf16: 29.4 us with 768 groups, 33.0 with 512, 37.7 with
-// 1024; 4096 x 4096: 62.5 with 256, 64.3 with 512, 74.0 with 768.
+// of the rows.  4096 x 2048, bf16: 29.4 us with at most 768 groups (683 of 6 rows), 33.0
+// with 512, 37.7 with 1024; 4096 x 4096: 62.5 with 256, 64.3 with 512, 74.0 with 683.
 int norm_groups(int n_rows, int n) {
     const int most = n <= 1024 ? 1024 : n <= 2048 ? 768 : 256;
     if (n_rows <= most) return n_rows;

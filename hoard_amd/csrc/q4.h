@@ -17,7 +17,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 // 16.0 adds exactly itself, so eight codes cost four shifts and four masked ors.
 // The sum over a group is then (sum of (16 + code) x) - (16 + zero) (sum of x),
 // whose terms are at most some five times the plain ones'.  Word j of the result
-// holds elements j (low) and j + 4 (high): x is laid out the same way (kOrder).
+// holds elements j (low) and j + 4 (high): x is laid out the same way (paired).
 template <typename T>
 struct Biased;
 template <>
