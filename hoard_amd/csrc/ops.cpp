@@ -16,6 +16,7 @@ bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) 
 
 constexpr int kMaxRows = 1 << 22;  // a launch's workgroups of 16 rows by 8 tiles of x within its 2^32 threads
 constexpr int kMaxCols = 1 << 20;  // 64 rows of x lie within the kernels' 32-bit offsets
+constexpr int kMaxMats = 1 << 30;  // a lane's run of matrices, rounded up, ends within 32 bits
 constexpr int kMaxN = 1 << 30;     // columns of the pairs' rows: a wave's step of 2048 past the last stays within 32 bits
 
 int launched(const char *what, hipError_t rc) {
@@ -30,6 +31,7 @@ int check_matrix(const char *what, const hoard_q4_matrix &m) {
     if (!m.codes || !m.scales) return fail_fmt(HOARD_ERR_INVALID, "%s: null codes or scales", what);
     if (!aligned(m.codes, 16)) return fail_fmt(HOARD_ERR_INVALID, "%s: codes are not 16-byte aligned", what);
     if (m.rows <= 0 || m.n_mat <= 0) return fail_fmt(HOARD_ERR_INVALID, "%s: rows %d, n_mat %d", what, m.rows, m.n_mat);
+    if (m.n_mat > kMaxMats) return fail_fmt(HOARD_ERR_UNSUPPORTED, "%s: n_mat %d above %d", what, m.n_mat, kMaxMats);
     if (m.rows > kMaxRows) return fail_fmt(HOARD_ERR_UNSUPPORTED, "%s: rows %d above %d", what, m.rows, kMaxRows);
     if (m.group != 32 && m.group != 64 && m.group != 128)
         return fail_fmt(HOARD_ERR_UNSUPPORTED, "%s: group %d is not 32, 64 or 128", what, m.group);

@@ -42,7 +42,7 @@ extern "C" {
 
 /* n_mat matrices of rows x cols weights, row r of matrix e at index e*rows + r:
    weight k = scale[k / group] * (code[k] - zero[k / group]), zero 8 without
-   zeros.  rows is at most 2^22; cols is a multiple of group, at most 2^20. */
+   zeros.  rows is at most 2^22, n_mat 2^30; cols is a multiple of group, at most 2^20. */
 typedef struct hoard_q4_matrix {
     const void *codes;    /* [n_mat*rows][cols/2] bytes, 16-byte aligned: byte j holds code 2j in
                              its low half and code 2j+1 in its high half */

@@ -26,3 +26,11 @@ def test_norm_workspace_of_many_rows(hlib, rows, n):
     a.r_out, a.w_pre, a.stats = A, A, A
     g = H.NormGrads(None, A, A, None, None, None, A)
     assert hlib.hoard_norm_backward(ctypes.byref(a), ctypes.byref(g), A, need.value - 1, None) == H.ERR_INVALID
+
+
+@pytest.mark.parametrize("n_mat", [2**30 + 1, 2**31 - 1])
+def test_too_many_matrices(hlib, n_mat):
+    w = ctypes.byref(H.Q4Matrix(A, A, None, 1, 32, 32, n_mat, H.TYPE_F16))
+    assert hlib.hoard_q4_matmul_sorted(w, None, H.TYPE_BF16, 1, A, A, A, None) == H.ERR_UNSUPPORTED
+    assert hlib.hoard_q4_matmul_ids(w, None, H.TYPE_BF16, 1, A, 1, A, A, None) == H.ERR_UNSUPPORTED
+    assert f"n_mat {n_mat}" in hlib.hoard_last_error().decode()
