@@ -59,7 +59,8 @@ def _given(name: str, t, shape, dtype, device, inputs=(), or_same=None) -> None:
         if i is None or (i is or_same and i.data_ptr() == first):
             continue
         _need(last <= i.data_ptr() or i.data_ptr() + i.numel() * i.element_size() <= first, f"{name}: overlaps an input")
-    torch.autograd.graph.increment_version(t)
+    if not t.is_inference():  # one made in inference mode has no version, and autograd keeps none
+        torch.autograd.graph.increment_version(t)
 
 
 def _type(name: str, t) -> int:

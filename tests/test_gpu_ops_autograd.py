@@ -62,3 +62,12 @@ def test_a_write_counts(calls, name, out):
     call(t)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         product.backward()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tensors_of_inference_mode(calls, name):
+    """Buffers made in inference mode are written to outside it."""
+    call, tensors = calls[name]
+    with torch.inference_mode():
+        t = {k: v.clone() for k, v in tensors.items()}
+    call(t)
