@@ -49,11 +49,10 @@ __device__ __forceinline__ v4u biased(uint32_t codes) {
 // Codes plus kInOrderBias in their own order, words {0, 1}, {2, 3}, {4, 5}, {6, 7}, for x
 // that is not rearranged.  f16: the code in the lowest fraction bits of 1024, so that a
 // byte permute and a masked or make a word; the sum is taken off exactly (less).  bf16:
-// half a byte is the 8-bit float (4 exponent bits, the lowest of which the code's fourth
-// bit is) of code * 2^-9, which one conversion to bf16 takes two at a time: no offset,
-// whose sums 32 bits would round at 128 + code for what a code of some 8 less its zero
-// point is worth (0.36 % of a prompt's results then fell to the other side of their
-// bf16 rounding).
+// half a byte is the 8-bit float of code * 2^-9 (4 exponent bits, the lowest of which is
+// the code's fourth bit), which one conversion to bf16 takes two at a time.  There is no
+// offset to correct: sums of 128 + code, at the same cost, lost four bits to it, and
+// 0.36 % of a prompt's results fell to the other side of their bf16 rounding (now 0.015).
 template <typename T>
 constexpr float kInOrderBias = __is_same(T, bf16) ? 0.0f : 1024.0f;
 template <typename T>

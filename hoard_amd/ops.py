@@ -20,9 +20,9 @@ A layer whose experts are 4-bit codes, M tokens, k of E experts each:
 Gradients: sort_combine(dxs, place) is sort_gather's, sort_combine_grad and
 norm_backward are those of sort_combine and norm_forward.  The 4-bit products
 have none (their weights are constants, and they serve inference), nor has the
-stage: a chain through the experts takes the caller's own gradient there.  No call records
-itself for autograd: where gradients are recorded, a tensor that wants one is refused
-(detach it, or call under torch.no_grad(), and run the backward calls yourself).
+stage: a chain through the experts takes the caller's own gradient there.  No call
+records itself for autograd: where gradients are recorded, a tensor that wants one is
+refused (detach it, or call under torch.no_grad(), and run the backward calls yourself).
 """
 from __future__ import annotations
 
@@ -56,8 +56,8 @@ def _given(name: str, t, shape, dtype, device, inputs=(), or_same=None) -> None:
     _tensor(name, t, shape, dtype, device)
     first, last = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
     for i in (*inputs, or_same):
-        if i is None or (i is or_same and i.data_ptr() == first):
-            continue
+        if not isinstance(i, torch.Tensor) or (i is or_same and i.data_ptr() == first):
+            continue  # what is no tensor is refused by its own checks
         _need(last <= i.data_ptr() or i.data_ptr() + i.numel() * i.element_size() <= first, f"{name}: overlaps an input")
     if not t.is_inference():  # one made in inference mode has no version, and autograd keeps none
         torch.autograd.graph.increment_version(t)

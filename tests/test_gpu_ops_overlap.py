@@ -40,3 +40,11 @@ def test_overlaps():
     ops.sort_combine(y, place, wt, x, out=x)
     ops.sort_combine_grad(x, y, place, wt, dy=y)
     ops.norm_forward(x, at(400, 3, 40), w_pre=par, eps=1e-6, r_out=x)
+
+
+def test_what_is_no_tensor_is_refused_as_that():
+    from hoard_amd import ops
+    r, b, par = torch.randn((3, 40), device="cuda"), torch.randn((3, 40), device="cuda"), torch.ones(40, device="cuda")
+    for kw in (dict(gate=[1.0] * 40), dict(gate=0.5), dict(w_post=[1.0] * 40)):
+        with pytest.raises(H.HoardError):
+            ops.norm_forward(r, b, w_pre=par, eps=1e-6, r_out=r, **kw)
