@@ -19,6 +19,7 @@ TYPE_Q3_K = 11
 TYPE_Q4_K = 12
 TYPE_Q5_K = 13
 TYPE_Q6_K = 14
+TYPE_I8 = 24
 TYPE_BF16 = 30
 BLOCK_BYTES = {TYPE_Q3_K: 110, TYPE_Q4_K: 144, TYPE_Q5_K: 176, TYPE_Q6_K: 210}
 
@@ -114,8 +115,37 @@ class NormGrads(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("dr_out", "dh", "dr", "db", "dgate", "dw_post", "dw_pre")]
 
 
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, ctypes.c_int32) for n in ("type", "n_pages", "page", "n_kv_heads", "head_dim")]
+
+
+class HeadsArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("type", "n_tokens", "n_q_heads", "n_kv_heads", "head_dim", "rot_dim", "rope",
+                                              "n_axes")] + \
+               [(n, ctypes.c_float) for n in ("eps", "w_offset")] + \
+               [(n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("q", "k", "v", "w_q", "w_k", "pos", "freq", "axis", "q_out", "k_out", "stats",
+                                               "cache", "slots")]
+
+
+class HeadsGrads(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dq_out", "dk_out", "dq", "dk", "dw_q", "dw_k")] + \
+               [(n, ctypes.c_int64) for n in ("dq_stride", "dk_stride")]
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("type", "n_seq", "n_new", "n_q_heads", "max_pages")] + \
+               [("scale", ctypes.c_float), ("q_stride", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("q", "pages", "lens", "out", "lse")]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_int64
 # name -> (restype, argtypes); every symbol the public headers declare
 ABI = {
     "hoard_last_error": (ctypes.c_char_p, []),
@@ -171,6 +201,13 @@ ABI = {
     "hoard_norm_forward": (_I, [_P, _P]),
     "hoard_norm_backward": (_I, [_P, _P, _P, ctypes.c_size_t, _P]),
     "hoard_norm_workspace": (_I, [_P, ctypes.POINTER(ctypes.c_size_t)]),
+    "hoard_kv_write": (_I, [_P, _I, _I, _P, _P, _L, _P, _L, _P]),
+    "hoard_kv_read": (_I, [_P, _I, _I, _P, _P, _L, _P, _L, _P]),
+    "hoard_heads_forward": (_I, [_P, _P]),
+    "hoard_heads_backward": (_I, [_P, _P, _P, ctypes.c_size_t, _P]),
+    "hoard_heads_workspace": (_I, [_P, ctypes.POINTER(ctypes.c_size_t)]),
+    "hoard_attn_decode": (_I, [_P, _P, _P, ctypes.c_size_t, _P]),
+    "hoard_attn_workspace": (_I, [_P, _P, ctypes.POINTER(ctypes.c_size_t)]),
     "hoard_synth_key": (ctypes.c_uint64, [ctypes.c_uint32] * 5),
     "hoard_synth_fill_blocks": (_I, [_I, ctypes.c_uint64, _P, ctypes.c_size_t, ctypes.c_float]),
     "hoard_synth_fill_normal": (None, [ctypes.c_uint64, _P, ctypes.c_size_t, ctypes.c_float]),
