@@ -1,106 +1,104 @@
-// Attention of a few new tokens a sequence over a paged cache (hoard_attn_decode).
-//
-//   S_j = scale <q, k_j>,  out = sum_j exp(S_j - m) v_j / sum_j exp(S_j - m),  m = max_j S_j,
-// over the keys that the row sees; lse = m + log sum_j exp(S_j - m).
-//
-// A workgroup takes one query head of one new token, its four waves every fourth run of 64
-// keys: a lane forms its key's score, then the lanes take the columns of the values.  Sums
-// and maxima of what a wave has seen run along and are joined at the end.
+// Attention over a paged cache: how a call is split, and its parts joined
+// (hoard_attn_decode).  The attention itself is in attn_tiles.h.
 #include "attn.h"
+#include "attn_split.h"
 #include "opsdev.h"
 
 namespace hoard {
 
 namespace {
 
-// The cache's row of key j; -1 where its page is none.
-__device__ __forceinline__ int64_t row_of(const hoard_kv_cache &c, const int32_t *pages, int head, int j) {
-    const int page = pages[j / c.page];
-    if (page < 0 || page >= c.n_pages) return -1;
-    return ((int64_t)page * c.n_kv_heads + head) * c.page + j % c.page;
-}
+typedef float v4f __attribute__((ext_vector_type(4)));
 
-template <typename T, typename C>
-__global__ __launch_bounds__(256) void attn_kernel(hoard_kv_cache c, hoard_attn_args a) {
-    __shared__ float q[256], part[4][256], top[4], sum[4];
-    const int64_t token = blockIdx.x;
-    const int head = blockIdx.y, kv = head / (a.n_q_heads / c.n_kv_heads), dim = c.head_dim;
-    const int lane = threadIdx.x & 63, wave = wave_index();
-    const int n = (int)min((int64_t)a.lens[token], (int64_t)a.max_pages * c.page);
-    const int32_t *pages = a.pages + token / a.n_new * a.max_pages;
-    if ((int)threadIdx.x < dim) q[threadIdx.x] = (float)(static_cast<const T *>(a.q) + token * a.q_stride + head * dim)[threadIdx.x];
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, acc[4] = {};
-    for (int at = wave * 64; at < n; at += 256) {
-        const int j = at + lane;
-        const int64_t row = j < n ? row_of(c, pages, kv, j) : -1;
-        float s = -INFINITY;
-        if (row >= 0) {
-            const C *k = static_cast<const C *>(c.k) + row * dim;
-            s = 0.0f;
-            for (int d = 0; d < dim; d++) s = fmaf(q[d], (float)k[d], s);
-            s *= a.scale;
-            if (sizeof(C) == 1) s *= c.k_scale[row];
-        }
-        const uint64_t seen = __ballot(row >= 0);
-        if (!seen) continue;
-        float most = row >= 0 ? s : -INFINITY;
-        for (int off = 1; off < 64; off *= 2) most = fmaxf(most, __shfl_xor(most, off));
-        most = fmaxf(m, most);
-        const float base = most > -INFINITY ? most : 0.0f, old = expf(m - base);
-        const float e = row >= 0 ? expf(s - base) : 0.0f;
-        m = most;
-        l = l * old + wave_sum_f(e);
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] *= old;
-        for (int i = 0; i < 64; i++) {
-            if (!(seen >> i & 1)) continue;
-            const int64_t r = __shfl(row, i);
-            float w = __shfl(e, i);
-            if (sizeof(C) == 1) w *= c.v_scale[r];
-            const C *v = static_cast<const C *>(c.v) + r * dim;
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (lane + 64 * k < dim) acc[k] = fmaf(w, (float)v[lane + 64 * k], acc[k]);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; k++) part[wave][lane + 64 * k] = acc[k];
-    if (lane == 0) {
-        top[wave] = m;
-        sum[wave] = l;
-    }
-    __syncthreads();
-    m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    const float base = m > -INFINITY ? m : 0.0f;
-    float o = 0.0f;
-    l = 0.0f;
-    for (int w = 0; w < 4; w++) {
-        const float f = expf(top[w] - base);
-        l += f * sum[w];
-        o += f * part[w][threadIdx.x];
-    }
-    if ((int)threadIdx.x < dim)
-        (static_cast<T *>(a.out) + (token * a.n_q_heads + head) * dim)[threadIdx.x] = (T)(l != 0.0f ? o / l : 0.0f);
-    if (threadIdx.x == 0 && a.lse) a.lse[token * a.n_q_heads + head] = base + logf(l);
-}
-
+// out = sum_s w_s part_s,  w_s = 2^(lse_s - m) / sum: the parts of one row, each already
+// divided by its own sum.  A workgroup takes a row: four columns a thread, the parts dealt
+// to the threads left over, which meet in LDS.
 template <typename T>
-void attn_type(const hoard_kv_cache &c, const hoard_attn_args &a, hipStream_t s) {
-    const dim3 grid(a.n_seq * a.n_new, a.n_q_heads);
-    if (c.type == HOARD_TYPE_F16) attn_kernel<T, f16><<<grid, 256, 0, s>>>(c, a);
-    else if (c.type == HOARD_TYPE_BF16) attn_kernel<T, bf16><<<grid, 256, 0, s>>>(c, a);
-    else attn_kernel<T, int8_t><<<grid, 256, 0, s>>>(c, a);
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnCall p) {
+    __shared__ float weight[kMaxSplits], stat[2][4];
+    __shared__ v4f outs[256];
+    const hoard_attn_args &a = p.a;
+    const int64_t token = blockIdx.x, row = token * a.n_q_heads + blockIdx.y, seq = token / a.n_new;
+    const int lane = threadIdx.x & 63, dim = p.c.head_dim;
+    const int limit = a.max_pages * p.c.page;
+    int most = 0;
+    for (int t = 0; t < a.n_new; t++) most = max(most, min(max(a.lens[seq * a.n_new + t], 0), limit));
+    const AttnParts parts = attn_parts(most, p.splits, 4 / p.row_waves);
+    if (parts.used <= 1) return;
+    const float *lse = p.part_lse + row * p.splits;
+    const float mine = (int)threadIdx.x < parts.used ? lse[threadIdx.x] : -INFINITY;
+    // a NaN of one part is everyone's
+    const float top = wave_max_f(mine);
+    if (lane == 0) stat[0][wave_index()] = top;
+    __syncthreads();
+    float m = fmaxf(fmaxf(stat[0][0], stat[0][1]), fmaxf(stat[0][2], stat[0][3]));
+    m = m > -INFINITY ? m : 0.0f;
+    const float w = exp2f(mine - m), s = wave_sum_f(w);
+    if (lane == 0) stat[1][wave_index()] = s;
+    if ((int)threadIdx.x < kMaxSplits) weight[threadIdx.x] = w;
+    __syncthreads();
+    const float sum = (stat[1][0] + stat[1][1]) + (stat[1][2] + stat[1][3]), f = sum != 0.0f ? 1.0f / sum : 0.0f;
+    const int quads = dim / 4, deep = 256 / quads, quad = threadIdx.x % quads, from = threadIdx.x / quads;
+    v4f o = {0, 0, 0, 0};
+    if (from < deep) {
+        const float *part = p.part_out + row * p.splits * dim + 4 * quad;
+#pragma unroll 4
+        for (int i = from; i < parts.used; i += deep) {
+            const float wi = weight[i];
+            // a part of which the row sees nothing holds zeros
+            o += wi * *reinterpret_cast<const v4f *>(part + (int64_t)i * dim);
+        }
+    }
+    outs[threadIdx.x] = o;
+    __syncthreads();
+    if (from == 0) {
+        for (int i = 1; i < deep; i++) o += outs[i * quads + quad];
+        T *to = static_cast<T *>(a.out) + row * dim + 4 * quad;
+#pragma unroll
+        for (int k = 0; k < 4; k++) to[k] = (T)(o[k] * f);
+    }
+    if (threadIdx.x == 0 && a.lse) a.lse[row] = (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Waves side by side over the rows where there are more than 16; workgroups for about two
+// a CU, a sequence split into as many parts as that leaves.
+AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work) {
+    AttnCall p{};
+    p.c = c;
+    p.a = a;
+    const int rows = a.n_new * (a.n_q_heads / c.n_kv_heads), tiles = (rows + 15) / 16;
+    p.row_waves = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
+    p.row_blocks = (tiles + p.row_waves - 1) / p.row_waves;
+    const int64_t groups = (int64_t)a.n_seq * c.n_kv_heads * p.row_blocks;
+    const int64_t keys = (int64_t)a.max_pages * c.page, deep = 4 / p.row_waves;
+    const int64_t most = (keys + kKeyTile * deep - 1) / (kKeyTile * deep);
+    int64_t splits = groups ? kAttnGroups / groups : 1;
+    splits = splits > most ? most : splits;
+    p.splits = (int)(splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits);
+    const int64_t all = (int64_t)a.n_seq * a.n_new * a.n_q_heads * p.splits;
+    p.part_out = work;
+    p.part_lse = work ? work + all * c.head_dim : nullptr;
+    return p;
 }
 
 }  // namespace
 
-size_t attn_work_bytes(const hoard_kv_cache &, const hoard_attn_args &) { return 0; }
+size_t attn_work_bytes(const hoard_kv_cache &c, const hoard_attn_args &a) {
+    const AttnCall p = call_of(c, a, nullptr);
+    if (p.splits == 1) return 0;
+    return sizeof(float) * (size_t)(c.head_dim + 1) * a.n_seq * a.n_new * a.n_q_heads * p.splits;
+}
 
-hipError_t launch_attn(const hoard_kv_cache &c, const hoard_attn_args &a, float *, hipStream_t s) {
-    if (a.type == HOARD_TYPE_F32) attn_type<float>(c, a, s);
-    else if (a.type == HOARD_TYPE_F16) attn_type<f16>(c, a, s);
-    else attn_type<bf16>(c, a, s);
+hipError_t launch_attn(const hoard_kv_cache &c, const hoard_attn_args &a, float *work, hipStream_t s) {
+    const AttnCall p = call_of(c, a, work);
+    const hipError_t rc = c.type == HOARD_TYPE_F16    ? launch_attn_f16(p, s)
+                          : c.type == HOARD_TYPE_BF16 ? launch_attn_bf16(p, s)
+                                                      : launch_attn_i8(p, s);
+    if (rc != hipSuccess || p.splits == 1) return rc;
+    const dim3 grid(a.n_seq * a.n_new, a.n_q_heads);
+    if (a.type == HOARD_TYPE_F32) attn_join_kernel<float><<<grid, 256, 0, s>>>(p);
+    else if (a.type == HOARD_TYPE_F16) attn_join_kernel<f16><<<grid, 256, 0, s>>>(p);
+    else attn_join_kernel<bf16><<<grid, 256, 0, s>>>(p);
     return hipGetLastError();
 }
 

@@ -1,0 +1,523 @@
+// Attention of a few new tokens a sequence over a paged cache, on matrix instructions
+// (v_mfma_f32_16x16x32_{f16,bf16}).
+//
+//   S_j = scale <q, k_j>,  out = sum_j exp(S_j - m) v_j / sum_j exp(S_j - m),  m = max_j S_j
+//
+// The rows that share a key head, the query heads of its group for each new token, are
+// taken 16 at a time; a wave takes 16 of them and every KW-th tile of 32 keys.  It needs no
+// LDS and no other lane's data in its loop but two exchanges for the maximum:
+//   S^T = K Q^T: a lane reads 16 bytes of one key (operand A) and gets 8 scores of one row
+//   (column lane % 16; keys 4 (lane / 16) + 0..3 of either half of the tile).  Those are,
+//   as they lie, operand B of
+//   out^T = V^T P^T, whose order of keys is free as long as V's is the same: a lane reads 8
+//   columns of those same 8 keys and transposes the 8 x 8 values in its registers.  It ends
+//   with 32 consecutive columns of one row, and the row's maximum and factor are its own.
+// The next tile's keys are fetched once this tile's scores are formed, its values once this
+// tile's are used, so that half a tile or more is in flight all the time.
+//
+// Bound by memory: 4 rows * dim operations a key for 2 dim values, 16 rows at a time, is
+// far below what the matrix instructions do meanwhile.  So they take more of them where
+// that keeps digits: weights as two 16-bit planes (f16: 22 bits, bf16: 16; three for fp32:
+// 24), fp32 queries as two f16 planes of a row brought by a power of two to 2^14 or as three
+// bf16 planes.  8-bit codes become f16 exactly (the byte as a subnormal, times 2^15 less a
+// quarter: code * 2^-9); a key's scale multiplies its score, a value's its weight, relative
+// to the power of two above the largest scale so far, so that the weights stay in f16's range.
+#pragma once
+
+#include <math.h>
+
+#include "attn.h"
+#include "attn_split.h"
+#include "opsdev.h"
+
+namespace hoard {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+namespace attn {
+
+// The elements that products are formed in, and the planes of queries and weights.
+template <typename T, typename C>
+struct Core {
+    typedef f16 E;
+    static constexpr int qp = __is_same(T, float) ? 2 : 1, pp = 2;
+};
+template <typename T>
+struct Core<T, bf16> {
+    typedef bf16 E;
+    static constexpr int qp = __is_same(T, float) ? 3 : __is_same(T, f16) ? 2 : 1, pp = __is_same(T, float) ? 3 : 2;
+};
+
+__device__ __forceinline__ v4f product(f16, v4u a, v4u b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f product(bf16, v4u a, v4u b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+// Two values rounded to nearest, and what that leaves of them.
+__device__ __forceinline__ uint32_t plane(f16, v2f &x) {
+    const v2h h = __builtin_convertvector(x, v2h);
+    x -= __builtin_convertvector(h, v2f);
+    return __builtin_bit_cast(uint32_t, h);
+}
+__device__ __forceinline__ uint32_t plane(bf16, v2f &x) {
+    const v2bf h = __builtin_convertvector(x, v2bf);
+    x -= __builtin_convertvector(h, v2f);
+    return __builtin_bit_cast(uint32_t, h);
+}
+
+// Waits out the last matrix instruction (8 wait states) before vector instructions read
+// its result behind a branch, over which the compiler does not count them.
+__device__ __forceinline__ void settle(v4f &a, v4f &b) { asm volatile("s_nop 7" : "+v"(a), "+v"(b)); }
+template <int N>
+__device__ __forceinline__ void settle(v4f (&a)[N]) {
+    static_assert(N % 4 == 0, "four at a time");
+    // the products come in ascending order: behind the last four's wait all are done
+    asm volatile("s_nop 7" : "+v"(a[N - 4]), "+v"(a[N - 3]), "+v"(a[N - 2]), "+v"(a[N - 1]));
+#pragma unroll
+    for (int i = 0; i + 4 < N; i += 4) asm volatile("s_nop 7" : "+v"(a[i]), "+v"(a[i + 1]), "+v"(a[i + 2]), "+v"(a[i + 3]));
+}
+
+// Maximum and sum over the four lanes 16 apart, in all of them.
+__device__ __forceinline__ float far_max(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float far_sum(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ int row16_max_i(int v) {
+    v = max(v, dpp_i<kDppQuadXor1>(v));
+    v = max(v, dpp_i<kDppQuadXor2>(v));
+    v = max(v, dpp_i<kDppRowHalfMirror>(v));
+    return max(v, dpp_i<kDppRowMirror>(v));
+}
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Two codes (plus 128), the low bytes of the halves of w, as f16: code * 2^-9.
+constexpr int kCodeShift = 9;
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
+    const v2h up = {(f16)32768.0f, (f16)32768.0f}, less = {(f16)-0.25f, (f16)-0.25f};
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(v2h, w), up, less));
+}
+// Eight codes of a key, in their order.
+__device__ __forceinline__ v4u codes_row(v2u w) {
+    w ^= 0x80808080u;
+    v4u o;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        o[2 * i] = codes_f16(__builtin_amdgcn_perm(0, w[i], 0x0c010c00));
+        o[2 * i + 1] = codes_f16(__builtin_amdgcn_perm(0, w[i], 0x0c030c02));
+    }
+    return o;
+}
+
+// A lane's part of a tile of 32 keys as it lies in memory: of the keys 16-byte pieces for
+// the products' steps, of the values DV columns (a piece) of each of 8 keys.
+template <typename C, int DP>
+struct Shape {
+    static constexpr int DV = DP == 64 ? 4 : 8;              // columns of a lane, and once more 128 further on
+    static constexpr int H = DP / (16 * DV), NC = DV * H;    // products of a tile's values
+    static constexpr int STEPS = DP / 32;                    // products of a tile's keys, each half
+    static constexpr int KL = DP * (int)sizeof(C) / 64;      // pieces of a key
+    static constexpr int VW = DV * (int)sizeof(C) / 4;       // words of a piece of a value
+    typedef uint32_t piece __attribute__((ext_vector_type(VW)));
+};
+
+}  // namespace attn
+
+// One workgroup: 4 waves, `row_waves` wide over the rows and 4 / row_waves deep over the
+// keys of part blockIdx.x % splits of sequence blockIdx.x / splits.
+template <typename T, typename C, int DP, bool WHOLE>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCall p) {
+    using namespace attn;
+    typedef Shape<C, DP> G;
+    typedef Core<T, C> K;
+    typedef typename K::E E;
+    constexpr bool CODES = sizeof(C) == 1, HALF = __is_same(E, f16), SCALED = HALF && !__is_same(T, f16);
+    constexpr int DV = G::DV, NC = G::NC, STEPS = G::STEPS;
+    // f16 weights reach from 2^15 down
+    constexpr float kLift = HALF ? 15.0f : 0.0f;
+    __shared__ float stat[4][2][16];
+    __shared__ v4f outs[4][16][16 * DV / 4 + 1];
+
+    const hoard_kv_cache &c = p.c;
+    const hoard_attn_args &a = p.a;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wave = wave_index();
+    const int seq = blockIdx.x / p.splits, split = blockIdx.x % p.splits, kv = blockIdx.y;
+    const int group = a.n_q_heads / c.n_kv_heads, rows = a.n_new * group, dim = WHOLE ? DP : c.head_dim;
+    const int rw = wave % p.row_waves, kw = wave / p.row_waves, kw_all = 4 / p.row_waves;
+    const int row0 = (blockIdx.z * p.row_waves + rw) * 16, row = min(row0 + n, rows - 1);
+
+    // the keys that each new token sees, most of all, and most and fewest of the wave's rows
+    const int limit = a.max_pages * c.page;
+    const int seen = lane < a.n_new ? min(max(a.lens[(int64_t)seq * a.n_new + lane], 0), limit) : 0;
+    int most = row16_max_i(seen);
+    most = max(max(__builtin_amdgcn_readlane(most, 0), __builtin_amdgcn_readlane(most, 16)),
+               max(__builtin_amdgcn_readlane(most, 32), __builtin_amdgcn_readlane(most, 48)));
+    const int mine = __shfl(seen, row / group);
+    const int hi = row0 < rows ? __builtin_amdgcn_readfirstlane(row16_max_i(mine)) : 0;
+    const int lo = -__builtin_amdgcn_readfirstlane(row16_max_i(-mine));
+
+    const AttnParts parts = attn_parts(most, p.splits, kw_all);
+    if (split && split >= parts.used) return;
+    const int end = min(min((split + 1) * parts.per, parts.tiles), (hi + kKeyTile - 1) / kKeyTile);
+    int ti = split * parts.per + kw;
+
+    // queries, as planes: the k-th values of a product's step are those that the keys' pieces hold
+    v4u q[K::qp][STEPS];
+    int up = 0;  // q is held times 2^up
+    {
+        const T *from = static_cast<const T *>(a.q) + ((int64_t)seq * a.n_new + row / group) * a.q_stride +
+                        (kv * group + row % group) * dim;
+        float x[STEPS][8];
+        int top = 0;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const int d = CODES ? (s / 2) * 64 + 16 * g + (s % 2) * 8 : s * 32 + 8 * g;
+            widen(fetch(from, Cols{d < dim ? d : 0, 0}, dim), x[s]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[s][i] = d < dim && row0 + n < rows ? x[s][i] : 0.0f;
+                top = max(top, __float_as_int(x[s][i]) & 0x7fffffff);
+            }
+        }
+        if constexpr (SCALED) {
+            auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            top = max((int)r[0], (int)r[1]);
+            r = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+            top = max((int)r[0], (int)r[1]);
+            up = top ? 14 + 127 - (top >> 23) : 0;
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v2f v = {x[s][2 * i], x[s][2 * i + 1]};
+                if constexpr (SCALED) v = v2f{ldexpf(v[0], up), ldexpf(v[1], up)};
+#pragma unroll
+                for (int pl = 0; pl < K::qp; pl++) q[pl][s][i] = plane(E(), v);
+            }
+    }
+    const float to_log2 = a.scale * 1.4426950408889634f;
+    const int down = (CODES ? kCodeShift : 0) - up;
+
+    // page numbers of 64 pages from `page0` on, a lane each
+    const int shift = 31 - __builtin_clz(c.page), last_page = (max(most, 1) - 1) >> shift;
+    const int32_t *table = a.pages + (int64_t)seq * a.max_pages;
+    int page0 = 0, numbers = 0;
+    struct Where {
+        int64_t at[2];  // the cache's rows of the tile's halves
+        bool ok[2];
+    };
+    auto fill = [&](int from) {
+        page0 = from;
+        numbers = table[min(from + lane, last_page)];
+    };
+    auto where = [&](int tile) {
+        Where w;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int j = tile * kKeyTile + 16 * t, page = min(j >> shift, last_page);
+            if (page - page0 >= 64) fill(page);
+            const int number = __builtin_amdgcn_readlane(numbers, page - page0);
+            w.ok[t] = (uint32_t)number < (uint32_t)c.n_pages;
+            w.at[t] = ((int64_t)(w.ok[t] ? number : 0) * c.n_kv_heads + kv) * c.page + (j & (c.page - 1));
+        }
+        return w;
+    };
+
+    v4u key[2][G::KL];
+    typename G::piece val[8][G::H];
+    v4f key_scale[2], val_scale[2];
+    auto fetch_keys = [&](const Where &w) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const char *from = static_cast<const char *>(c.k) + w.at[t] * dim * (int64_t)sizeof(C);
+#pragma unroll
+            for (int s = 0; s < G::KL; s++) {
+                const int d = (s * 64 + 16 * g) / (int)sizeof(C);
+                const int off = (n * dim + (WHOLE || d < dim ? d : 0)) * (int)sizeof(C);
+                key[t][s] = *reinterpret_cast<const v4u *>(from + off);
+            }
+            if constexpr (CODES) key_scale[t] = *reinterpret_cast<const v4f *>(c.k_scale + w.at[t] + 4 * g);
+        }
+    };
+    auto fetch_values = [&](const Where &w) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const char *from = static_cast<const char *>(c.v) + w.at[t] * dim * (int64_t)sizeof(C);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int h = 0; h < G::H; h++) {
+                    const int d = DV * n + 16 * DV * h;
+                    const int off = ((4 * g + r) * dim + (WHOLE || d < dim ? d : 0)) * (int)sizeof(C);
+                    val[4 * t + r][h] = *reinterpret_cast<const typename G::piece *>(from + off);
+                }
+            if constexpr (CODES) val_scale[t] = *reinterpret_cast<const v4f *>(c.v_scale + w.at[t] + 4 * g);
+        }
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    v4f acc[NC] = {};
+    int val_up = 0;  // acc is held times 2^-val_up
+    float val_most = 0.0f;
+    bool odd = false;
+    Where cur{}, next{};
+    if (ti < end) {
+        fill((ti * kKeyTile) >> shift);
+        cur = where(ti);
+        fetch_keys(cur);
+        fetch_values(cur);
+    }
+    for (; ti < end; ti += kw_all, cur = next) {
+        const bool full = (ti + 1) * kKeyTile <= lo && cur.ok[0] && cur.ok[1];
+        const bool more = ti + kw_all < end;
+        if (more) next = where(ti + kw_all);
+
+        if constexpr (!WHOLE) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int s = 0; s < G::KL; s++)
+                    if ((s * 64 + 16 * g) / (int)sizeof(C) >= dim) key[t][s] = v4u{0, 0, 0, 0};
+        }
+        v4f score[2] = {};
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                v4u k;
+                if constexpr (CODES) {
+                    const v4u w = key[t][s / 2];
+                    k = codes_row(s % 2 ? v2u{w[2], w[3]} : v2u{w[0], w[1]});
+                } else {
+                    k = key[t][s];
+                }
+#pragma unroll
+                for (int pl = 0; pl < K::qp; pl++) score[t] = product(E(), k, q[pl][s], score[t]);
+            }
+        settle(score[0], score[1]);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[i] = score[i / 4][i % 4] * to_log2;
+            if constexpr (CODES) x[i] *= key_scale[i / 4][i % 4];
+            if constexpr (CODES || SCALED) x[i] = ldexpf(x[i], down);
+        }
+        if (more) fetch_keys(next);
+        if (!full) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4 >= mine || !cur.ok[i / 4]) x[i] = -INFINITY;
+        }
+        const float top = far_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
+        if (__any(top > m)) {
+            const float f = top > m ? exp2_of(m - top) : 1.0f;
+            settle(acc);
+            m = fmaxf(m, top);
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < NC; i++) acc[i] *= f;
+        }
+        const float base = (m > -INFINITY ? m : 0.0f) - kLift;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[i] = exp2_of(x[i] - base);
+            l += x[i];
+        }
+
+        // Values of keys that no row of the wave sees count as zeros, and so do, where a row
+        // does not see the key, those that are not finite: zero times them is not zero.  The
+        // rows that do see them get them after the loop.
+        if (!full) {
+            constexpr uint32_t exponent = HALF ? 0x7c00u : 0x7f80u;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int j = ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4;
+                const bool none = j >= hi || !cur.ok[i / 4];
+                if constexpr (CODES) {
+                    const float scale = val_scale[i / 4][i % 4];
+                    const bool bad = j >= lo && !(fabsf(scale) <= 3.4028235e38f);
+                    odd |= bad && !none;
+                    val_scale[i / 4][i % 4] = none || bad ? 0.0f : scale;
+                } else {
+#pragma unroll
+                    for (int h = 0; h < G::H; h++)
+#pragma unroll
+                        for (int w = 0; w < G::VW; w++) {
+                            const uint32_t v = val[i][h][w];
+                            const bool low = (v & exponent) == exponent, high = (v >> 16 & exponent) == exponent;
+                            const uint32_t kept = j < lo ? v : v & (low ? 0xffff0000u : ~0u) & (high ? 0x0000ffffu : ~0u);
+                            odd |= kept != v && !none;
+                            val[i][h][w] = none ? 0u : kept;
+                        }
+                }
+            }
+        }
+        if constexpr (CODES) {
+            float largest = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) largest = fmaxf(largest, fabsf(val_scale[i / 4][i % 4]));
+            if (__any(largest > val_most)) {
+                // the power of two above the largest scale
+                largest = wave_max_f(largest);
+                const int to = ((__float_as_int(largest) >> 23) & 0xff) - 126;
+                settle(acc);
+#pragma unroll
+                for (int i = 0; i < NC; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[i][r] = ldexpf(acc[i][r], val_up - to);
+                val_up = to;
+                val_most = ldexpf(1.0f, to);
+            }
+        }
+        // weights as planes: word w holds keys 2w and 2w + 1 of the lane's eight
+        v4u weight[K::pp];
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            v2f v = {x[2 * w], x[2 * w + 1]};
+            if constexpr (CODES) {
+                v[0] *= ldexpf(val_scale[w / 2][2 * w % 4], -val_up);
+                v[1] *= ldexpf(val_scale[w / 2][2 * w % 4 + 1], -val_up);
+            }
+#pragma unroll
+            for (int pl = 0; pl < K::pp; pl++) weight[pl][w] = plane(E(), v);
+        }
+        // the lane's keys of column i, in the weights' order
+        auto column = [&](int i, int h) {
+            v4u o;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                if constexpr (CODES)
+                    o[w] = codes_f16(__builtin_amdgcn_perm(val[2 * w + 1][h][i / 4] ^ 0x80808080u, val[2 * w][h][i / 4] ^ 0x80808080u,
+                                                           0x0c040c00u + 0x00010001u * (i % 4)));
+                else
+                    o[w] = __builtin_amdgcn_perm(val[2 * w + 1][h][i / 2], val[2 * w][h][i / 2], i % 2 ? 0x07060302u : 0x05040100u);
+            }
+            return o;
+        };
+#pragma unroll
+        for (int h = 0; h < G::H; h++)
+#pragma unroll
+            for (int i = 0; i < DV; i++) {
+                const v4u o = column(i, h);
+#pragma unroll
+                for (int pl = 0; pl < K::pp; pl++) acc[h * DV + i] = product(E(), o, weight[pl], acc[h * DV + i]);
+            }
+        if (more) fetch_values(next);
+    }
+    settle(acc);
+    l = far_sum(l);
+    // what was not finite, to the rows that see it
+    if (__any(odd)) {
+        for (int j = max(lo, 0); j < hi; j++) {
+            if (j / kKeyTile < split * parts.per || (j / kKeyTile - split * parts.per) % kw_all != kw || j / kKeyTile >= end) continue;
+            const int number = table[j >> shift];
+            if (j >= mine || (uint32_t)number >= (uint32_t)c.n_pages) continue;
+            const int64_t at = ((int64_t)number * c.n_kv_heads + kv) * c.page + (j & (c.page - 1));
+            const C *from = static_cast<const C *>(c.v) + at * dim;
+#pragma unroll
+            for (int h = 0; h < G::H; h++)
+#pragma unroll
+                for (int i = 0; i < DV; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int d = 16 * DV * h + DV * (4 * g + r) + i;
+                        float v = 0.0f;
+                        if constexpr (CODES) v = c.v_scale[at];
+                        else if (d < dim) v = (float)from[d];
+                        if (!(fabsf(v) <= 3.4028235e38f)) acc[h * DV + i][r] += v;
+                    }
+        }
+    }
+
+    // the waves of the same rows joined: each scales its sums to the maximum of all
+    if (g == 0) {
+        stat[wave][0][n] = m;
+        stat[wave][1][n] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY, total = 0.0f;
+    for (int w = 0; w < kw_all; w++) top = fmaxf(top, stat[w * p.row_waves + rw][0][n]);
+    const float base = top > -INFINITY ? top : 0.0f;
+    for (int w = 0; w < kw_all; w++) total += exp2_of(stat[w * p.row_waves + rw][0][n] - base) * stat[w * p.row_waves + rw][1][n];
+    const float f = total != 0.0f ? exp2_of(m - base) / total : 0.0f;
+    const bool alone = parts.used <= 1;
+    if (kw == 0 && g == 0 && row0 + n < rows) {
+        const int64_t out = ((int64_t)seq * a.n_new + row / group) * a.n_q_heads + kv * group + row % group;
+        const float log2_sum = base + (log2f(total) - kLift);
+        if (!alone) p.part_lse[out * p.splits + split] = log2_sum;
+        else if (a.lse) a.lse[out] = log2_sum * 0.6931471805599453f;
+    }
+#pragma unroll
+    for (int h = 0; h < G::H; h++) {
+        if (h) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < DV; i += 4)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                v4f v;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    v[k] = acc[h * DV + i + k][r] * f;
+                    if constexpr (CODES) v[k] = ldexpf(v[k], val_up + kCodeShift);
+                }
+                outs[wave][n][(DV * (4 * g + r) + i) / 4] = v;
+            }
+        __syncthreads();
+        for (int at = threadIdx.x; at < p.row_waves * 16 * 4 * DV; at += 256) {
+            const int quad = at % (4 * DV), r = at / (4 * DV) % 16, tile = at / (4 * DV * 16);
+            const int d = 16 * DV * h + 4 * quad, of = (blockIdx.z * p.row_waves + tile) * 16 + r;
+            if (of >= rows || d >= dim) continue;
+            v4f v = outs[tile][r][quad];
+            for (int w = 1; w < kw_all; w++) v += outs[w * p.row_waves + tile][r][quad];
+            const int64_t out = ((int64_t)seq * a.n_new + of / group) * a.n_q_heads + kv * group + of % group;
+            if (alone) {
+                T o[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) o[k] = (T)v[k];
+                T *to = static_cast<T *>(a.out) + out * dim + d;
+#pragma unroll
+                for (int k = 0; k < 4; k++) to[k] = o[k];
+            } else {
+                *reinterpret_cast<v4f *>(p.part_out + (out * p.splits + split) * dim + d) = v;
+            }
+        }
+    }
+}
+
+template <typename T, typename C, int DP>
+void launch_attn_dim(const AttnCall &p, hipStream_t s) {
+    const dim3 grid(p.a.n_seq * p.splits, p.c.n_kv_heads, p.row_blocks);
+    if (p.c.head_dim == DP) attn_tile_kernel<T, C, DP, true><<<grid, 256, 0, s>>>(p);
+    else attn_tile_kernel<T, C, DP, false><<<grid, 256, 0, s>>>(p);
+}
+template <typename T, typename C>
+hipError_t launch_attn_typed(const AttnCall &p, hipStream_t s) {
+    if (p.c.head_dim <= 64) launch_attn_dim<T, C, 64>(p, s);
+    else if (p.c.head_dim <= 128) launch_attn_dim<T, C, 128>(p, s);
+    else launch_attn_dim<T, C, 256>(p, s);
+    return hipGetLastError();
+}
+template <typename C>
+hipError_t launch_attn_cache(const AttnCall &p, hipStream_t s) {
+    if (p.a.type == HOARD_TYPE_F32) return launch_attn_typed<float, C>(p, s);
+    if (p.a.type == HOARD_TYPE_F16) return launch_attn_typed<f16, C>(p, s);
+    return launch_attn_typed<bf16, C>(p, s);
+}
+
+}  // namespace hoard
