@@ -12,89 +12,111 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 // out = sum_s w_s part_s,  w_s = 2^(lse_s - m) / sum: the parts of one row, each already
 // divided by its own sum.  A workgroup takes a row: four columns a thread, the parts dealt
-// to the threads left over, which meet in LDS.
+// to the threads left over, which meet in LDS.  What a thread reads first it asks for before
+// the weights are known: the launch is latency alone.
+constexpr int kFetch = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall p) {
-    __shared__ float weight[kMaxSplits], stat[2][4];
+    __shared__ float weight[kRuns], stat[2][4];
     __shared__ v4f outs[256];
     const hoard_attn_args &a = p.a;
-    const int64_t token = blockIdx.x, row = token * a.n_q_heads + blockIdx.y, seq = token / a.n_new;
+    const int token = blockIdx.x, head = blockIdx.y, seq = token / a.n_new, group = a.n_q_heads / p.c.n_kv_heads;
+    const int row = token % a.n_new * group + head % group, block = row / p.block_rows;
+    const int lanes = p.c.n_kv_heads * p.row_blocks, of = head / group * p.row_blocks + block;
+    const AttnPlace place = attn_place(p, seq);
+    // the lane's tiles, and the workgroups whose runs they fall in
+    const int tiles = attn_tiles(place.keys), begin = place.first + of * tiles;
+    const int from_run = begin / place.run, parts = (begin + tiles - 1) / place.run - from_run + 1;
+    if (parts == 1) return;
     const int lane = threadIdx.x & 63, dim = p.c.head_dim;
-    const int limit = a.max_pages * p.c.page;
-    int most = 0;
-    for (int t = 0; t < a.n_new; t++) most = max(most, min(max(a.lens[seq * a.n_new + t], 0), limit));
-    const AttnParts parts = attn_parts(most, p.splits, 4 / p.row_waves);
-    if (parts.used <= 1) return;
-    const float *lse = p.part_lse + row * p.splits;
-    const float mine = (int)threadIdx.x < parts.used ? lse[threadIdx.x] : -INFINITY;
-    // a NaN of one part is everyone's
+    const int64_t first = ((int64_t)from_run + (int64_t)seq * lanes + of) * p.block_rows + row % p.block_rows;
+    const int step = p.block_rows;
+    const float mine = (int)threadIdx.x < parts ? p.part_lse[first + (int)threadIdx.x * step] : -INFINITY;
+    const int quads = dim / 4, deep = 256 / quads, quad = threadIdx.x % quads, from = threadIdx.x / quads;
+    const float *part = p.part_out + first * dim + 4 * quad;
+    v4f ahead[kFetch];
+#pragma unroll
+    for (int i = 0; i < kFetch; i++)
+        ahead[i] = *reinterpret_cast<const v4f *>(part + (int64_t)min(from + i * deep, parts - 1) * step * dim);
     const float top = wave_max_f(mine);
     if (lane == 0) stat[0][wave_index()] = top;
     __syncthreads();
     float m = fmaxf(fmaxf(stat[0][0], stat[0][1]), fmaxf(stat[0][2], stat[0][3]));
     m = m > -INFINITY ? m : 0.0f;
-    const float w = exp2f(mine - m), s = wave_sum_f(w);
+    const float w = exp2f(mine - m), s = wave_sum_f(w);  // a NaN is everyone's
     if (lane == 0) stat[1][wave_index()] = s;
-    if ((int)threadIdx.x < kMaxSplits) weight[threadIdx.x] = w;
+    weight[threadIdx.x] = w;
     __syncthreads();
     const float sum = (stat[1][0] + stat[1][1]) + (stat[1][2] + stat[1][3]), f = sum != 0.0f ? 1.0f / sum : 0.0f;
-    const int quads = dim / 4, deep = 256 / quads, quad = threadIdx.x % quads, from = threadIdx.x / quads;
     v4f o = {0, 0, 0, 0};
     if (from < deep) {
-        const float *part = p.part_out + row * p.splits * dim + 4 * quad;
+#pragma unroll
+        for (int i = 0; i < kFetch; i++)
+            if (from + i * deep < parts) o += weight[from + i * deep] * ahead[i];
 #pragma unroll 4
-        for (int i = from; i < parts.used; i += deep) {
-            const float wi = weight[i];
-            // a part of which the row sees nothing holds zeros
-            o += wi * *reinterpret_cast<const v4f *>(part + (int64_t)i * dim);
-        }
+        for (int i = from + kFetch * deep; i < parts; i += deep)
+            o += weight[i] * *reinterpret_cast<const v4f *>(part + (int64_t)i * step * dim);
     }
     outs[threadIdx.x] = o;
     __syncthreads();
+    const int64_t out = (int64_t)token * a.n_q_heads + head;
     if (from == 0) {
         for (int i = 1; i < deep; i++) o += outs[i * quads + quad];
-        T *to = static_cast<T *>(a.out) + row * dim + 4 * quad;
+        T *to = static_cast<T *>(a.out) + out * dim + 4 * quad;
 #pragma unroll
         for (int k = 0; k < 4; k++) to[k] = (T)(o[k] * f);
     }
-    if (threadIdx.x == 0 && a.lse) a.lse[row] = (m + log2f(sum)) * 0.6931471805599453f;
+    if (threadIdx.x == 0 && a.lse) a.lse[out] = (m + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Waves side by side over the rows where there are more than 16; workgroups for about two
-// a CU, a sequence split into as many parts as that leaves.
+// Waves side by side over the rows where there are more than 16.
 AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work) {
     AttnCall p{};
     p.c = c;
     p.a = a;
     const int rows = a.n_new * (a.n_q_heads / c.n_kv_heads), tiles = (rows + 15) / 16;
-    p.row_waves = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
+    p.row_waves = tiles >= 3 ? 4 : tiles;
     p.row_blocks = (tiles + p.row_waves - 1) / p.row_waves;
-    const int64_t groups = (int64_t)a.n_seq * c.n_kv_heads * p.row_blocks;
-    const int64_t keys = (int64_t)a.max_pages * c.page, deep = 4 / p.row_waves;
-    const int64_t most = (keys + kKeyTile * deep - 1) / (kKeyTile * deep);
-    int64_t splits = groups ? kAttnGroups / groups : 1;
-    splits = splits > most ? most : splits;
-    p.splits = (int)(splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits);
-    const int64_t all = (int64_t)a.n_seq * a.n_new * a.n_q_heads * p.splits;
-    p.part_out = work;
-    p.part_lse = work ? work + all * c.head_dim : nullptr;
+    p.block_rows = rows < 16 * p.row_waves ? rows : 16 * p.row_waves;
+    // cut where the lanes alone would leave the chip half empty or uneven, and there is something
+    // to cut; the row of tiles is counted in 32 bits
+    const int64_t tiles_most = ((int64_t)a.max_pages * c.page + kKeyTile - 1) / kKeyTile;
+    p.split = attn_lanes(p) < 2 * kRuns && a.n_seq <= kMaxSplitSeqs && tiles_most > 32 && attn_lanes(p) * tiles_most < INT32_MAX;
+    if (p.split) {
+        p.part_out = work;
+        p.part_lse = work ? work + attn_parts(p) * p.block_rows * c.head_dim : nullptr;
+    }
     return p;
 }
+
+constexpr int64_t kMaxGrid = 1 << 23;
 
 }  // namespace
 
 size_t attn_work_bytes(const hoard_kv_cache &c, const hoard_attn_args &a) {
     const AttnCall p = call_of(c, a, nullptr);
-    if (p.splits == 1) return 0;
-    return sizeof(float) * (size_t)(c.head_dim + 1) * a.n_seq * a.n_new * a.n_q_heads * p.splits;
+    return p.split ? sizeof(float) * (size_t)(c.head_dim + 1) * attn_parts(p) * p.block_rows : 0;
 }
 
 hipError_t launch_attn(const hoard_kv_cache &c, const hoard_attn_args &a, float *work, hipStream_t s) {
-    const AttnCall p = call_of(c, a, work);
-    const hipError_t rc = c.type == HOARD_TYPE_F16    ? launch_attn_f16(p, s)
-                          : c.type == HOARD_TYPE_BF16 ? launch_attn_bf16(p, s)
-                                                      : launch_attn_i8(p, s);
-    if (rc != hipSuccess || p.splits == 1) return rc;
+    AttnCall p = call_of(c, a, work);
+    // as many sequences at a time as a grid takes
+    const int64_t lanes = (int64_t)c.n_kv_heads * p.row_blocks, at_once = kMaxGrid / lanes > 1 ? kMaxGrid / lanes : 1;
+    const size_t z = a.type == HOARD_TYPE_F32 ? 4 : 2;
+    for (int64_t seq = 0; seq < a.n_seq; seq += at_once) {
+        const int64_t token = seq * a.n_new;
+        p.a.n_seq = (int)(a.n_seq - seq < at_once ? a.n_seq - seq : at_once);
+        p.a.q = static_cast<const char *>(a.q) + token * a.q_stride * z;
+        p.a.pages = a.pages + seq * a.max_pages;
+        p.a.lens = a.lens + token;
+        p.a.out = static_cast<char *>(a.out) + token * a.n_q_heads * c.head_dim * z;
+        p.a.lse = a.lse ? a.lse + token * a.n_q_heads : nullptr;
+        const hipError_t rc = c.type == HOARD_TYPE_F16    ? launch_attn_f16(p, s)
+                              : c.type == HOARD_TYPE_BF16 ? launch_attn_bf16(p, s)
+                                                          : launch_attn_i8(p, s);
+        if (rc != hipSuccess) return rc;
+    }
+    if (!p.split) return hipSuccess;
     const dim3 grid(a.n_seq * a.n_new, a.n_q_heads);
     if (a.type == HOARD_TYPE_F32) attn_join_kernel<float><<<grid, 256, 0, s>>>(p);
     else if (a.type == HOARD_TYPE_F16) attn_join_kernel<f16><<<grid, 256, 0, s>>>(p);

@@ -1,41 +1,123 @@
 // How the attention over a cache is split over its length: shared by the kernel of the
 // tiles, that of the join and the host.
+//
+// A lane of work is one sequence's for one key head and block of rows: its tiles of 32 keys,
+// at least one (a row that sees nothing has its zeros to write).  Where there are fewer lanes
+// than keep the chip busy and level, the tiles of all of them are one row, as the lengths
+// are found on the device, and every workgroup takes an equal run of it: the end of one lane,
+// some whole ones, the beginning of another.  A lane that no run holds whole goes to the
+// workspace in its parts, and a second launch joins them.  The parts in the order of the row are
+// numbered by workgroup + lane, as one of the two grows from each to the next.
+//
+// Equal runs, as one compute unit reads no more than twice its share of the memory's rate:
+// with whole lanes cut into up to four parts each, 64 sequences of 512 to 8192 tokens took
+// 69 us (a workgroup for each part, 65 to 69 with other sizes) against 49 for as many tokens
+// in equal sequences.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
 #include "attn.h"
+#include "wave.h"
 
 namespace hoard {
+
+constexpr int kKeyTile = 32;
+constexpr int kRuns = 256;     // a workgroup a CU
+constexpr int kMinRun = 8;     // tiles of a run: one a wave
+constexpr int kMaxSplitSeqs = 256;
+
+// Waves of the tiles' workgroup: two a SIMD where their registers leave room.
+constexpr int attn_waves(int dim) { return dim > 128 ? 4 : 8; }
 
 struct AttnCall {
     hoard_kv_cache c;
     hoard_attn_args a;
-    int splits;      // parts that a sequence may be split into, at most
+    int split;       // whether lanes may be cut
     int row_waves;   // 1, 2 or 4: waves of a workgroup side by side over the rows
     int row_blocks;  // workgroups over the rows
-    float *part_out, *part_lse;  // [rows][splits][head_dim] and [rows][splits], with splits > 1
+    int block_rows;  // rows of a workgroup
+    float *part_out, *part_lse;  // [parts][block_rows][head_dim] and [parts][block_rows], with split
 };
 
-constexpr int kKeyTile = 32;
-constexpr int kMaxSplits = 256;
-constexpr int kAttnGroups = 512;
+// The keys that each new token of a sequence sees, a lane each, and the most of them.
+__device__ __forceinline__ int attn_seen(const hoard_attn_args &a, int limit, int seq) {
+    const int lane = threadIdx.x & 63;
+    return lane < a.n_new ? min(max(a.lens[(int64_t)seq * a.n_new + lane], 0), limit) : 0;
+}
+__device__ __forceinline__ int attn_most(int v) {
+    v = max(v, dpp_i<kDppQuadXor1>(v));
+    v = max(v, dpp_i<kDppQuadXor2>(v));
+    v = max(v, dpp_i<kDppRowHalfMirror>(v));
+    v = max(v, dpp_i<kDppRowMirror>(v));
+    return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+// The running sum over the wave's lanes: within rows of 16, then the rows before.
+__device__ __forceinline__ int attn_running(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, kDppRowBcast15, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, kDppRowBcast31, 0xc, 0xf, false);
+    return v;
+}
+// A lane's tiles.
+__device__ __forceinline__ int attn_tiles(int keys) {
+    return max((int)(((uint32_t)keys + kKeyTile - 1) / kKeyTile), 1);
+}
 
-// The parts of a sequence of which `keys` keys are seen: as many as there may be, but of a
-// tile a wave at least.
-struct AttnParts {
-    int tiles, per, used;
+// Where in the row of tiles a sequence lies: its keys, its first tile and what a run holds.
+struct AttnPlace {
+    int seq, keys, first, run, total;
 };
-__device__ __forceinline__ AttnParts attn_parts(int keys, int splits, int waves) {
-    AttnParts p;
-    p.tiles = (keys + kKeyTile - 1) / kKeyTile;
-    p.per = max((p.tiles + splits - 1) / splits, waves);
-    p.used = (p.tiles + p.per - 1) / p.per;
-    return p;
+// The sequence that holds tile (blockIdx.x * run) of the row, or with `seq` >= 0 that one; seq
+// -1 where the row is shorter.  By all lanes of a wave.
+__device__ __forceinline__ AttnPlace attn_place(const AttnCall &p, int seq) {
+    constexpr int STEPS = kMaxSplitSeqs / 64;
+    const hoard_attn_args &a = p.a;
+    const int limit = a.max_pages * p.c.page, lanes = p.c.n_kv_heads * p.row_blocks, lane = threadIdx.x & 63;
+    int keys[STEPS], sums[STEPS], before = 0;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        keys[i] = 0;
+        if (i * 64 + lane < a.n_seq) {
+            const int32_t *lens = a.lens + (int64_t)(i * 64 + lane) * a.n_new;
+#pragma unroll 4
+            for (int t = 0; t < a.n_new; t++) keys[i] = max(keys[i], lens[t]);
+            keys[i] = min(keys[i], limit);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        sums[i] = before;
+        if (i * 64 >= a.n_seq) continue;
+        // of this sequence and those before it
+        sums[i] += attn_running(i * 64 + lane < a.n_seq ? attn_tiles(keys[i]) * lanes : 0);
+        before = __builtin_amdgcn_readlane(sums[i], 63);
+    }
+    AttnPlace r{-1, 0, 0, 0, before};
+    r.run = max((r.total + kRuns - 1) / kRuns, kMinRun);
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        if (i * 64 >= a.n_seq || r.seq >= 0) continue;
+        const int at = seq >= 0 ? seq - i * 64 : __popcll(__ballot(sums[i] <= (int)blockIdx.x * r.run));
+        if (at >= 64 || i * 64 + at >= a.n_seq) continue;
+        r.seq = i * 64 + at;
+        r.keys = __builtin_amdgcn_readlane(keys[i], at);
+        r.first = __builtin_amdgcn_readlane(sums[i], at) - attn_tiles(r.keys) * lanes;
+    }
+    return r;
 }
 
 hipError_t launch_attn_f16(const AttnCall &p, hipStream_t s);
 hipError_t launch_attn_bf16(const AttnCall &p, hipStream_t s);
 hipError_t launch_attn_i8(const AttnCall &p, hipStream_t s);
+
+// Lanes of work, workgroups of the tiles' kernel, and parts in the workspace.
+inline int64_t attn_lanes(const AttnCall &p) { return (int64_t)p.a.n_seq * p.c.n_kv_heads * p.row_blocks; }
+inline int attn_grid(const AttnCall &p) { return p.split ? kRuns : (int)attn_lanes(p); }
+inline int64_t attn_parts(const AttnCall &p) { return p.split ? kRuns + attn_lanes(p) : 0; }
 
 }  // namespace hoard

@@ -26,6 +26,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "attn.h"
 #include "attn_split.h"
 #include "opsdev.h"
@@ -134,14 +136,16 @@ struct Shape {
     static constexpr int KL = DP * (int)sizeof(C) / 64;      // pieces of a key
     static constexpr int VW = DV * (int)sizeof(C) / 4;       // words of a piece of a value
     typedef uint32_t piece __attribute__((ext_vector_type(VW)));
+    static constexpr int NW = attn_waves(DP);                // waves of a workgroup
 };
 
 }  // namespace attn
 
-// One workgroup: 4 waves, `row_waves` wide over the rows and 4 / row_waves deep over the
-// keys of part blockIdx.x % splits of sequence blockIdx.x / splits.
+// The tiles first .. last - 1 of a lane of work by one workgroup: NW waves, `row_waves` wide
+// over the rows and NW / row_waves deep over the tiles.  part: where the result goes in the
+// workspace, or -1 for a lane that is whole.
 template <typename T, typename C, int DP, bool WHOLE>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCall p) {
+__device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_no, int seen, int keys, int first, int last, int64_t part) {
     using namespace attn;
     typedef Shape<C, DP> G;
     typedef Core<T, C> K;
@@ -150,81 +154,44 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCa
     constexpr int DV = G::DV, NC = G::NC, STEPS = G::STEPS;
     // f16 weights reach from 2^15 down
     constexpr float kLift = HALF ? 15.0f : 0.0f;
-    __shared__ float stat[4][2][16];
-    __shared__ v4f outs[4][16][16 * DV / 4 + 1];
+    __shared__ float stat[G::NW][2][16];
+    __shared__ v4f outs[G::NW][16][16 * DV / 4 + 1];
 
     const hoard_kv_cache &c = p.c;
     const hoard_attn_args &a = p.a;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wave = wave_index();
-    const int seq = blockIdx.x / p.splits, split = blockIdx.x % p.splits, kv = blockIdx.y;
+    const int kv = lane_no / p.row_blocks, block = lane_no % p.row_blocks;
     const int group = a.n_q_heads / c.n_kv_heads, rows = a.n_new * group, dim = WHOLE ? DP : c.head_dim;
-    const int rw = wave % p.row_waves, kw = wave / p.row_waves, kw_all = 4 / p.row_waves;
-    const int row0 = (blockIdx.z * p.row_waves + rw) * 16, row = min(row0 + n, rows - 1);
+    const int rw = wave % p.row_waves, kw = wave / p.row_waves, kw_all = G::NW / p.row_waves;
+    const int row0 = (block * p.row_waves + rw) * 16, row = min(row0 + n, rows - 1);
 
-    // the keys that each new token sees, most of all, and most and fewest of the wave's rows
-    const int limit = a.max_pages * c.page;
-    const int seen = lane < a.n_new ? min(max(a.lens[(int64_t)seq * a.n_new + lane], 0), limit) : 0;
-    int most = row16_max_i(seen);
-    most = max(max(__builtin_amdgcn_readlane(most, 0), __builtin_amdgcn_readlane(most, 16)),
-               max(__builtin_amdgcn_readlane(most, 32), __builtin_amdgcn_readlane(most, 48)));
-    const int mine = __shfl(seen, row / group);
-    const int hi = row0 < rows ? __builtin_amdgcn_readfirstlane(row16_max_i(mine)) : 0;
-    const int lo = -__builtin_amdgcn_readfirstlane(row16_max_i(-mine));
-
-    const AttnParts parts = attn_parts(most, p.splits, kw_all);
-    if (split && split >= parts.used) return;
-    const int end = min(min((split + 1) * parts.per, parts.tiles), (hi + kKeyTile - 1) / kKeyTile);
-    int ti = split * parts.per + kw;
-
-    // queries, as planes: the k-th values of a product's step are those that the keys' pieces hold
-    v4u q[K::qp][STEPS];
-    int up = 0;  // q is held times 2^up
+    // page numbers of 64 pages from page0 on, a lane each
+    const int shift = 31 - __builtin_clz(c.page), last_page = (max(keys, 1) - 1) >> shift;
+    const int32_t *table = a.pages + (int64_t)seq * a.max_pages;
+    int ti = first + kw, page0 = (min(ti, last - 1) * kKeyTile) >> shift, numbers = -1;
+    if (keys) numbers = table[min(page0 + lane, a.max_pages - 1)];
+    // the queries, asked for before the first keys and used behind them
+    Raw<T> q_raw[STEPS];
     {
         const T *from = static_cast<const T *>(a.q) + ((int64_t)seq * a.n_new + row / group) * a.q_stride +
                         (kv * group + row % group) * dim;
-        float x[STEPS][8];
-        int top = 0;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
             const int d = CODES ? (s / 2) * 64 + 16 * g + (s % 2) * 8 : s * 32 + 8 * g;
-            widen(fetch(from, Cols{d < dim ? d : 0, 0}, dim), x[s]);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                x[s][i] = d < dim && row0 + n < rows ? x[s][i] : 0.0f;
-                top = max(top, __float_as_int(x[s][i]) & 0x7fffffff);
-            }
+            q_raw[s] = fetch(from, Cols{d < dim ? d : 0, 0}, dim);
         }
-        if constexpr (SCALED) {
-            auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-            top = max((int)r[0], (int)r[1]);
-            r = __builtin_amdgcn_permlane16_swap(top, top, false, false);
-            top = max((int)r[0], (int)r[1]);
-            up = top ? 14 + 127 - (top >> 23) : 0;
-        }
-#pragma unroll
-        for (int s = 0; s < STEPS; s++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                v2f v = {x[s][2 * i], x[s][2 * i + 1]};
-                if constexpr (SCALED) v = v2f{ldexpf(v[0], up), ldexpf(v[1], up)};
-#pragma unroll
-                for (int pl = 0; pl < K::qp; pl++) q[pl][s][i] = plane(E(), v);
-            }
     }
-    const float to_log2 = a.scale * 1.4426950408889634f;
-    const int down = (CODES ? kCodeShift : 0) - up;
-
-    // page numbers of 64 pages from `page0` on, a lane each
-    const int shift = 31 - __builtin_clz(c.page), last_page = (max(most, 1) - 1) >> shift;
-    const int32_t *table = a.pages + (int64_t)seq * a.max_pages;
-    int page0 = 0, numbers = 0;
+    asm volatile("" : "+v"(numbers));
     struct Where {
         int64_t at[2];  // the cache's rows of the tile's halves
         bool ok[2];
     };
     auto fill = [&](int from) {
         page0 = from;
-        numbers = table[min(from + lane, last_page)];
+        numbers = table[min(from + lane, a.max_pages - 1)];
+        // waited for here, once in 64 pages: where the numbers are used the wait would be for
+        // the keys and values in flight as well
+        asm volatile("" : "+v"(numbers));
     };
     auto where = [&](int tile) {
         Where w;
@@ -276,17 +243,59 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCa
     int val_up = 0;  // acc is held times 2^-val_up
     float val_most = 0.0f;
     bool odd = false;
-    Where cur{}, next{};
-    if (ti < end) {
-        fill((ti * kKeyTile) >> shift);
-        cur = where(ti);
-        fetch_keys(cur);
-        fetch_values(cur);
+    // without a condition (a wave without a tile fetches the last one, a lane without keys the
+    // cache's first page), so that the queries' wait is not for these as well
+    Where cur = where(min(ti, last - 1)), next{};
+    fetch_keys(cur);
+    fetch_values(cur);
+
+    // the keys that the wave's rows see: each its own, the most and the fewest
+    const int mine = __shfl(seen, row / group);
+    const int hi = row0 < rows ? __builtin_amdgcn_readfirstlane(row16_max_i(mine)) : 0;
+    const int lo = -__builtin_amdgcn_readfirstlane(row16_max_i(-mine));
+    const int end = min(last, (int)(((uint32_t)hi + kKeyTile - 1) / kKeyTile));
+
+    // queries, as planes: the k-th values of a product's step are those that the keys' pieces hold
+    v4u q[K::qp][STEPS];
+    int up = 0;  // q is held times 2^up
+    {
+        float x[STEPS][8];
+        int top = 0;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const int d = CODES ? (s / 2) * 64 + 16 * g + (s % 2) * 8 : s * 32 + 8 * g;
+            widen(q_raw[s], x[s]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[s][i] = d < dim && row0 + n < rows ? x[s][i] : 0.0f;
+                top = max(top, __float_as_int(x[s][i]) & 0x7fffffff);
+            }
+        }
+        if constexpr (SCALED) {
+            auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            top = max((int)r[0], (int)r[1]);
+            r = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+            top = max((int)r[0], (int)r[1]);
+            up = top ? 14 + 127 - (top >> 23) : 0;
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v2f v = {x[s][2 * i], x[s][2 * i + 1]};
+                if constexpr (SCALED) v = v2f{ldexpf(v[0], up), ldexpf(v[1], up)};
+#pragma unroll
+                for (int pl = 0; pl < K::qp; pl++) q[pl][s][i] = plane(E(), v);
+            }
     }
-    for (; ti < end; ti += kw_all, cur = next) {
+    const float to_log2 = a.scale * 1.4426950408889634f;
+    const int down = (CODES ? kCodeShift : 0) - up;
+
+    // The last tile is a copy of the loop without fetches: under a condition the compiler
+    // could not count them, and would wait for all.
+    auto step = [&](auto more) {
         const bool full = (ti + 1) * kKeyTile <= lo && cur.ok[0] && cur.ok[1];
-        const bool more = ti + kw_all < end;
-        if (more) next = where(ti + kw_all);
+        if constexpr (more.value) next = where(ti + kw_all);
 
         if constexpr (!WHOLE) {
 #pragma unroll
@@ -318,7 +327,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCa
             if constexpr (CODES) x[i] *= key_scale[i / 4][i % 4];
             if constexpr (CODES || SCALED) x[i] = ldexpf(x[i], down);
         }
-        if (more) fetch_keys(next);
+        if constexpr (more.value) fetch_keys(next);
         if (!full) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -344,27 +353,42 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCa
         // does not see the key, those that are not finite: zero times them is not zero.  The
         // rows that do see them get them after the loop.
         if (!full) {
-            constexpr uint32_t exponent = HALF ? 0x7c00u : 0x7f80u;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const int j = ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4;
-                const bool none = j >= hi || !cur.ok[i / 4];
-                if constexpr (CODES) {
-                    const float scale = val_scale[i / 4][i % 4];
-                    const bool bad = j >= lo && !(fabsf(scale) <= 3.4028235e38f);
-                    odd |= bad && !none;
-                    val_scale[i / 4][i % 4] = none || bad ? 0.0f : scale;
-                } else {
+                const bool none = ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4 >= hi || !cur.ok[i / 4];
+                if constexpr (CODES) val_scale[i / 4][i % 4] = none ? 0.0f : val_scale[i / 4][i % 4];
+                else
 #pragma unroll
-                    for (int h = 0; h < G::H; h++)
+                    for (int h = 0; h < G::H; h++) val[i][h] = none ? typename G::piece{} : val[i][h];
+            }
+            if (lo < hi && (ti + 1) * kKeyTile > lo) {
+                // an exponent of ones carries into the sign's place
+                constexpr uint32_t exponent = HALF ? 0x7c007c00u : 0x7f807f80u, one = HALF ? 0x04000400u : 0x00800080u;
+                uint32_t carried = 0;
 #pragma unroll
-                        for (int w = 0; w < G::VW; w++) {
-                            const uint32_t v = val[i][h][w];
-                            const bool low = (v & exponent) == exponent, high = (v >> 16 & exponent) == exponent;
-                            const uint32_t kept = j < lo ? v : v & (low ? 0xffff0000u : ~0u) & (high ? 0x0000ffffu : ~0u);
-                            odd |= kept != v && !none;
-                            val[i][h][w] = none ? 0u : kept;
-                        }
+                for (int i = 0; i < 8; i++) {
+                    if constexpr (CODES) carried |= fabsf(val_scale[i / 4][i % 4]) <= 3.4028235e38f ? 0u : 0x80008000u;
+                    else
+#pragma unroll
+                        for (int h = 0; h < G::H; h++)
+#pragma unroll
+                            for (int w = 0; w < G::VW; w++) carried |= (val[i][h][w] & exponent) + one;
+                }
+                if (__any(carried & 0x80008000u)) {
+                    odd = true;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4 < lo) continue;
+                        if constexpr (CODES) val_scale[i / 4][i % 4] = fabsf(val_scale[i / 4][i % 4]) <= 3.4028235e38f ? val_scale[i / 4][i % 4] : 0.0f;
+                        else
+#pragma unroll
+                            for (int h = 0; h < G::H; h++)
+#pragma unroll
+                                for (int w = 0; w < G::VW; w++) {
+                                    const uint32_t bad = ((val[i][h][w] & exponent) + one) & 0x80008000u;
+                                    val[i][h][w] &= (bad & 0x8000u ? 0u : 0xffffu) | (bad >> 31 ? 0u : 0xffff0000u);
+                                }
+                    }
                 }
             }
         }
@@ -418,14 +442,16 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCa
 #pragma unroll
                 for (int pl = 0; pl < K::pp; pl++) acc[h * DV + i] = product(E(), o, weight[pl], acc[h * DV + i]);
             }
-        if (more) fetch_values(next);
-    }
+        if constexpr (more.value) fetch_values(next);
+    };
+    for (; ti + kw_all < end; ti += kw_all, cur = next) step(std::true_type{});
+    if (ti < end) step(std::false_type{});
     settle(acc);
     l = far_sum(l);
     // what was not finite, to the rows that see it
-    if (__any(odd)) {
+    if (odd) {
         for (int j = max(lo, 0); j < hi; j++) {
-            if (j / kKeyTile < split * parts.per || (j / kKeyTile - split * parts.per) % kw_all != kw || j / kKeyTile >= end) continue;
+            if (j / kKeyTile < first || (j / kKeyTile - first) % kw_all != kw || j / kKeyTile >= end) continue;
             const int number = table[j >> shift];
             if (j >= mine || (uint32_t)number >= (uint32_t)c.n_pages) continue;
             const int64_t at = ((int64_t)number * c.n_kv_heads + kv) * c.page + (j & (c.page - 1));
@@ -456,11 +482,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCa
     const float base = top > -INFINITY ? top : 0.0f;
     for (int w = 0; w < kw_all; w++) total += exp2_of(stat[w * p.row_waves + rw][0][n] - base) * stat[w * p.row_waves + rw][1][n];
     const float f = total != 0.0f ? exp2_of(m - base) / total : 0.0f;
-    const bool alone = parts.used <= 1;
     if (kw == 0 && g == 0 && row0 + n < rows) {
         const int64_t out = ((int64_t)seq * a.n_new + row / group) * a.n_q_heads + kv * group + row % group;
         const float log2_sum = base + (log2f(total) - kLift);
-        if (!alone) p.part_lse[out * p.splits + split] = log2_sum;
+        if (part >= 0) p.part_lse[part * p.block_rows + rw * 16 + n] = log2_sum;
         else if (a.lse) a.lse[out] = log2_sum * 0.6931471805599453f;
     }
 #pragma unroll
@@ -479,14 +504,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCa
                 outs[wave][n][(DV * (4 * g + r) + i) / 4] = v;
             }
         __syncthreads();
-        for (int at = threadIdx.x; at < p.row_waves * 16 * 4 * DV; at += 256) {
+        for (int at = threadIdx.x; at < p.row_waves * 16 * 4 * DV; at += 64 * G::NW) {
             const int quad = at % (4 * DV), r = at / (4 * DV) % 16, tile = at / (4 * DV * 16);
-            const int d = 16 * DV * h + 4 * quad, of = (blockIdx.z * p.row_waves + tile) * 16 + r;
+            const int d = 16 * DV * h + 4 * quad, of = (block * p.row_waves + tile) * 16 + r;
             if (of >= rows || d >= dim) continue;
             v4f v = outs[tile][r][quad];
             for (int w = 1; w < kw_all; w++) v += outs[w * p.row_waves + tile][r][quad];
             const int64_t out = ((int64_t)seq * a.n_new + of / group) * a.n_q_heads + kv * group + of % group;
-            if (alone) {
+            if (part < 0) {
                 T o[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) o[k] = (T)v[k];
@@ -494,17 +519,48 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCa
 #pragma unroll
                 for (int k = 0; k < 4; k++) to[k] = o[k];
             } else {
-                *reinterpret_cast<v4f *>(p.part_out + (out * p.splits + split) * dim + d) = v;
+                *reinterpret_cast<v4f *>(p.part_out + (part * p.block_rows + tile * 16 + r) * dim + d) = v;
             }
         }
     }
 }
 
+template <typename T, typename C, int DP, bool WHOLE>
+__global__ __launch_bounds__(64 * attn_waves(DP), DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCall p) {
+    const int lanes = p.c.n_kv_heads * p.row_blocks, limit = p.a.max_pages * p.c.page;
+    if (!p.split) {
+        const int seq = blockIdx.x / lanes, seen = attn_seen(p.a, limit, seq), keys = attn_most(seen);
+        attn_part<T, C, DP, WHOLE>(p, seq, blockIdx.x % lanes, seen, keys, 0, attn_tiles(keys), -1);
+        return;
+    }
+    const AttnPlace place = attn_place(p, -1);
+    if (place.seq < 0) return;
+    int seq = place.seq, seen = attn_seen(p.a, limit, seq), tiles = attn_tiles(place.keys), keys = place.keys;
+    int left = min(place.run, place.total - (int)blockIdx.x * place.run);
+    int at = blockIdx.x * place.run - place.first, lane = at / tiles;
+    at -= lane * tiles;
+    while (true) {
+        const int last = min(tiles, at + left);
+        const bool whole = at == 0 && last == tiles;
+        attn_part<T, C, DP, WHOLE>(p, seq, lane, seen, keys, at, last, whole ? -1 : (int64_t)blockIdx.x + (int64_t)seq * lanes + lane);
+        left -= last - at;
+        if (left <= 0) return;
+        at = 0;
+        if (++lane == lanes) {
+            lane = 0;
+            seen = attn_seen(p.a, limit, ++seq);
+            keys = attn_most(seen);
+            tiles = attn_tiles(keys);
+        }
+        __syncthreads();  // the LDS of the part before
+    }
+}
+
 template <typename T, typename C, int DP>
 void launch_attn_dim(const AttnCall &p, hipStream_t s) {
-    const dim3 grid(p.a.n_seq * p.splits, p.c.n_kv_heads, p.row_blocks);
-    if (p.c.head_dim == DP) attn_tile_kernel<T, C, DP, true><<<grid, 256, 0, s>>>(p);
-    else attn_tile_kernel<T, C, DP, false><<<grid, 256, 0, s>>>(p);
+    const int grid = attn_grid(p);
+    if (p.c.head_dim == DP) attn_tile_kernel<T, C, DP, true><<<grid, 64 * attn_waves(DP), 0, s>>>(p);
+    else attn_tile_kernel<T, C, DP, false><<<grid, 64 * attn_waves(DP), 0, s>>>(p);
 }
 template <typename T, typename C>
 hipError_t launch_attn_typed(const AttnCall &p, hipStream_t s) {

@@ -128,8 +128,8 @@ int hoard_heads_workspace(const hoard_heads_args *a, size_t *bytes);
    where key j of the sequence is place j % page of page pages[s][j / page].  A row that
    sees no key (n <= 0) has out 0 and lse -infinity.  n beyond max_pages * page counts as
    that; a page number outside [0, n_pages) hides the keys of its page.  Keys and values
-   that a row does not see may hold anything; a page table's entries behind the last key
-   are not read.  Keys and values are used as the cache holds them, q and the weights
+   that a row does not see may hold anything, and so may a page table's entries behind
+   the last key.  Keys and values are used as the cache holds them, q and the weights
    with at least 16 bits for 16-bit activations and 22 for fp32 ones.  1 <= n_new <= 64,
    n_q_heads a multiple of the cache's n_kv_heads up to 1024, n_seq * n_new < 2^24.
    workspace: hoard_attn_workspace's bytes (possibly 0), 16-byte aligned, used by the
