@@ -23,13 +23,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall p) {
     const int token = blockIdx.x, head = blockIdx.y, seq = token / a.n_new, group = a.n_q_heads / p.c.n_kv_heads;
     const int row = token % a.n_new * group + head % group, block = row / p.block_rows;
     const int lanes = p.c.n_kv_heads * p.row_blocks, of = head / group * p.row_blocks + block;
-    const AttnPlace place = attn_place(p, seq);
     // the lane's tiles, and the workgroups whose runs they fall in
-    const int tiles = attn_tiles(place.keys), begin = place.first + of * tiles;
-    const int from_run = begin / place.run, parts = (begin + tiles - 1) / place.run - from_run + 1;
+    const int before = seq ? p.sums[seq - 1] : 0, run = p.sums[a.n_seq];
+    const int tiles = (p.sums[seq] - before) / lanes, begin = before + of * tiles;
+    const int from_run = begin / run, parts = (begin + tiles - 1) / run - from_run + 1;
     if (parts == 1) return;
     const int lane = threadIdx.x & 63, dim = p.c.head_dim;
-    const int64_t first = ((int64_t)from_run + (int64_t)seq * lanes + of) * p.block_rows + row % p.block_rows;
+    const int64_t first = (from_run + (attn_own(run) ? 0 : (int64_t)seq * lanes + of)) * p.block_rows + row % p.block_rows;
     const int step = p.block_rows;
     const float mine = (int)threadIdx.x < parts ? p.part_lse[first + (int)threadIdx.x * step] : -INFINITY;
     const int quads = dim / 4, deep = 256 / quads, quad = threadIdx.x % quads, from = threadIdx.x / quads;
@@ -69,6 +69,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall p) {
     if (threadIdx.x == 0 && a.lse) a.lse[out] = (m + log2f(sum)) * 0.6931471805599453f;
 }
 
+// Lanes of so many tiles are not cut: the join would take longer.
+constexpr int kWholeTiles = 16;
+
 // Waves side by side over the rows where there are more than 16.
 AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work) {
     AttnCall p{};
@@ -77,14 +80,16 @@ AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work)
     const int rows = a.n_new * (a.n_q_heads / c.n_kv_heads), tiles = (rows + 15) / 16;
     p.row_waves = tiles >= 3 ? 4 : tiles;
     p.row_blocks = (tiles + p.row_waves - 1) / p.row_waves;
+    p.min_run = attn_waves(c.head_dim) / p.row_waves;
     p.block_rows = rows < 16 * p.row_waves ? rows : 16 * p.row_waves;
     // cut where the lanes alone would leave the chip half empty or uneven, and there is something
     // to cut; the row of tiles is counted in 32 bits
     const int64_t tiles_most = ((int64_t)a.max_pages * c.page + kKeyTile - 1) / kKeyTile;
-    p.split = attn_lanes(p) < 2 * kRuns && a.n_seq <= kMaxSplitSeqs && tiles_most > 32 && attn_lanes(p) * tiles_most < INT32_MAX;
+    p.split = attn_lanes(p) < 2 * kRuns && a.n_seq <= kMaxSplitSeqs && tiles_most > kWholeTiles && attn_lanes(p) * tiles_most < INT32_MAX;
     if (p.split) {
         p.part_out = work;
         p.part_lse = work ? work + attn_parts(p) * p.block_rows * c.head_dim : nullptr;
+        p.sums = work ? reinterpret_cast<int32_t *>(p.part_lse + attn_parts(p) * p.block_rows) : nullptr;
     }
     return p;
 }
@@ -95,7 +100,7 @@ constexpr int64_t kMaxGrid = 1 << 23;
 
 size_t attn_work_bytes(const hoard_kv_cache &c, const hoard_attn_args &a) {
     const AttnCall p = call_of(c, a, nullptr);
-    return p.split ? sizeof(float) * (size_t)(c.head_dim + 1) * attn_parts(p) * p.block_rows : 0;
+    return p.split ? sizeof(float) * ((size_t)(c.head_dim + 1) * attn_parts(p) * p.block_rows + a.n_seq + 1) : 0;
 }
 
 hipError_t launch_attn(const hoard_kv_cache &c, const hoard_attn_args &a, float *work, hipStream_t s) {

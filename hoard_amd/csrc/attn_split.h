@@ -7,7 +7,10 @@
 // are found on the device, and every workgroup takes an equal run of it: the end of one lane,
 // some whole ones, the beginning of another.  A lane that no run holds whole goes to the
 // workspace in its parts, and a second launch joins them.  The parts in the order of the row are
-// numbered by workgroup + lane, as one of the two grows from each to the next.
+// numbered by workgroup + lane, as one of the two grows from each to the next.  Where the runs
+// are short a second part costs a workgroup more than an even share gains: there every lane
+// begins a run of its own, and the parts are numbered by workgroup (1025 tokens by 4 lanes: 13.3
+// us with runs over lanes, 2048 tokens 11.1).
 //
 // Equal runs, as one compute unit reads no more than twice its share of the memory's rate:
 // with whole lanes cut into up to four parts each, 64 sequences of 512 to 8192 tokens took
@@ -24,11 +27,11 @@ namespace hoard {
 
 constexpr int kKeyTile = 32;
 constexpr int kRuns = 256;     // a workgroup a CU
-constexpr int kMinRun = 8;     // tiles of a run: one a wave
+constexpr int kOwnRun = 16;    // shorter runs hold one lane's tiles only
 constexpr int kMaxSplitSeqs = 256;
 
 // Waves of the tiles' workgroup: two a SIMD where their registers leave room.
-constexpr int attn_waves(int dim) { return dim > 128 ? 4 : 8; }
+constexpr int attn_waves(int dim) { return 4; }
 
 struct AttnCall {
     hoard_kv_cache c;
@@ -37,7 +40,9 @@ struct AttnCall {
     int row_waves;   // 1, 2 or 4: waves of a workgroup side by side over the rows
     int row_blocks;  // workgroups over the rows
     int block_rows;  // rows of a workgroup
+    int min_run;     // tiles of a run, at least: one a wave
     float *part_out, *part_lse;  // [parts][block_rows][head_dim] and [parts][block_rows], with split
+    int32_t *sums;   // [n_seq + 1]: tiles of all lanes of the sequences up to each, a run's; with split
 };
 
 // The keys that each new token of a sequence sees, a lane each, and the most of them.
@@ -72,13 +77,18 @@ __device__ __forceinline__ int attn_tiles(int keys) {
 struct AttnPlace {
     int seq, keys, first, run, total;
 };
-// The sequence that holds tile (blockIdx.x * run) of the row, or with `seq` >= 0 that one; seq
-// -1 where the row is shorter.  By all lanes of a wave.
-__device__ __forceinline__ AttnPlace attn_place(const AttnCall &p, int seq) {
+// Whether runs of that length hold one lane's tiles only, and a lane's tiles then.
+__device__ __forceinline__ bool attn_own(int run) { return run < kOwnRun; }
+__device__ __forceinline__ int attn_row_tiles(int tiles, int run) {
+    return attn_own(run) ? (tiles + run - 1) / run * run : tiles;
+}
+// The sequence that holds tile (blockIdx.x * run) of the row; seq -1 where the row is shorter.  By
+// all lanes of a wave.  The first workgroup leaves the sums for the join.
+__device__ __forceinline__ AttnPlace attn_place(const AttnCall &p) {
     constexpr int STEPS = kMaxSplitSeqs / 64;
     const hoard_attn_args &a = p.a;
     const int limit = a.max_pages * p.c.page, lanes = p.c.n_kv_heads * p.row_blocks, lane = threadIdx.x & 63;
-    int keys[STEPS], sums[STEPS], before = 0;
+    int keys[STEPS], sums[STEPS], all = 0, before = 0;
 #pragma unroll
     for (int i = 0; i < STEPS; i++) {
         keys[i] = 0;
@@ -90,24 +100,35 @@ __device__ __forceinline__ AttnPlace attn_place(const AttnCall &p, int seq) {
         }
     }
 #pragma unroll
+    for (int i = 0; i < STEPS; i++)
+        if (i * 64 < a.n_seq)
+            all += __builtin_amdgcn_readlane(attn_running(i * 64 + lane < a.n_seq ? attn_tiles(keys[i]) : 0), 63);
+    AttnPlace r{-1, 0, 0, 0, 0};
+    r.run = max((all * lanes + kRuns - 1) / kRuns, p.min_run);
+#pragma unroll
     for (int i = 0; i < STEPS; i++) {
         sums[i] = before;
         if (i * 64 >= a.n_seq) continue;
         // of this sequence and those before it
-        sums[i] += attn_running(i * 64 + lane < a.n_seq ? attn_tiles(keys[i]) * lanes : 0);
+        sums[i] += attn_running(i * 64 + lane < a.n_seq ? attn_row_tiles(attn_tiles(keys[i]), r.run) * lanes : 0);
         before = __builtin_amdgcn_readlane(sums[i], 63);
+        if (blockIdx.x == 0 && threadIdx.x < 64 && i * 64 + lane < a.n_seq) p.sums[i * 64 + lane] = sums[i];
     }
-    AttnPlace r{-1, 0, 0, 0, before};
-    r.run = max((r.total + kRuns - 1) / kRuns, kMinRun);
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.sums[a.n_seq] = r.run;
+    r.total = before;
 #pragma unroll
     for (int i = 0; i < STEPS; i++) {
         if (i * 64 >= a.n_seq || r.seq >= 0) continue;
-        const int at = seq >= 0 ? seq - i * 64 : __popcll(__ballot(sums[i] <= (int)blockIdx.x * r.run));
+        const int at = __popcll(__ballot(sums[i] <= (int)blockIdx.x * r.run));
         if (at >= 64 || i * 64 + at >= a.n_seq) continue;
         r.seq = i * 64 + at;
         r.keys = __builtin_amdgcn_readlane(keys[i], at);
-        r.first = __builtin_amdgcn_readlane(sums[i], at) - attn_tiles(r.keys) * lanes;
+        r.first = __builtin_amdgcn_readlane(sums[i], at) - attn_row_tiles(attn_tiles(r.keys), r.run) * lanes;
     }
+    // one value for the wave, which the addresses of its buffers have to be seen to be
+    r.seq = __builtin_amdgcn_readfirstlane(r.seq);
+    r.keys = __builtin_amdgcn_readfirstlane(r.keys);
+    r.first = __builtin_amdgcn_readfirstlane(r.first);
     return r;
 }
 
@@ -117,7 +138,7 @@ hipError_t launch_attn_i8(const AttnCall &p, hipStream_t s);
 
 // Lanes of work, workgroups of the tiles' kernel, and parts in the workspace.
 inline int64_t attn_lanes(const AttnCall &p) { return (int64_t)p.a.n_seq * p.c.n_kv_heads * p.row_blocks; }
-inline int attn_grid(const AttnCall &p) { return p.split ? kRuns : (int)attn_lanes(p); }
+inline int attn_grid(const AttnCall &p) { return (int)attn_lanes(p) + (p.split ? kRuns : 0); }
 inline int64_t attn_parts(const AttnCall &p) { return p.split ? kRuns + attn_lanes(p) : 0; }
 
 }  // namespace hoard

@@ -126,6 +126,17 @@ __device__ __forceinline__ v4u codes_row(v2u w) {
     return o;
 }
 
+// `bytes` bytes from `at` on as a buffer, and W words of it; those behind its end are zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *at, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(at), (short)0, bytes, 0x00020000);
+}
+template <int W>
+__device__ __forceinline__ auto load(__amdgpu_buffer_rsrc_t from, int at) {
+    if constexpr (W == 4) return __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
+    else if constexpr (W == 2) return __builtin_amdgcn_raw_buffer_load_b64(from, at, 0, 0);
+    else return __builtin_bit_cast(uint32_t __attribute__((ext_vector_type(1))), __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
+}
+
 // A lane's part of a tile of 32 keys as it lies in memory: of the keys 16-byte pieces for
 // the products' steps, of the values DV columns (a piece) of each of 8 keys.
 template <typename C, int DP>
@@ -181,27 +192,32 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
             q_raw[s] = fetch(from, Cols{d < dim ? d : 0, 0}, dim);
         }
     }
+    // the keys that the wave's rows see: each its own, the most and the fewest
+    const int mine = __shfl(seen, row / group);
+    const int hi = row0 < rows ? __builtin_amdgcn_readfirstlane(row16_max_i(mine)) : 0;
+    const int lo = -__builtin_amdgcn_readfirstlane(row16_max_i(-mine));
+    const int end = min(last, (int)(((uint32_t)hi + kKeyTile - 1) / kKeyTile));
     asm volatile("" : "+v"(numbers));
     struct Where {
         int64_t at[2];  // the cache's rows of the tile's halves
-        bool ok[2];
-    };
-    auto fill = [&](int from) {
-        page0 = from;
-        numbers = table[min(from + lane, a.max_pages - 1)];
-        // waited for here, once in 64 pages: where the numbers are used the wait would be for
-        // the keys and values in flight as well
-        asm volatile("" : "+v"(numbers));
+        int n[2];       // of which the wave's rows see so many
     };
     auto where = [&](int tile) {
         Where w;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const int j = tile * kKeyTile + 16 * t, page = min(j >> shift, last_page);
-            if (page - page0 >= 64) fill(page);
+            if (page - page0 >= 64) {
+                page0 = page;
+                numbers = table[min(page + lane, a.max_pages - 1)];
+                // waited for here, once in 64 pages: where the numbers are used the wait would be
+                // for the keys and values in flight as well
+                asm volatile("" : "+v"(numbers));
+            }
             const int number = __builtin_amdgcn_readlane(numbers, page - page0);
-            w.ok[t] = (uint32_t)number < (uint32_t)c.n_pages;
-            w.at[t] = ((int64_t)(w.ok[t] ? number : 0) * c.n_kv_heads + kv) * c.page + (j & (c.page - 1));
+            const bool ok = (uint32_t)number < (uint32_t)c.n_pages;
+            w.n[t] = ok ? min(max(hi - j, 0), 16) : 0;
+            w.at[t] = ((int64_t)(ok ? number : 0) * c.n_kv_heads + kv) * c.page + (j & (c.page - 1));
         }
         return w;
     };
@@ -209,32 +225,32 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     v4u key[2][G::KL];
     typename G::piece val[8][G::H];
     v4f key_scale[2], val_scale[2];
+    // Through buffers that end behind the last key that is seen: what lies behind reads as
+    // zeros, so no value there, whatever it is, meets a weight of zero.
     auto fetch_keys = [&](const Where &w) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const char *from = static_cast<const char *>(c.k) + w.at[t] * dim * (int64_t)sizeof(C);
+            const auto from = buffer(static_cast<const C *>(c.k) + w.at[t] * dim, w.n[t] * dim * (int)sizeof(C));
 #pragma unroll
             for (int s = 0; s < G::KL; s++) {
                 const int d = (s * 64 + 16 * g) / (int)sizeof(C);
-                const int off = (n * dim + (WHOLE || d < dim ? d : 0)) * (int)sizeof(C);
-                key[t][s] = *reinterpret_cast<const v4u *>(from + off);
+                key[t][s] = load<4>(from, (n * dim + (WHOLE || d < dim ? d : 0)) * (int)sizeof(C));
             }
-            if constexpr (CODES) key_scale[t] = *reinterpret_cast<const v4f *>(c.k_scale + w.at[t] + 4 * g);
+            if constexpr (CODES) key_scale[t] = __builtin_bit_cast(v4f, load<4>(buffer(c.k_scale + w.at[t], w.n[t] * 4), 16 * g));
         }
     };
     auto fetch_values = [&](const Where &w) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const char *from = static_cast<const char *>(c.v) + w.at[t] * dim * (int64_t)sizeof(C);
+            const auto from = buffer(static_cast<const C *>(c.v) + w.at[t] * dim, w.n[t] * dim * (int)sizeof(C));
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int h = 0; h < G::H; h++) {
                     const int d = DV * n + 16 * DV * h;
-                    const int off = ((4 * g + r) * dim + (WHOLE || d < dim ? d : 0)) * (int)sizeof(C);
-                    val[4 * t + r][h] = *reinterpret_cast<const typename G::piece *>(from + off);
+                    val[4 * t + r][h] = load<G::VW>(from, ((4 * g + r) * dim + (WHOLE || d < dim ? d : 0)) * (int)sizeof(C));
                 }
-            if constexpr (CODES) val_scale[t] = *reinterpret_cast<const v4f *>(c.v_scale + w.at[t] + 4 * g);
+            if constexpr (CODES) val_scale[t] = __builtin_bit_cast(v4f, load<4>(buffer(c.v_scale + w.at[t], w.n[t] * 4), 16 * g));
         }
     };
 
@@ -248,12 +264,6 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     Where cur = where(min(ti, last - 1)), next{};
     fetch_keys(cur);
     fetch_values(cur);
-
-    // the keys that the wave's rows see: each its own, the most and the fewest
-    const int mine = __shfl(seen, row / group);
-    const int hi = row0 < rows ? __builtin_amdgcn_readfirstlane(row16_max_i(mine)) : 0;
-    const int lo = -__builtin_amdgcn_readfirstlane(row16_max_i(-mine));
-    const int end = min(last, (int)(((uint32_t)hi + kKeyTile - 1) / kKeyTile));
 
     // queries, as planes: the k-th values of a product's step are those that the keys' pieces hold
     v4u q[K::qp][STEPS];
@@ -294,7 +304,7 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     // The last tile is a copy of the loop without fetches: under a condition the compiler
     // could not count them, and would wait for all.
     auto step = [&](auto more) {
-        const bool full = (ti + 1) * kKeyTile <= lo && cur.ok[0] && cur.ok[1];
+        const bool full = (ti + 1) * kKeyTile <= lo && cur.n[0] == 16 && cur.n[1] == 16;
         if constexpr (more.value) next = where(ti + kw_all);
 
         if constexpr (!WHOLE) {
@@ -331,7 +341,10 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
         if (!full) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4 >= mine || !cur.ok[i / 4]) x[i] = -INFINITY;
+                if (ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4 >= mine || 4 * g + i % 4 >= cur.n[i / 4]) {
+                    x[i] = -INFINITY;
+                    if constexpr (CODES) val_scale[i / 4][i % 4] = 0.0f;  // whatever it is
+                }
         }
         const float top = far_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
         if (__any(top > m)) {
@@ -349,49 +362,35 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
             l += x[i];
         }
 
-        // Values of keys that no row of the wave sees count as zeros, and so do, where a row
-        // does not see the key, those that are not finite: zero times them is not zero.  The
-        // rows that do see them get them after the loop.
-        if (!full) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const bool none = ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4 >= hi || !cur.ok[i / 4];
-                if constexpr (CODES) val_scale[i / 4][i % 4] = none ? 0.0f : val_scale[i / 4][i % 4];
-                else
-#pragma unroll
-                    for (int h = 0; h < G::H; h++) val[i][h] = none ? typename G::piece{} : val[i][h];
-            }
+        // Where some rows of the wave see a key and others do not, its values that are not finite
+        // count as zeros: zero times them is not zero.  The rows that do see them get them
+        // after the loop.  (Of codes only the scale may be so, which each row has as its own.)
+        if constexpr (!CODES)
             if (lo < hi && (ti + 1) * kKeyTile > lo) {
                 // an exponent of ones carries into the sign's place
                 constexpr uint32_t exponent = HALF ? 0x7c007c00u : 0x7f807f80u, one = HALF ? 0x04000400u : 0x00800080u;
                 uint32_t carried = 0;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if constexpr (CODES) carried |= fabsf(val_scale[i / 4][i % 4]) <= 3.4028235e38f ? 0u : 0x80008000u;
-                    else
+                for (int i = 0; i < 8; i++)
 #pragma unroll
-                        for (int h = 0; h < G::H; h++)
+                    for (int h = 0; h < G::H; h++)
 #pragma unroll
-                            for (int w = 0; w < G::VW; w++) carried |= (val[i][h][w] & exponent) + one;
-                }
+                        for (int w = 0; w < G::VW; w++) carried |= (val[i][h][w] & exponent) + one;
                 if (__any(carried & 0x80008000u)) {
                     odd = true;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         if (ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4 < lo) continue;
-                        if constexpr (CODES) val_scale[i / 4][i % 4] = fabsf(val_scale[i / 4][i % 4]) <= 3.4028235e38f ? val_scale[i / 4][i % 4] : 0.0f;
-                        else
 #pragma unroll
-                            for (int h = 0; h < G::H; h++)
+                        for (int h = 0; h < G::H; h++)
 #pragma unroll
-                                for (int w = 0; w < G::VW; w++) {
-                                    const uint32_t bad = ((val[i][h][w] & exponent) + one) & 0x80008000u;
-                                    val[i][h][w] &= (bad & 0x8000u ? 0u : 0xffffu) | (bad >> 31 ? 0u : 0xffff0000u);
-                                }
+                            for (int w = 0; w < G::VW; w++) {
+                                const uint32_t bad = ((val[i][h][w] & exponent) + one) & 0x80008000u;
+                                val[i][h][w] &= (bad & 0x8000u ? 0u : 0xffffu) | (bad >> 31 ? 0u : 0xffff0000u);
+                            }
                     }
                 }
             }
-        }
         if constexpr (CODES) {
             float largest = 0.0f;
 #pragma unroll
@@ -449,28 +448,26 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     settle(acc);
     l = far_sum(l);
     // what was not finite, to the rows that see it
-    if (odd) {
-        for (int j = max(lo, 0); j < hi; j++) {
-            if (j / kKeyTile < first || (j / kKeyTile - first) % kw_all != kw || j / kKeyTile >= end) continue;
-            const int number = table[j >> shift];
-            if (j >= mine || (uint32_t)number >= (uint32_t)c.n_pages) continue;
-            const int64_t at = ((int64_t)number * c.n_kv_heads + kv) * c.page + (j & (c.page - 1));
-            const C *from = static_cast<const C *>(c.v) + at * dim;
+    if constexpr (!CODES)
+        if (odd) {
+            for (int j = max(lo, 0); j < hi; j++) {
+                if (j / kKeyTile < first || (j / kKeyTile - first) % kw_all != kw || j / kKeyTile >= end) continue;
+                const int number = table[j >> shift];
+                if (j >= mine || (uint32_t)number >= (uint32_t)c.n_pages) continue;
+                const int64_t at = ((int64_t)number * c.n_kv_heads + kv) * c.page + (j & (c.page - 1));
+                const C *from = static_cast<const C *>(c.v) + at * dim;
 #pragma unroll
-            for (int h = 0; h < G::H; h++)
+                for (int h = 0; h < G::H; h++)
 #pragma unroll
-                for (int i = 0; i < DV; i++)
+                    for (int i = 0; i < DV; i++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int d = 16 * DV * h + DV * (4 * g + r) + i;
-                        float v = 0.0f;
-                        if constexpr (CODES) v = c.v_scale[at];
-                        else if (d < dim) v = (float)from[d];
-                        if (!(fabsf(v) <= 3.4028235e38f)) acc[h * DV + i][r] += v;
-                    }
+                        for (int r = 0; r < 4; r++) {
+                            const int d = 16 * DV * h + DV * (4 * g + r) + i;
+                            const float v = d < dim ? (float)from[d] : 0.0f;
+                            if (!(fabsf(v) <= 3.4028235e38f)) acc[h * DV + i][r] += v;
+                        }
+            }
         }
-    }
-
     // the waves of the same rows joined: each scales its sums to the maximum of all
     if (g == 0) {
         stat[wave][0][n] = m;
@@ -533,16 +530,21 @@ __global__ __launch_bounds__(64 * attn_waves(DP), DP > 128 ? 1 : 2) void attn_ti
         attn_part<T, C, DP, WHOLE>(p, seq, blockIdx.x % lanes, seen, keys, 0, attn_tiles(keys), -1);
         return;
     }
-    const AttnPlace place = attn_place(p, -1);
+    const AttnPlace place = attn_place(p);
     if (place.seq < 0) return;
-    int seq = place.seq, seen = attn_seen(p.a, limit, seq), tiles = attn_tiles(place.keys), keys = place.keys;
-    int left = min(place.run, place.total - (int)blockIdx.x * place.run);
-    int at = blockIdx.x * place.run - place.first, lane = at / tiles;
-    at -= lane * tiles;
+    int seq = place.seq, seen = attn_seen(p.a, limit, seq), keys = place.keys, tiles = attn_tiles(keys);
+    const bool own = attn_own(place.run);
+    int at = blockIdx.x * place.run - place.first, lane = at / attn_row_tiles(tiles, place.run);
+    at -= lane * attn_row_tiles(tiles, place.run);
+    int left = min(place.run, own ? tiles - at : place.total - (int)blockIdx.x * place.run);
+    lane = __builtin_amdgcn_readfirstlane(lane);
+    at = __builtin_amdgcn_readfirstlane(at);
+    left = __builtin_amdgcn_readfirstlane(left);
     while (true) {
         const int last = min(tiles, at + left);
         const bool whole = at == 0 && last == tiles;
-        attn_part<T, C, DP, WHOLE>(p, seq, lane, seen, keys, at, last, whole ? -1 : (int64_t)blockIdx.x + (int64_t)seq * lanes + lane);
+        const int64_t part = (int64_t)blockIdx.x + (own ? 0 : (int64_t)seq * lanes + lane);
+        attn_part<T, C, DP, WHOLE>(p, seq, lane, seen, keys, at, last, whole ? -1 : part);
         left -= last - at;
         if (left <= 0) return;
         at = 0;
