@@ -10,34 +10,50 @@ namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
+// A wave joins a row where there are many of them, of few parts each (64 sequences by 32 heads, two
+// parts: 4.9 us, a workgroup a row 7.3; 80 tokens by 16 heads, 9 parts: 7.3 and 5.7).
+constexpr int kJoinRows = 512, kJoinLanes = kRuns / 2;
+
+// The parts of one row: their number, the first one's row in the workspace and the distance to
+// the next one's.
+struct RowParts {
+    int parts, step;
+    int64_t first;
+};
+__device__ __forceinline__ RowParts row_parts(const AttnCall &p, int token, int head) {
+    const hoard_attn_args &a = p.a;
+    const int seq = token / a.n_new, group = a.n_q_heads / p.c.n_kv_heads;
+    const int row = token % a.n_new * group + head % group, block = row / p.block_rows;
+    const int lanes = p.c.n_kv_heads * p.row_blocks, of = head / group * p.row_blocks + block;
+    // the lane's tiles, and the workgroups whose runs they fall in
+    const int before = seq ? p.sums[seq - 1] : 0, run = p.sums[a.n_seq];
+    const int tiles = (p.sums[seq] - before) / lanes, begin = before + of * tiles, from_run = begin / run;
+    return RowParts{(begin + tiles - 1) / run - from_run + 1, p.block_rows,
+                    (from_run + (attn_own(run) ? 0 : (int64_t)seq * lanes + of)) * p.block_rows + row % p.block_rows};
+}
+
 // out = sum_s w_s part_s,  w_s = 2^(lse_s - m) / sum: the parts of one row, each already
-// divided by its own sum.  A workgroup takes a row: four columns a thread, the parts dealt
-// to the threads left over, which meet in LDS.  What a thread reads first it asks for before
-// the weights are known: the launch is latency alone.
+// divided by its own sum.
+//
+// A workgroup takes a row: four columns a thread, the parts dealt to the threads left over,
+// which meet in LDS.  What a thread reads first it asks for before the weights are known: the
+// launch is latency alone.
 constexpr int kFetch = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall p) {
     __shared__ float weight[kRuns], stat[2][4];
     __shared__ v4f outs[256];
-    const hoard_attn_args &a = p.a;
-    const int token = blockIdx.x, head = blockIdx.y, seq = token / a.n_new, group = a.n_q_heads / p.c.n_kv_heads;
-    const int row = token % a.n_new * group + head % group, block = row / p.block_rows;
-    const int lanes = p.c.n_kv_heads * p.row_blocks, of = head / group * p.row_blocks + block;
-    // the lane's tiles, and the workgroups whose runs they fall in
-    const int before = seq ? p.sums[seq - 1] : 0, run = p.sums[a.n_seq];
-    const int tiles = (p.sums[seq] - before) / lanes, begin = before + of * tiles;
-    const int from_run = begin / run, parts = (begin + tiles - 1) / run - from_run + 1;
-    if (parts == 1) return;
+    const int token = blockIdx.x, head = blockIdx.y;
+    const RowParts row = row_parts(p, token, head);
+    if (row.parts == 1) return;
     const int lane = threadIdx.x & 63, dim = p.c.head_dim;
-    const int64_t first = (from_run + (attn_own(run) ? 0 : (int64_t)seq * lanes + of)) * p.block_rows + row % p.block_rows;
-    const int step = p.block_rows;
-    const float mine = (int)threadIdx.x < parts ? p.part_lse[first + (int)threadIdx.x * step] : -INFINITY;
+    const float mine = (int)threadIdx.x < row.parts ? p.part_lse[row.first + (int64_t)threadIdx.x * row.step] : -INFINITY;
     const int quads = dim / 4, deep = 256 / quads, quad = threadIdx.x % quads, from = threadIdx.x / quads;
-    const float *part = p.part_out + first * dim + 4 * quad;
+    const float *part = p.part_out + row.first * dim + 4 * quad;
     v4f ahead[kFetch];
 #pragma unroll
     for (int i = 0; i < kFetch; i++)
-        ahead[i] = *reinterpret_cast<const v4f *>(part + (int64_t)min(from + i * deep, parts - 1) * step * dim);
+        ahead[i] = *reinterpret_cast<const v4f *>(part + (int64_t)min(from + i * deep, row.parts - 1) * row.step * dim);
     const float top = wave_max_f(mine);
     if (lane == 0) stat[0][wave_index()] = top;
     __syncthreads();
@@ -52,21 +68,67 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall p) {
     if (from < deep) {
 #pragma unroll
         for (int i = 0; i < kFetch; i++)
-            if (from + i * deep < parts) o += weight[from + i * deep] * ahead[i];
+            if (from + i * deep < row.parts) o += weight[from + i * deep] * ahead[i];
 #pragma unroll 4
-        for (int i = from + kFetch * deep; i < parts; i += deep)
-            o += weight[i] * *reinterpret_cast<const v4f *>(part + (int64_t)i * step * dim);
+        for (int i = from + kFetch * deep; i < row.parts; i += deep)
+            o += weight[i] * *reinterpret_cast<const v4f *>(part + (int64_t)i * row.step * dim);
     }
     outs[threadIdx.x] = o;
     __syncthreads();
-    const int64_t out = (int64_t)token * a.n_q_heads + head;
+    const int64_t out = (int64_t)token * p.a.n_q_heads + head;
     if (from == 0) {
         for (int i = 1; i < deep; i++) o += outs[i * quads + quad];
-        T *to = static_cast<T *>(a.out) + out * dim + 4 * quad;
+        T *to = static_cast<T *>(p.a.out) + out * dim + 4 * quad;
 #pragma unroll
         for (int k = 0; k < 4; k++) to[k] = (T)(o[k] * f);
     }
-    if (threadIdx.x == 0 && a.lse) a.lse[out] = (m + log2f(sum)) * 0.6931471805599453f;
+    if (threadIdx.x == 0 && p.a.lse) p.a.lse[out] = (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Many rows of few parts: a wave takes one, its lanes four columns each.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnCall p) {
+    const int64_t out = (int64_t)blockIdx.x * 4 + wave_index();
+    if (out >= (int64_t)p.a.n_seq * p.a.n_new * p.a.n_q_heads) return;
+    const RowParts row = row_parts(p, (int)(out / p.a.n_q_heads), (int)(out % p.a.n_q_heads));
+    if (row.parts == 1) return;
+    const int lane = threadIdx.x & 63, dim = p.c.head_dim, quad = min(lane, dim / 4 - 1);
+    const float *part = p.part_out + row.first * dim + 4 * quad;
+    const v4f first = *reinterpret_cast<const v4f *>(part), second = *reinterpret_cast<const v4f *>(part + (int64_t)row.step * dim);
+    float lse[kRuns / 64], m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kRuns / 64; i++) {
+        lse[i] = i * 64 + lane < row.parts ? p.part_lse[row.first + (int64_t)(i * 64 + lane) * row.step] : -INFINITY;
+        m = fmaxf(m, lse[i]);
+    }
+    m = wave_max_f(m);
+    m = m > -INFINITY ? m : 0.0f;
+    v4f o = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kRuns / 64; i++) {
+        const float w = exp2f(lse[i] - m);
+        sum += w;
+#pragma unroll 4
+        for (int j = 0; j < min(row.parts - i * 64, 64); j++) {
+            const float wj = readlane_f(w, j);
+            o += wj * (i == 0 && j < 2 ? (j ? second : first) : *reinterpret_cast<const v4f *>(part + (int64_t)(i * 64 + j) * row.step * dim));
+        }
+    }
+    sum = wave_sum_f(sum);
+    const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
+    if (lane < dim / 4) {
+        T *to = static_cast<T *>(p.a.out) + out * dim + 4 * quad;
+#pragma unroll
+        for (int k = 0; k < 4; k++) to[k] = (T)(o[k] * f);
+    }
+    if (lane == 0 && p.a.lse) p.a.lse[out] = (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+template <typename T>
+void join(const AttnCall &p, hipStream_t s) {
+    const int64_t rows = (int64_t)p.a.n_seq * p.a.n_new * p.a.n_q_heads;
+    if (rows >= kJoinRows && attn_lanes(p) >= kJoinLanes) attn_join_rows_kernel<T><<<(int)((rows + 3) / 4), 256, 0, s>>>(p);
+    else attn_join_kernel<T><<<dim3(p.a.n_seq * p.a.n_new, p.a.n_q_heads), 256, 0, s>>>(p);
 }
 
 // Lanes of so many tiles are not cut: the join would take longer.
@@ -122,10 +184,9 @@ hipError_t launch_attn(const hoard_kv_cache &c, const hoard_attn_args &a, float 
         if (rc != hipSuccess) return rc;
     }
     if (!p.split) return hipSuccess;
-    const dim3 grid(a.n_seq * a.n_new, a.n_q_heads);
-    if (a.type == HOARD_TYPE_F32) attn_join_kernel<float><<<grid, 256, 0, s>>>(p);
-    else if (a.type == HOARD_TYPE_F16) attn_join_kernel<f16><<<grid, 256, 0, s>>>(p);
-    else attn_join_kernel<bf16><<<grid, 256, 0, s>>>(p);
+    if (a.type == HOARD_TYPE_F32) join<float>(p, s);
+    else if (a.type == HOARD_TYPE_F16) join<f16>(p, s);
+    else join<bf16>(p, s);
     return hipGetLastError();
 }
 
