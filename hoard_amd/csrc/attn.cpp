@@ -105,7 +105,7 @@ int check_attn(const hoard_kv_cache *cache, const hoard_attn_args *a) {
         return fail_fmt(HOARD_ERR_INVALID, "%d sequences of %d tokens", a->n_seq, a->n_new);
     if (a->n_q_heads < 1 || a->n_q_heads > kMaxHeads || a->n_q_heads % cache->n_kv_heads)
         return fail_fmt(HOARD_ERR_INVALID, "n_q_heads %d beside %d key heads", a->n_q_heads, cache->n_kv_heads);
-    if (a->max_pages < 0 || (int64_t)a->max_pages * cache->page > INT32_MAX)
+    if (a->max_pages < 0 || (int64_t)a->max_pages * cache->page > 1 << 30)  // the end of a tile behind the last is a number
         return fail_fmt(HOARD_ERR_INVALID, "max_pages %d of %d tokens", a->max_pages, cache->page);
     if (a->scale != a->scale) return fail_fmt(HOARD_ERR_INVALID, "scale is NaN");
     return 0;

@@ -145,9 +145,9 @@ AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work)
     p.min_run = attn_waves(c.head_dim) / p.row_waves;
     p.block_rows = rows < 16 * p.row_waves ? rows : 16 * p.row_waves;
     // cut where the lanes alone would leave the chip half empty or uneven, and there is something
-    // to cut; the row of tiles is counted in 32 bits
+    // to cut; the row of tiles, three times (runs behind its end have numbers too), in 32 bits
     const int64_t tiles_most = ((int64_t)a.max_pages * c.page + kKeyTile - 1) / kKeyTile;
-    p.split = attn_lanes(p) < 2 * kRuns && a.n_seq <= kMaxSplitSeqs && tiles_most > kWholeTiles && attn_lanes(p) * tiles_most < INT32_MAX;
+    p.split = attn_lanes(p) < 2 * kRuns && a.n_seq <= kMaxSplitSeqs && tiles_most > kWholeTiles && attn_lanes(p) * tiles_most < 1 << 28;
     if (p.split) {
         p.part_out = work;
         p.part_lse = work ? work + attn_parts(p) * p.block_rows * c.head_dim : nullptr;

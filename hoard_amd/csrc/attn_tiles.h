@@ -75,16 +75,15 @@ __device__ __forceinline__ uint32_t plane(bf16, v2f &x) {
     return __builtin_bit_cast(uint32_t, h);
 }
 
-// Waits out the last matrix instruction (8 wait states) before vector instructions read
-// its result behind a branch, over which the compiler does not count them.
-__device__ __forceinline__ void settle(v4f &a, v4f &b) { asm volatile("s_nop 7" : "+v"(a), "+v"(b)); }
+// Waits out the last matrix instruction (16 states, more than any of its kind takes) before
+// vector instructions read its result behind a branch, over which the compiler was seen not to
+// count them.
+__device__ __forceinline__ void settle(v4f &a, v4f &b) { asm volatile("s_nop 15" : "+v"(a), "+v"(b)); }
 template <int N>
 __device__ __forceinline__ void settle(v4f (&a)[N]) {
     static_assert(N % 4 == 0, "four at a time");
-    // the products come in ascending order: behind the last four's wait all are done
-    asm volatile("s_nop 7" : "+v"(a[N - 4]), "+v"(a[N - 3]), "+v"(a[N - 2]), "+v"(a[N - 1]));
 #pragma unroll
-    for (int i = 0; i + 4 < N; i += 4) asm volatile("s_nop 7" : "+v"(a[i]), "+v"(a[i + 1]), "+v"(a[i + 2]), "+v"(a[i + 3]));
+    for (int i = 0; i < N; i += 4) asm volatile("s_nop 15" : "+v"(a[i]), "+v"(a[i + 1]), "+v"(a[i + 2]), "+v"(a[i + 3]));
 }
 
 // Maximum and sum over the four lanes 16 apart, in all of them.

@@ -131,7 +131,8 @@ int hoard_heads_workspace(const hoard_heads_args *a, size_t *bytes);
    that a row does not see may hold anything, and so may a page table's entries behind
    the last key.  Keys and values are used as the cache holds them, q and the weights
    with at least 16 bits for 16-bit activations and 22 for fp32 ones.  1 <= n_new <= 64,
-   n_q_heads a multiple of the cache's n_kv_heads up to 1024, n_seq * n_new < 2^24.
+   n_q_heads a multiple of the cache's n_kv_heads up to 1024, n_seq * n_new < 2^24,
+   max_pages * page <= 2^30.
    workspace: hoard_attn_workspace's bytes (possibly 0), 16-byte aligned, used by the
    call alone while it runs.  `cache` and `a` are host memory. */
 typedef struct hoard_attn_args {

@@ -47,7 +47,7 @@ def rotate(x, ex, rope, back=False):
     y1, y2 = _halves(out, rot, pairs)
     y1.copy_(x1 * c - x2 * s)
     y2.copy_(x2 * c + x1 * s)
-    off = (x1.abs() + x2.abs()) * (ec + 3 * U32) + (e1 + e2) * (1 + ec)
+    off = (x1.detach().abs() + x2.detach().abs()) * (ec + 3 * U32) + (e1 + e2) * (1 + ec)
     for b in _halves(bound, rot, pairs):
         b.copy_(off)
     return out, bound

@@ -141,7 +141,7 @@ def test_heads_workspace(hlib):
     (dict(type=H.TYPE_I8), H.ERR_UNSUPPORTED, "type"), (dict(n_seq=-1), H.ERR_INVALID, "sequences"), (dict(n_new=0), H.ERR_INVALID, "n_new"),
     (dict(n_new=65), H.ERR_INVALID, "n_new"), (dict(n_seq=1 << 24), H.ERR_INVALID, "sequences"), (dict(n_q_heads=0), H.ERR_INVALID, "n_q_heads"),
     (dict(n_q_heads=3), H.ERR_INVALID, "n_q_heads"), (dict(n_q_heads=1026), H.ERR_INVALID, "n_q_heads"),
-    (dict(max_pages=-1), H.ERR_INVALID, "max_pages"), (dict(max_pages=1 << 27), H.ERR_INVALID, "max_pages"),
+    (dict(max_pages=-1), H.ERR_INVALID, "max_pages"), (dict(max_pages=1 << 27), H.ERR_INVALID, "max_pages"), (dict(max_pages=(1 << 26) + 1), H.ERR_INVALID, "max_pages"),
     (dict(scale=float("nan")), H.ERR_INVALID, "scale")])
 def test_attention(hlib, kw, code, word):
     c, a, need = cache(), attn(**kw), ctypes.c_size_t()

@@ -298,6 +298,41 @@ def test_graphs_streams_and_workspaces(longest):
         assert torch.equal(o.out, want[i % 2].out)
 
 
+@pytest.mark.parametrize("n,hkv,t,longest", [
+    (40, 2, 1, 900), (65, 1, 1, 700), (100, 2, 1, 600), (130, 1, 3, 560), (256, 1, 1, 640), (257, 1, 1, 700), (300, 2, 1, 200),
+    (3, 2, 4, 3000), (5, 4, 1, 5000), (70, 4, 1, 600), (2, 1, 64, 700)])
+@pytest.mark.parametrize("ct", [F16, I8])
+def test_batches(n, hkv, t, longest, ct):
+    """Batches on both sides of where lanes are cut, share runs or have their own, some sequences empty, all of one table."""
+    page, d = 16, 64
+    width = -(-longest // page)
+    c = cache_of(200, page, hkv, d, ct, 131)
+    pages = torch.randint(0, 200, (n, width), generator=gen(132), dtype=torch.int32).cuda()
+    lens = torch.randint(0, longest + 1, (n, 1), generator=gen(133), dtype=torch.int32) - torch.arange(t - 1, -1, -1, dtype=torch.int32)
+    lens[torch.rand(n, generator=gen(134)) < 0.1] = 0
+    lens[n // 2, -1] = longest
+    q = (2.0 * torch.randn((n * t, 2 * hkv, d), generator=gen(135))).to(BF16).cuda()
+    check(q, c, pages, lens.cuda().contiguous())
+
+
+def test_a_sequence_whose_tokens_see_far_apart_numbers_of_keys():
+    """Rows of one tile that see 1 key, all of them, or none, over several parts, with values that are not finite between."""
+    c = cache_of(300, 16, 1, 128, BF16, 141)
+    pages = table(1, 260, 300, 142)
+    lens = torch.tensor([[1, 4000, 0, 70, 4160, 2000]], dtype=torch.int32, device="cuda")
+    q = torch.randn((6, 2, 128), generator=gen(143)).to(BF16).cuda()
+    got = check(q, c, pages, lens)
+    clean = got.out.clone()
+    for j, value in ((3000, math.inf), (3999, -math.inf), (2500, math.nan)):
+        c.v[int(pages[0, j // 16]), 0, j % 16, 5] = value
+    from hoard_amd import attn
+    got = attn.attn_decode(q, c, pages, lens).out
+    for r in (0, 2, 3, 5):
+        assert torch.equal(got[r], clean[r]), r
+    for r in (1, 4):
+        assert got[r, :, 5].isnan().all() and torch.isfinite(got[r][:, [0, 1, 2, 3, 4, 6, 127]]).all()
+
+
 def test_refusals():
     from hoard_amd import attn
     c = cache_of(4, 16, 2, 64, F16, 121)
