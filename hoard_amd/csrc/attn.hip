@@ -26,10 +26,10 @@ __device__ __forceinline__ RowParts row_parts(const AttnCall &p, int token, int 
     const int row = token % a.n_new * group + head % group, block = row / p.block_rows;
     const int lanes = p.c.n_kv_heads * p.row_blocks, of = head / group * p.row_blocks + block;
     // the lane's tiles, and the workgroups whose runs they fall in
-    const int before = seq ? p.sums[seq - 1] : 0, run = p.sums[a.n_seq];
+    const int before = seq ? p.sums[seq - 1] : 0, run = p.sums[a.n_seq], own = p.sums[a.n_seq + 1];
     const int tiles = (p.sums[seq] - before) / lanes, begin = before + of * tiles, from_run = begin / run;
     return RowParts{(begin + tiles - 1) / run - from_run + 1, p.block_rows,
-                    (from_run + (attn_own(run) ? 0 : (int64_t)seq * lanes + of)) * p.block_rows + row % p.block_rows};
+                    (from_run + (own ? 0 : (int64_t)seq * lanes + of)) * p.block_rows + row % p.block_rows};
 }
 
 // out = sum_s w_s part_s,  w_s = 2^(lse_s - m) / sum: the parts of one row, each already
@@ -131,10 +131,14 @@ void join(const AttnCall &p, hipStream_t s) {
     else attn_join_kernel<T><<<dim3(p.a.n_seq * p.a.n_new, p.a.n_q_heads), 256, 0, s>>>(p);
 }
 
-// Lanes of so many tiles are not cut: the join would take longer.
+// Lanes of so many tiles are not cut: the join takes longer than it gains (512 tokens by 4 lanes
+// 8.3 us in the kernel, some 10 with a join; 1024 tokens 12.5 and 10.3).
 constexpr int kWholeTiles = 16;
 
-// Waves side by side over the rows where there are more than 16.
+// Waves side by side over the rows where there are more than 16, which so read a tile at about
+// the same time.  (Two tiles of rows a wave, that unpack keys and values once for both, took 30 to
+// 36 us against 27 to 33 for 16 sequences of 3 new tokens by 8 heads, 3000 keys, and spilled in
+// fp32 at 256 columns.)
 AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work) {
     AttnCall p{};
     p.c = c;
@@ -142,7 +146,7 @@ AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work)
     const int rows = a.n_new * (a.n_q_heads / c.n_kv_heads), tiles = (rows + 15) / 16;
     p.row_waves = tiles >= 3 ? 4 : tiles;
     p.row_blocks = (tiles + p.row_waves - 1) / p.row_waves;
-    p.min_run = attn_waves(c.head_dim) / p.row_waves;
+    p.min_run = kAttnWaves / p.row_waves;
     p.block_rows = rows < 16 * p.row_waves ? rows : 16 * p.row_waves;
     // cut where the lanes alone would leave the chip half empty or uneven, and there is something
     // to cut; the row of tiles, three times (runs behind its end have numbers too), in 32 bits
@@ -162,7 +166,7 @@ constexpr int64_t kMaxGrid = 1 << 23;
 
 size_t attn_work_bytes(const hoard_kv_cache &c, const hoard_attn_args &a) {
     const AttnCall p = call_of(c, a, nullptr);
-    return p.split ? sizeof(float) * ((size_t)(c.head_dim + 1) * attn_parts(p) * p.block_rows + a.n_seq + 1) : 0;
+    return p.split ? sizeof(float) * ((size_t)(c.head_dim + 1) * attn_parts(p) * p.block_rows + a.n_seq + 2) : 0;
 }
 
 hipError_t launch_attn(const hoard_kv_cache &c, const hoard_attn_args &a, float *work, hipStream_t s) {

@@ -9,13 +9,17 @@
 // workspace in its parts, and a second launch joins them.  The parts in the order of the row are
 // numbered by workgroup + lane, as one of the two grows from each to the next.  Where the runs
 // are short a second part costs a workgroup more than an even share gains: there every lane
-// begins a run of its own, and the parts are numbered by workgroup (1025 tokens by 4 lanes: 13.3
-// us with runs over lanes, 2048 tokens 11.1).
+// begins a run of its own, and the parts are numbered by workgroup (a call with 1025 tokens by
+// 4 lanes takes 11 us, 13.3 with runs over lanes; with 2048 tokens 11).  Their runs are so long
+// that there are no more of them than CUs, where the lanes leave room for that: at 256 columns
+// a CU holds one workgroup, and the rest would come second (16 sequences of 5 new tokens, 28000
+// keys in all: 43 us with runs of a 256th of the tiles, 30 so).
 //
-// Equal runs, as one compute unit reads no more than twice its share of the memory's rate:
-// with whole lanes cut into up to four parts each, 64 sequences of 512 to 8192 tokens took
-// 69 us (a workgroup for each part, 65 to 69 with other sizes) against 49 for as many tokens
-// in equal sequences.
+// One workgroup a CU: 64 equal sequences of 4352 tokens by 4 lanes, 8-bit codes, take 55 us in
+// 256 runs, 62 in 512, 64 in 1024 (the join of the parts included); 16 of some 1600 by 2 lanes of
+// 256 columns 20, 28 and 28.  Equal runs, as a CU reads no more than twice its share of the
+// memory's rate: 64 sequences of 512 to 8192 tokens 70 us, 78 where each lane is cut by itself
+// into parts of up to the same length, 82 into two.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -27,11 +31,12 @@ namespace hoard {
 
 constexpr int kKeyTile = 32;
 constexpr int kRuns = 256;     // a workgroup a CU
-constexpr int kOwnRun = 16;    // shorter runs hold one lane's tiles only
+constexpr int kOwnRun = 16;    // where even runs would be shorter each holds one lane's tiles only
 constexpr int kMaxSplitSeqs = 256;
 
-// Waves of the tiles' workgroup: two a SIMD where their registers leave room.
-constexpr int attn_waves(int dim) { return 4; }
+// Waves of the tiles' workgroup.  Eight read no faster (one sequence of 32768 tokens in bf16
+// 19.3 us against 18.4), and take longer to start (256 tokens, the kernel: 6.9 against 6.1).
+constexpr int kAttnWaves = 4;
 
 struct AttnCall {
     hoard_kv_cache c;
@@ -42,7 +47,8 @@ struct AttnCall {
     int block_rows;  // rows of a workgroup
     int min_run;     // tiles of a run, at least: one a wave
     float *part_out, *part_lse;  // [parts][block_rows][head_dim] and [parts][block_rows], with split
-    int32_t *sums;   // [n_seq + 1]: tiles of all lanes of the sequences up to each, a run's; with split
+    int32_t *sums;   // [n_seq + 2]: tiles of all lanes of the sequences up to each, a run's, whether
+                     // runs hold one lane's tiles only; with split
 };
 
 // The keys that each new token of a sequence sees, a lane each, and the most of them.
@@ -76,11 +82,11 @@ __device__ __forceinline__ int attn_tiles(int keys) {
 // Where in the row of tiles a sequence lies: its keys, its first tile and what a run holds.
 struct AttnPlace {
     int seq, keys, first, run, total;
+    bool own;
 };
-// Whether runs of that length hold one lane's tiles only, and a lane's tiles then.
-__device__ __forceinline__ bool attn_own(int run) { return run < kOwnRun; }
-__device__ __forceinline__ int attn_row_tiles(int tiles, int run) {
-    return attn_own(run) ? (tiles + run - 1) / run * run : tiles;
+// A lane's tiles in the row: whole runs where they hold one lane's only.
+__device__ __forceinline__ int attn_row_tiles(int tiles, int run, bool own) {
+    return own ? (tiles + run - 1) / run * run : tiles;
 }
 // The sequence that holds tile (blockIdx.x * run) of the row; seq -1 where the row is shorter.  By
 // all lanes of a wave.  The first workgroup leaves the sums for the join.
@@ -103,18 +109,26 @@ __device__ __forceinline__ AttnPlace attn_place(const AttnCall &p) {
     for (int i = 0; i < STEPS; i++)
         if (i * 64 < a.n_seq)
             all += __builtin_amdgcn_readlane(attn_running(i * 64 + lane < a.n_seq ? attn_tiles(keys[i]) : 0), 63);
-    AttnPlace r{-1, 0, 0, 0, 0};
-    r.run = max((all * lanes + kRuns - 1) / kRuns, p.min_run);
+    AttnPlace r{-1, 0, 0, 0, 0, false};
+    r.run = (all * lanes + kRuns - 1) / kRuns;
+    r.own = r.run < kOwnRun;
+    if (r.own) {
+        const int runs = max(kRuns - a.n_seq * lanes, kRuns / 2);
+        r.run = max((all * lanes + runs - 1) / runs, p.min_run);
+    }
 #pragma unroll
     for (int i = 0; i < STEPS; i++) {
         sums[i] = before;
         if (i * 64 >= a.n_seq) continue;
         // of this sequence and those before it
-        sums[i] += attn_running(i * 64 + lane < a.n_seq ? attn_row_tiles(attn_tiles(keys[i]), r.run) * lanes : 0);
+        sums[i] += attn_running(i * 64 + lane < a.n_seq ? attn_row_tiles(attn_tiles(keys[i]), r.run, r.own) * lanes : 0);
         before = __builtin_amdgcn_readlane(sums[i], 63);
         if (blockIdx.x == 0 && threadIdx.x < 64 && i * 64 + lane < a.n_seq) p.sums[i * 64 + lane] = sums[i];
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.sums[a.n_seq] = r.run;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.sums[a.n_seq] = r.run;
+        p.sums[a.n_seq + 1] = r.own;
+    }
     r.total = before;
 #pragma unroll
     for (int i = 0; i < STEPS; i++) {
@@ -123,7 +137,7 @@ __device__ __forceinline__ AttnPlace attn_place(const AttnCall &p) {
         if (at >= 64 || i * 64 + at >= a.n_seq) continue;
         r.seq = i * 64 + at;
         r.keys = __builtin_amdgcn_readlane(keys[i], at);
-        r.first = __builtin_amdgcn_readlane(sums[i], at) - attn_row_tiles(attn_tiles(r.keys), r.run) * lanes;
+        r.first = __builtin_amdgcn_readlane(sums[i], at) - attn_row_tiles(attn_tiles(r.keys), r.run, r.own) * lanes;
     }
     // one value for the wave, which the addresses of its buffers have to be seen to be
     r.seq = __builtin_amdgcn_readfirstlane(r.seq);

@@ -15,13 +15,20 @@
 // The next tile's keys are fetched once this tile's scores are formed, its values once this
 // tile's are used, so that half a tile or more is in flight all the time.
 //
-// Bound by memory: 4 rows * dim operations a key for 2 dim values, 16 rows at a time, is
-// far below what the matrix instructions do meanwhile.  So they take more of them where
-// that keeps digits: weights as two 16-bit planes (f16: 22 bits, bf16: 16; three for fp32:
-// 24), fp32 queries as two f16 planes of a row brought by a power of two to 2^14 or as three
-// bf16 planes.  8-bit codes become f16 exactly (the byte as a subnormal, times 2^15 less a
-// quarter: code * 2^-9); a key's scale multiplies its score, a value's its weight, relative
-// to the power of two above the largest scale so far, so that the weights stay in f16's range.
+// Bound by memory from some 10 MB on: 131071 tokens of 8-bit codes by 4 key heads of 128 (138
+// MB) take 28 us, 4.9 TB/s, and 5 for the join; 8 x 2048 tokens by 16 key heads in f16 (134 MB)
+// 24, 5.5 TB/s; below, by the latencies one after the other (lengths, pages and queries, keys,
+// joining the waves: 4 us) and a tile's 1 us a wave: 257 tokens 6.4 us.  A load of keys takes 64
+// bytes of each of 16 rows: one CU reads 16-bit caches at 62 bytes a ns so (138 in whole rows),
+// three times what it gets where all of them read.
+//
+// The matrix instructions have far less to do than they could meanwhile (4 rows * dim operations
+// a key for 2 dim values).  So they take more of them where that keeps digits: weights as two
+// 16-bit planes (f16: 22 bits, bf16: 16; three for fp32: 24), fp32 queries as two f16 planes of a
+// row brought by a power of two to 2^14 or as three bf16 planes.  8-bit codes become f16
+// exactly (the byte as a subnormal, times 2^15 less a quarter: code * 2^-9); a key's scale
+// multiplies its score, a value's its weight, relative to the power of two above the largest
+// scale so far, so that the weights stay in f16's range.
 #pragma once
 
 #include <math.h>
@@ -146,13 +153,12 @@ struct Shape {
     static constexpr int KL = DP * (int)sizeof(C) / 64;      // pieces of a key
     static constexpr int VW = DV * (int)sizeof(C) / 4;       // words of a piece of a value
     typedef uint32_t piece __attribute__((ext_vector_type(VW)));
-    static constexpr int NW = attn_waves(DP);                // waves of a workgroup
 };
 
 }  // namespace attn
 
-// The tiles first .. last - 1 of a lane of work by one workgroup: NW waves, `row_waves` wide
-// over the rows and NW / row_waves deep over the tiles.  part: where the result goes in the
+// The tiles first .. last - 1 of a lane of work by one workgroup: `row_waves` of its waves
+// side by side over the rows, kAttnWaves / row_waves deep over the tiles.  part: where the result goes in the
 // workspace, or -1 for a lane that is whole.
 template <typename T, typename C, int DP, bool WHOLE>
 __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_no, int seen, int keys, int first, int last, int64_t part) {
@@ -164,15 +170,15 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     constexpr int DV = G::DV, NC = G::NC, STEPS = G::STEPS;
     // f16 weights reach from 2^15 down
     constexpr float kLift = HALF ? 15.0f : 0.0f;
-    __shared__ float stat[G::NW][2][16];
-    __shared__ v4f outs[G::NW][16][16 * DV / 4 + 1];
+    __shared__ float stat[kAttnWaves][2][16];
+    __shared__ v4f outs[kAttnWaves][16][16 * DV / 4 + 1];
 
     const hoard_kv_cache &c = p.c;
     const hoard_attn_args &a = p.a;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wave = wave_index();
     const int kv = lane_no / p.row_blocks, block = lane_no % p.row_blocks;
     const int group = a.n_q_heads / c.n_kv_heads, rows = a.n_new * group, dim = WHOLE ? DP : c.head_dim;
-    const int rw = wave % p.row_waves, kw = wave / p.row_waves, kw_all = G::NW / p.row_waves;
+    const int rw = wave % p.row_waves, kw = wave / p.row_waves, kw_all = kAttnWaves / p.row_waves;
     const int row0 = (block * p.row_waves + rw) * 16, row = min(row0 + n, rows - 1);
 
     // page numbers of 64 pages from page0 on, a lane each
@@ -500,7 +506,7 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
                 outs[wave][n][(DV * (4 * g + r) + i) / 4] = v;
             }
         __syncthreads();
-        for (int at = threadIdx.x; at < p.row_waves * 16 * 4 * DV; at += 64 * G::NW) {
+        for (int at = threadIdx.x; at < p.row_waves * 16 * 4 * DV; at += 64 * kAttnWaves) {
             const int quad = at % (4 * DV), r = at / (4 * DV) % 16, tile = at / (4 * DV * 16);
             const int d = 16 * DV * h + 4 * quad, of = (block * p.row_waves + tile) * 16 + r;
             if (of >= rows || d >= dim) continue;
@@ -522,7 +528,7 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
 }
 
 template <typename T, typename C, int DP, bool WHOLE>
-__global__ __launch_bounds__(64 * attn_waves(DP), DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCall p) {
+__global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnCall p) {
     const int lanes = p.c.n_kv_heads * p.row_blocks, limit = p.a.max_pages * p.c.page;
     if (!p.split) {
         const int seq = blockIdx.x / lanes, seen = attn_seen(p.a, limit, seq), keys = attn_most(seen);
@@ -532,9 +538,10 @@ __global__ __launch_bounds__(64 * attn_waves(DP), DP > 128 ? 1 : 2) void attn_ti
     const AttnPlace place = attn_place(p);
     if (place.seq < 0) return;
     int seq = place.seq, seen = attn_seen(p.a, limit, seq), keys = place.keys, tiles = attn_tiles(keys);
-    const bool own = attn_own(place.run);
-    int at = blockIdx.x * place.run - place.first, lane = at / attn_row_tiles(tiles, place.run);
-    at -= lane * attn_row_tiles(tiles, place.run);
+    const bool own = place.own;
+    const int row_tiles = attn_row_tiles(tiles, place.run, own);
+    int at = blockIdx.x * place.run - place.first, lane = at / row_tiles;
+    at -= lane * row_tiles;
     int left = min(place.run, own ? tiles - at : place.total - (int)blockIdx.x * place.run);
     lane = __builtin_amdgcn_readfirstlane(lane);
     at = __builtin_amdgcn_readfirstlane(at);
@@ -560,8 +567,8 @@ __global__ __launch_bounds__(64 * attn_waves(DP), DP > 128 ? 1 : 2) void attn_ti
 template <typename T, typename C, int DP>
 void launch_attn_dim(const AttnCall &p, hipStream_t s) {
     const int grid = attn_grid(p);
-    if (p.c.head_dim == DP) attn_tile_kernel<T, C, DP, true><<<grid, 64 * attn_waves(DP), 0, s>>>(p);
-    else attn_tile_kernel<T, C, DP, false><<<grid, 64 * attn_waves(DP), 0, s>>>(p);
+    if (p.c.head_dim == DP) attn_tile_kernel<T, C, DP, true><<<grid, 64 * kAttnWaves, 0, s>>>(p);
+    else attn_tile_kernel<T, C, DP, false><<<grid, 64 * kAttnWaves, 0, s>>>(p);
 }
 template <typename T, typename C>
 hipError_t launch_attn_typed(const AttnCall &p, hipStream_t s) {
