@@ -18,7 +18,7 @@
 // One workgroup a CU: 64 equal sequences of 4352 tokens by 4 lanes, 8-bit codes, take 55 us in
 // 256 runs, 62 in 512, 64 in 1024 (the join of the parts included); 16 of some 1600 by 2 lanes of
 // 256 columns 20, 28 and 28.  Equal runs, as a CU reads no more than twice its share of the
-// memory's rate: 64 sequences of 512 to 8192 tokens 70 us, 78 where each lane is cut by itself
+// memory's rate: 64 sequences of 512 to 8192 tokens 70 us (the two launches), 78 where each lane is cut by itself
 // into parts of up to the same length, 82 into two.
 #pragma once
 
