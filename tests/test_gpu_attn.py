@@ -315,6 +315,20 @@ def test_batches(n, hkv, t, longest, ct):
     check(q, c, pages, lens.cuda().contiguous())
 
 
+@pytest.mark.parametrize("n,t,longest,d", [(16, 5, 3001, 256), (8, 20, 1500, 256), (60, 1, 900, 256), (130, 1, 700, 256), (9, 7, 2000, 160)])
+@pytest.mark.parametrize("dtype,ct", [(BF16, BF16), (F32, F16), (F16, I8)])
+def test_batches_of_wide_heads(n, t, longest, d, dtype, ct):
+    """Heads of which a CU holds one workgroup, in one or several blocks of rows: runs of one lane, fewer and more than CUs."""
+    page, hkv = 32, 2
+    width = -(-longest // page)
+    c = cache_of(150, page, hkv, d, ct, 151)
+    pages = torch.randint(0, 150, (n, width), generator=gen(152), dtype=torch.int32).cuda()
+    lens = torch.randint(0, longest + 1, (n, 1), generator=gen(153), dtype=torch.int32) - torch.arange(t - 1, -1, -1, dtype=torch.int32)
+    lens[n // 2, -1] = longest
+    q = (2.0 * torch.randn((n * t, 8 * hkv, d), generator=gen(154))).to(dtype).cuda()
+    check(q, c, pages, lens.cuda().contiguous())
+
+
 def test_a_sequence_whose_tokens_see_far_apart_numbers_of_keys():
     """Rows of one tile that see 1 key, all of them, or none, over several parts, with values that are not finite between."""
     c = cache_of(300, 16, 1, 128, BF16, 141)
