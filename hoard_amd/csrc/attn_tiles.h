@@ -27,8 +27,10 @@
 // 16-bit planes (f16: 22 bits, bf16: 16; three for fp32: 24), fp32 queries as two f16 planes of a
 // row brought by a power of two to 2^14 or as three bf16 planes.  8-bit codes become f16
 // exactly (the byte as a subnormal, times 2^15 less a quarter: code * 2^-9); a key's scale
-// multiplies its score, a value's its weight, relative to the power of two above the largest
-// scale so far, so that the weights stay in f16's range.
+// multiplies its score, a value's its weight.  Each row has a power of two of its own that its
+// weighted sums are held by, that of the largest product of a weight and a scale that it has seen,
+// so that the products stay in f16's range: no other row's keys and no scale that weighs nothing
+// take digits from it.
 #pragma once
 
 #include <math.h>
@@ -105,6 +107,12 @@ __device__ __forceinline__ float far_sum(float v) {
     v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ int far_max_i(int v) {
+    auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max((int)r[0], (int)r[1]);
+    r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max((int)r[0], (int)r[1]);
 }
 __device__ __forceinline__ int row16_max_i(int v) {
     v = max(v, dpp_i<kDppQuadXor1>(v));
@@ -261,8 +269,9 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
 
     float m = -INFINITY, l = 0.0f;
     v4f acc[NC] = {};
-    int val_up = 0;  // acc is held times 2^-val_up
-    float val_most = 0.0f;
+    // of codes acc is held times 2^-acc_up, a power of the row's own: kLowest while nothing counts
+    constexpr int kLowest = -512;
+    int acc_up = kLowest;
     bool odd = false;
     // without a condition (a wave without a tile fetches the last one, a lane without keys the
     // cache's first page), so that the queries' wait is not for these as well
@@ -287,10 +296,7 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
             }
         }
         if constexpr (SCALED) {
-            auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-            top = max((int)r[0], (int)r[1]);
-            r = __builtin_amdgcn_permlane16_swap(top, top, false, false);
-            top = max((int)r[0], (int)r[1]);
+            top = far_max_i(top);
             up = top ? 14 + 127 - (top >> 23) : 0;
         }
 #pragma unroll
@@ -353,12 +359,20 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
         }
         const float top = far_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
         if (__any(top > m)) {
-            const float f = top > m ? exp2_of(m - top) : 1.0f;
-            settle(acc);
-            m = fmaxf(m, top);
-            l *= f;
+            if constexpr (CODES) {
+                // a whole number, by which acc's power falls as the earlier weights do: acc stays as it is
+                const float to = top > m ? ceilf(top) : m, rise = to > m ? to - m : 0.0f;
+                acc_up = max(acc_up - (int)fminf(rise, 1024.0f), kLowest);
+                l *= exp2_of(-rise);
+                m = to;
+            } else {
+                const float f = top > m ? exp2_of(m - top) : 1.0f;
+                settle(acc);
+                m = fmaxf(m, top);
+                l *= f;
 #pragma unroll
-            for (int i = 0; i < NC; i++) acc[i] *= f;
+                for (int i = 0; i < NC; i++) acc[i] *= f;
+            }
         }
         const float base = (m > -INFINITY ? m : 0.0f) - kLift;
 #pragma unroll
@@ -397,31 +411,45 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
                 }
             }
         if constexpr (CODES) {
-            float largest = 0.0f;
+            float scaled[8];
+            uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) largest = fmaxf(largest, fabsf(val_scale[i / 4][i % 4]));
-            if (__any(largest > val_most)) {
-                // the power of two above the largest scale
-                largest = wave_max_f(largest);
-                const int to = ((__float_as_int(largest) >> 23) & 0xff) - 126;
+            for (int i = 0; i < 8; i++) {
+                scaled[i] = x[i] * ldexpf(val_scale[i / 4][i % 4], -acc_up);
+                most = max(most, __float_as_uint(scaled[i]));
+            }
+            // near the end of f16's range (or a NaN, or below zero): exponents added, which no scale
+            // leaves, and products below 2^14, so that it is not the next tile's turn at once (64
+            // sequences of 512 to 8192 tokens 78.0 us, 80.7 with products below 2^15 and so checked)
+            if (__any(most > __float_as_uint(65000.0f))) {
+                int need = kLowest;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float scale = fabsf(val_scale[i / 4][i % 4]);
+                    if (x[i] > 0.0f && scale > 0.0f && scale < INFINITY)
+                        need = max(need, __builtin_amdgcn_frexp_expf(x[i]) + __builtin_amdgcn_frexp_expf(scale) - 14);
+                }
+                const int to = max(acc_up, far_max_i(need));
                 settle(acc);
 #pragma unroll
                 for (int i = 0; i < NC; i++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) acc[i][r] = ldexpf(acc[i][r], val_up - to);
-                val_up = to;
-                val_most = ldexpf(1.0f, to);
+                    for (int r = 0; r < 4; r++) acc[i][r] = ldexpf(acc[i][r], acc_up - to);
+                acc_up = to;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float scale = val_scale[i / 4][i % 4];
+                    scaled[i] = ldexpf(x[i] * __builtin_amdgcn_frexp_mantf(scale), __builtin_amdgcn_frexp_expf(scale) - acc_up);
+                }
             }
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = scaled[i];
         }
         // weights as planes: word w holds keys 2w and 2w + 1 of the lane's eight
         v4u weight[K::pp];
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             v2f v = {x[2 * w], x[2 * w + 1]};
-            if constexpr (CODES) {
-                v[0] *= ldexpf(val_scale[w / 2][2 * w % 4], -val_up);
-                v[1] *= ldexpf(val_scale[w / 2][2 * w % 4 + 1], -val_up);
-            }
 #pragma unroll
             for (int pl = 0; pl < K::pp; pl++) weight[pl][w] = plane(E(), v);
         }
@@ -483,7 +511,9 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     for (int w = 0; w < kw_all; w++) top = fmaxf(top, stat[w * p.row_waves + rw][0][n]);
     const float base = top > -INFINITY ? top : 0.0f;
     for (int w = 0; w < kw_all; w++) total += exp2_of(stat[w * p.row_waves + rw][0][n] - base) * stat[w * p.row_waves + rw][1][n];
-    const float f = total != 0.0f ? exp2_of(m - base) / total : 0.0f;
+    // of codes the maxima are whole numbers, and the step between them goes with acc's power
+    const float f = total == 0.0f ? 0.0f : CODES ? 1.0f / total : exp2_of(m - base) / total;
+    const int out_up = CODES ? acc_up + kCodeShift + (int)fmaxf(m - base, -2048.0f) : 0;
     if (kw == 0 && g == 0 && row0 + n < rows) {
         const int64_t out = ((int64_t)seq * a.n_new + row / group) * a.n_q_heads + kv * group + row % group;
         const float log2_sum = base + (log2f(total) - kLift);
@@ -501,7 +531,7 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     v[k] = acc[h * DV + i + k][r] * f;
-                    if constexpr (CODES) v[k] = ldexpf(v[k], val_up + kCodeShift);
+                    if constexpr (CODES) v[k] = ldexpf(v[k], out_up);
                 }
                 outs[wave][n][(DV * (4 * g + r) + i) / 4] = v;
             }

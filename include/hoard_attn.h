@@ -129,8 +129,11 @@ int hoard_heads_workspace(const hoard_heads_args *a, size_t *bytes);
    sees no key (n <= 0) has out 0 and lse -infinity.  n beyond max_pages * page counts as
    that; a page number outside [0, n_pages) hides the keys of its page.  Keys and values
    that a row does not see may hold anything, and so may a page table's entries behind
-   the last key.  Keys and values are used as the cache holds them, q and the weights
-   with at least 16 bits for 16-bit activations and 22 for fp32 ones.  1 <= n_new <= 64,
+   the last key.  Keys and values are used as the cache holds them.  q and the weights are
+   held to 2^-16 of each (2^-22 for fp32 activations) or, over f16 and I8 caches, to 2^-37
+   of the row's largest, whichever is more; with I8 a weight's product with its value's
+   scale is held so, by the keys that the row sees.  A weight below 2^-126 may count as
+   none.  1 <= n_new <= 64,
    n_q_heads a multiple of the cache's n_kv_heads up to 1024, n_seq * n_new < 2^24,
    max_pages * page <= 2^30.
    workspace: hoard_attn_workspace's bytes (possibly 0), 16-byte aligned, used by the
