@@ -70,12 +70,15 @@ def _apart(a, b) -> bool:
 
 
 def _written(name: str, t, inputs=(), or_same=None) -> None:
-    """A tensor to write to, its own checks done: apart from the inputs, or all of `or_same`.  Its version counts the
-    write: autograd refuses a gradient that needs what it held."""
-    for i in (*inputs, or_same):
+    """A tensor to write to, its own checks done: apart from the inputs, but for one of them, `or_same`, whose whole it may
+    be.  Another input that is the same tensor goes on being read, by other waves.  Its version counts the write:
+    autograd refuses a gradient that needs what it held."""
+    for i in inputs:
         if isinstance(i, torch.Tensor):
-            same = i is or_same and i.data_ptr() == t.data_ptr() and i.stride() == t.stride() and i.shape == t.shape
-            _need(same or _apart(t, i), f"{name}: overlaps an input")
+            if i is or_same and i.data_ptr() == t.data_ptr() and i.stride() == t.stride() and i.shape == t.shape:
+                or_same = None
+                continue
+            _need(_apart(t, i), f"{name}: overlaps an input")
     if not t.is_inference():
         torch.autograd.graph.increment_version(t)
 
@@ -254,7 +257,7 @@ def heads_forward(q=None, k=None, v=None, *, w_q=None, w_k=None, rope: Rope | No
             t = torch.empty(x.shape, dtype=dtype, device=device)
         elif t is not None:
             _heads(name, t, x.shape, dtype, device)
-            _written(name, t, [i for i in (*inputs, *outs) if i is not same], same)
+            _written(name, t, (*inputs, *outs), same)
         if t is not None:
             setattr(a, name + "_stride", _heads(name, t))
             setattr(a, name, _p(t))
@@ -287,7 +290,8 @@ def heads_backward(dq_out=None, dk_out=None, *, q=None, k=None, w_q=None, w_k=No
         a.stats = _p(stats)
     _need(stats is not None or (w_q is None and w_k is None), "stats: heads_forward was called without want_stats")
     g, outs = HeadsGrads(), []
-    inputs = [dq_out, dk_out, q, k, w_q, w_k, stats] + (list(rope[:3]) if rope is not None else [])
+    inputs = [dq_out, dk_out, q if w_q is not None else None, k if w_k is not None else None, w_q, w_k, stats]
+    inputs += list(rope[:3]) if rope is not None else []
     for name, x, dx, to in (("q", use_q, dq_out, dq), ("k", use_k, dk_out, dk)):
         _need(to is None or dx is not None, f"d{name}: without d{name}_out")
         if dx is None:
@@ -299,7 +303,7 @@ def heads_backward(dq_out=None, dk_out=None, *, q=None, k=None, w_q=None, w_k=No
             to = torch.empty(x.shape, dtype=dtype, device=device)
         else:
             _heads(f"d{name}", to, x.shape, dtype, device)
-            _written(f"d{name}", to, [i for i in (*inputs, *outs) if i is not dx], dx)
+            _written(f"d{name}", to, (*inputs, *outs), dx)
         setattr(g, f"d{name}_stride", _heads(f"d{name}", to))
         setattr(g, "d" + name + "_out", _p(dx))
         setattr(g, "d" + name, _p(to))
