@@ -88,7 +88,8 @@ def _written(name: str, t, inputs=(), or_same=None) -> None:
 
 class KVCache:
     """Keys and values [n_pages, n_kv_heads, page, head_dim] as float16, bfloat16 or, with scales float32 [n_pages,
-    n_kv_heads, page], int8 codes.  Slot s is place s % page of page s // page."""
+    n_kv_heads, page], int8 codes.  Slot s is place s % page of page s // page.  To be written to, its tensors lie apart
+    from each other."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _tensor("k", k)
@@ -116,8 +117,9 @@ class KVCache:
         return [t for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None]
 
     def _write(self, inputs) -> None:
-        for t in self._tensors():
-            _written("cache", t, inputs)
+        tensors = self._tensors()
+        for n, t in enumerate(tensors):
+            _written("cache", t, (*inputs, *tensors[:n]))
 
 
 def _slots(slots, n, device):
