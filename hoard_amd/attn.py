@@ -288,6 +288,11 @@ def heads_backward(dq_out=None, dk_out=None, *, q=None, k=None, w_q=None, w_k=No
     use_k = k if k is not None else dk_out
     a, n, d, dtype, device = _fill_heads(use_q, use_k, None, w_q, w_k, rope, eps, w_offset, None)
     if stats is not None:
+        _need(isinstance(stats, torch.Tensor) and stats.dim() == 2, "stats: no matrix")
+        if use_q is None:  # the columns of the heads that are not given
+            a.n_q_heads = max(stats.shape[1] - a.n_kv_heads, 0)
+        if use_k is None:
+            a.n_kv_heads = max(stats.shape[1] - a.n_q_heads, 0)
         _tensor("stats", stats, (n, a.n_q_heads + a.n_kv_heads), torch.float32, device)
         a.stats = _p(stats)
     _need(stats is not None or (w_q is None and w_k is None), "stats: heads_forward was called without want_stats")

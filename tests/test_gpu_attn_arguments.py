@@ -1,5 +1,5 @@
 """Calls of the attention half on torch tensors that its documentation allows or refuses: one tensor for two arguments,
-a cache whose tensors overlap."""
+a cache whose tensors overlap, one of the two gradients alone."""
 import pytest
 
 import hoard_amd as H
@@ -58,3 +58,28 @@ def test_a_cache_over_itself():
         with pytest.raises(H.HoardError, match="cache: overlaps"):
             attn.heads_forward(k=x, v=x, cache=c, slots=slots)
     attn.kv_write(attn.KVCache(half, buf[1024:].view(1, 2, 16, 32)), slots, x, x)
+
+
+@pytest.mark.parametrize("rope", [False, True])
+def test_one_gradient_alone(rope):
+    """One of the two, with the statistics of both heads: the other's heads need not be given."""
+    from hoard_amd import attn
+    q, k, w_q, w_k, dq_out, dk_out = rand(7, 4, 32), rand(7, 2, 32), rand(32), rand(32), rand(7, 4, 32), rand(7, 2, 32)
+    r = attn.Rope(torch.arange(7, dtype=torch.int32, device="cuda"), attn.rope_freq(16, 100.0)) if rope else None
+    st = attn.heads_forward(q, k, w_q=w_q, w_k=w_k, rope=r, want_stats=True)
+    both = attn.heads_backward(dq_out, dk_out, q=q, k=k, w_q=w_q, w_k=w_k, rope=r, stats=st.stats)
+    one = attn.heads_backward(dq_out, q=q, w_q=w_q, rope=r, stats=st.stats)
+    assert torch.equal(one.dq, both.dq) and one.dk is None and one.dw_k is None
+    # few tokens: a workgroup's sums, in the same order
+    assert torch.allclose(one.dw_q, both.dw_q, rtol=1e-5, atol=1e-5)
+    one = attn.heads_backward(None, dk_out, k=k, w_k=w_k, rope=r, stats=st.stats)
+    assert torch.equal(one.dk, both.dk) and one.dq is None and one.dw_q is None
+    assert torch.allclose(one.dw_k, both.dw_k, rtol=1e-5, atol=1e-5)
+    # q normed beside heads that go into a cache, whose columns the statistics have too
+    cache = attn.KVCache.new(1, 16, 2, 32, torch.float16)
+    slots = torch.arange(7, dtype=torch.int32, device="cuda")
+    st = attn.heads_forward(q, None, k, w_q=w_q, rope=r, want_stats=True, cache=cache, slots=slots)
+    assert torch.equal(attn.heads_backward(dq_out, q=q, w_q=w_q, rope=r, stats=st.stats).dq, both.dq)
+    for stats in (st.stats[:, :3].contiguous(), st.stats[:6], rand(7, 4, 2), rand(7), 5):
+        with pytest.raises(H.HoardError, match="stats"):
+            attn.heads_backward(dq_out, q=q, w_q=w_q, stats=stats)
