@@ -126,9 +126,14 @@ def _slots(slots, n, device):
     _tensor("slots", slots, (n,), torch.int32, device)
 
 
+def _cache(cache):
+    _need(isinstance(cache, KVCache), "cache: no KVCache")
+
+
 def kv_write(cache: KVCache, slots, k=None, v=None) -> None:
     """Rows of k and v [tokens, n_kv_heads, head_dim] to their slots int32 [tokens]; a slot outside the cache drops its
     token, the others must be distinct."""
+    _cache(cache)
     first = k if k is not None else v
     _need(isinstance(first, torch.Tensor) and first.dim() == 3, "neither k nor v")
     n, dtype = first.shape[0], first.dtype
@@ -145,10 +150,12 @@ def kv_write(cache: KVCache, slots, k=None, v=None) -> None:
 def kv_read(cache: KVCache, slots, dtype=None, *, k=None, v=None):
     """(k, v) [tokens, n_kv_heads, head_dim] of the slots int32 [tokens], into the tensors given or new ones of `dtype`
     (the cache's; bfloat16 for codes).  Rows of a slot outside the cache are left as they are (zero in new tensors)."""
+    _cache(cache)
     _need(isinstance(slots, torch.Tensor) and slots.dim() == 1, "slots: no vector")
     n = slots.shape[0]
     _slots(slots, n, cache.device)
     given = k if k is not None else v
+    _need(given is None or isinstance(given, torch.Tensor), "k or v: no tensor")
     dtype = dtype or (given.dtype if given is not None else torch.bfloat16 if cache.k.dtype == torch.int8 else cache.k.dtype)
     _need(dtype in _TYPES, f"{dtype} is no activation type")
     shape, strides, out = (n, cache.n_kv_heads, cache.head_dim), [], []
@@ -186,7 +193,7 @@ def rope_freq(rot_dim: int, base: float, device="cuda"):
 
 def split_heads(qkv, n_q: int, n_kv: int, dim: int):
     """The q, k and v heads of a fused projection's rows [tokens, (n_q + 2 n_kv) * dim], as views."""
-    _need(qkv.dim() == 2 and qkv.shape[1] == (n_q + 2 * n_kv) * dim, f"qkv: shape {tuple(qkv.shape)}")
+    _need(isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.shape[1] == (n_q + 2 * n_kv) * dim, "qkv: no matrix of that many heads")
     return torch.split(qkv.view(qkv.shape[0], n_q + 2 * n_kv, dim), [n_q, n_kv, n_kv], dim=1)
 
 
@@ -213,6 +220,7 @@ def _fill_heads(q, k, v, w_q, w_k, rope, eps, w_offset, cache):
     if q is not None:
         a.q_stride, a.n_q_heads, a.q = _heads("q", q, (n, q.shape[1], d), dtype, device), q.shape[1], _p(q)
     kv = k if k is not None else v
+    _need(kv is None or isinstance(kv, torch.Tensor) and kv.dim() == 3, "k or v: no heads")
     heads = kv.shape[1] if kv is not None else cache.n_kv_heads if cache is not None else 0
     a.n_kv_heads = heads
     if k is not None:
@@ -224,6 +232,7 @@ def _fill_heads(q, k, v, w_q, w_k, rope, eps, w_offset, cache):
             _tensor(name, w, (d,), torch.float32, device)
             setattr(a, name, _p(w))
     if rope is not None:
+        _need(isinstance(rope, Rope), "rope: no Rope")
         _need(isinstance(rope.freq, torch.Tensor) and rope.freq.dim() == 1, "freq: no vector")
         _tensor("freq", rope.freq, None, torch.float64, device)
         _need(isinstance(rope.pos, torch.Tensor) and rope.pos.dim() in (1, 2), "pos: no vector or matrix")
@@ -242,6 +251,8 @@ def heads_forward(q=None, k=None, v=None, *, w_q=None, w_k=None, rope: Rope | No
     """Each head of q and k normed by its weight (w_offset + w_q, w_k [head_dim]; None: not normed) and rotated.  With a
     cache the rotated k and v as it is go to slots int32 [tokens], and k_out is only written if given; without one it
     is a new tensor.  q_out may be q, and k_out k."""
+    if cache is not None:
+        _cache(cache)
     a, n, d, dtype, device = _fill_heads(q, k, v, w_q, w_k, rope, eps, w_offset, cache)
     inputs = (q, k, v, w_q, w_k, slots) + (tuple(rope[:3]) if rope is not None else ())
     if cache is not None:
@@ -276,7 +287,8 @@ def heads_forward(q=None, k=None, v=None, *, w_q=None, w_k=None, rope: Rope | No
 def heads_backward(dq_out=None, dk_out=None, *, q=None, k=None, w_q=None, w_k=None, rope: Rope | None = None, stats=None,
                    eps: float = 1e-6, w_offset: float = 0.0, dq=None, dk=None) -> HeadsGradients:
     """Gradients of heads_forward given those of q_out and k_out (either may be None): of q and k, and of the weights
-    that are given, which need the forward call's q (k) and stats.  dq may be dq_out, and dk dk_out."""
+    that are given, which need the forward call's q (k) and stats, the columns of all of its heads.  dq may be dq_out, and
+    dk dk_out."""
     given = [t for t in (dq_out, dk_out) if t is not None]
     _need(len(given) > 0, "neither dq_out nor dk_out")
     for name, x, dx in (("q", q, dq_out), ("k", k, dk_out)):
@@ -339,6 +351,7 @@ def attn_decode(q, cache: KVCache, pages, lens, *, scale: float | None = None, o
     [sequences, max_pages], lens int32 [sequences] or [sequences, n_new]: the keys that each sees (0: its row is 0).
     scale: head_dim ** -0.5 by default.  lse: the logarithm of the sum of exp(scale <q, k>), to join results over
     different keys by."""
+    _cache(cache)
     _need(isinstance(lens, torch.Tensor) and lens.dim() in (1, 2), "lens: no vector or matrix")
     _tensor("lens", lens, None, torch.int32, cache.device)
     n_seq, n_new = lens.shape[0], lens.shape[1] if lens.dim() == 2 else 1

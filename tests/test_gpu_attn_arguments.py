@@ -1,5 +1,5 @@
 """Calls of the attention half on torch tensors that its documentation allows or refuses: one tensor for two arguments,
-a cache whose tensors overlap, one of the two gradients alone."""
+a cache whose tensors overlap, one of the two gradients alone, what is no tensor."""
 import pytest
 
 import hoard_amd as H
@@ -83,3 +83,49 @@ def test_one_gradient_alone(rope):
     for stats in (st.stats[:, :3].contiguous(), st.stats[:6], rand(7, 4, 2), rand(7), 5):
         with pytest.raises(H.HoardError, match="stats"):
             attn.heads_backward(dq_out, q=q, w_q=w_q, stats=stats)
+
+
+def test_what_is_no_tensor():
+    from hoard_amd import attn
+    x, w = rand(3, 2, 32), rand(32)
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    cache = attn.KVCache.new(1, 16, 2, 32, torch.float16)
+    freq = attn.rope_freq(16, 100.0)
+    bad = [
+        lambda: attn.heads_forward([1.0], x),
+        lambda: attn.heads_forward(x, [1.0]),
+        lambda: attn.heads_forward(x, 5),
+        lambda: attn.heads_forward(x, rand(3, 64)),
+        lambda: attn.heads_forward(x, v=[1.0], cache=cache, slots=slots),
+        lambda: attn.heads_forward(x, w_q=1.0),
+        lambda: attn.heads_forward(x, rope=(slots, freq)),
+        lambda: attn.heads_forward(x, rope=attn.Rope(slots, [1.0])),
+        lambda: attn.heads_forward(x, rope=attn.Rope([1, 2, 3], freq)),
+        lambda: attn.heads_forward(x, rope=attn.Rope(slots, freq, [0])),
+        lambda: attn.heads_forward(k=x, cache=(x, x), slots=slots),
+        lambda: attn.heads_forward(k=x, cache=cache, slots=[0, 1, 2]),
+        lambda: attn.heads_forward(x, q_out=[1.0]),
+        lambda: attn.heads_backward([1.0]),
+        lambda: attn.heads_backward(x, 5),
+        lambda: attn.heads_backward(x, q=5, w_q=w, stats=rand(3, 2)),
+        lambda: attn.heads_backward(x, dq=[1.0]),
+        lambda: attn.kv_write(None, slots, x),
+        lambda: attn.kv_write(cache, slots, x, [1.0]),
+        lambda: attn.kv_write(cache, slots, [1.0], x),
+        lambda: attn.kv_read(None, slots),
+        lambda: attn.kv_read(cache, slots, k=[1.0]),
+        lambda: attn.kv_read(cache, slots, v=3),
+        lambda: attn.kv_read(cache, [0, 1]),
+        lambda: attn.attn_decode(rand(1, 4, 32), None, slots.view(3, 1), slots),
+        lambda: attn.attn_decode([1.0], cache, slots.view(3, 1), slots),
+        lambda: attn.attn_decode(rand(3, 4, 32), cache, [[0]], slots),
+        lambda: attn.attn_decode(rand(3, 4, 32), cache, slots.view(3, 1), [1]),
+        lambda: attn.attn_decode(rand(3, 4, 32), cache, slots.view(3, 1), slots, out=[1.0]),
+        lambda: attn.KVCache(None, None),
+        lambda: attn.KVCache(cache.k, [1.0]),
+        lambda: attn.split_heads([1.0], 1, 1, 1),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(H.HoardError):
+            call()
+            pytest.fail(str(i))
