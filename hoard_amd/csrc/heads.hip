@@ -101,20 +101,21 @@ __device__ __forceinline__ Place place_of(const hoard_heads_args &h) {
     return p;
 }
 
-// sin and cos of 2 pi f, |f| <= 1/2: of the nearest quarter turn and the rest, an angle of up to
-// pi / 4, by their series up to x^9 and x^10, which leave 2e-9 and 5e-10.
-__device__ __forceinline__ void sincos_turn(float f, float &s, float &c) {
-    const float quarter = rintf(4.0f * f), x = (f - 0.25f * quarter) * 6.2831853071795865f, y = x * x;
+// sin and cos of x + q pi / 2, |x| <= pi / 4: their series up to x^9 and x^10, which leave 2e-9 and
+// 5e-10.
+__device__ __forceinline__ void sincos_quarter(float x, int q, float &s, float &c) {
+    const float y = x * x;
     const float sx = fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), x);
     const float cx = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
-    const int q = (int)quarter;
     const float a = q & 1 ? cx : sx, b = q & 1 ? sx : cx;
     s = q & 2 ? -a : a;
     c = (q + 1) & 2 ? -b : b;
 }
 
 // Cosines and sines of the lane's four pairs.  A position times a frequency is taken in 64
-// bits to its fraction of a turn, so far positions keep their digits.
+// bits to what is left of the nearest quarter turn, so far positions keep their digits and the
+// angle rounds to 32 bits when it is small (errors of 1.2 roundings of 1 at most; 2.4 where the
+// fraction of a whole turn is rounded).
 struct Turn {
     float c[4], s[4];
 };
@@ -130,8 +131,12 @@ __device__ __forceinline__ Turn turn_of(const hoard_heads_args &a, const Place &
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int axis = a.axis ? min((int)a.axis[first + j], a.n_axes - 1) : 0;
-        const double turns = (double)a.pos[(int64_t)axis * a.n_tokens + token] * a.freq[first + j] * 0.15915494309189535;
-        sincos_turn((float)(turns - rint(turns)), t.s[j], t.c[j]);
+        const double quarters = (double)a.pos[(int64_t)axis * a.n_tokens + token] * a.freq[first + j] * 0.63661977236758134;
+        const double whole = rint(quarters);
+        // its last two bits, as those of a double between 2^52 and 2^53 (quarters past 2^51 have no
+        // digits to say which of four they are)
+        const int q = __double2loint(whole + 0x1.8p52);
+        sincos_quarter((float)((quarters - whole) * 1.5707963267948966), q, t.s[j], t.c[j]);
     }
     return t;
 }
