@@ -84,6 +84,20 @@ __device__ __forceinline__ uint32_t plane(bf16, v2f &x) {
     return __builtin_bit_cast(uint32_t, h);
 }
 
+// Of 16-bit pairs those that are not finite, as masks of their halves: an exponent of ones carries
+// into the sign's place.
+__device__ __forceinline__ uint32_t carried(f16, uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; }
+__device__ __forceinline__ uint32_t carried(bf16, uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; }
+template <typename E>
+__device__ __forceinline__ uint32_t not_finite(E, uint32_t w) {
+    const uint32_t c = carried(E(), w);
+    return (c & 0x8000u ? 0xffffu : 0u) | (c >> 31 ? 0xffff0000u : 0u);
+}
+// Their signs: one, minus one or zero.
+__device__ __forceinline__ uint32_t signs(uint32_t one, uint32_t w) {
+    return (w & 0x80008000u) | ((((w & 0x7fff7fffu) + 0x7fff7fffu) >> 15 & 0x00010001u) * one);
+}
+
 // Waits out the last matrix instruction (16 states, more than any of its kind takes) before
 // vector instructions read its result behind a branch, over which the compiler was seen not to
 // count them.
@@ -192,7 +206,8 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     // page numbers of 64 pages from page0 on, a lane each
     const int shift = 31 - __builtin_clz(c.page), last_page = (max(keys, 1) - 1) >> shift;
     const int32_t *table = a.pages + (int64_t)seq * a.max_pages;
-    int ti = first + kw, page0 = (min(ti, last - 1) * kKeyTile) >> shift, numbers = -1;
+    const int first_page = (min(first + kw, last - 1) * kKeyTile) >> shift;
+    int ti = first + kw, page0 = first_page, numbers = -1;
     if (keys) numbers = table[min(page0 + lane, a.max_pages - 1)];
     // the queries, asked for before the first keys and used behind them
     Raw<T> q_raw[STEPS];
@@ -272,7 +287,10 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     // of codes acc is held times 2^-acc_up, a power of the row's own: kLowest while nothing counts
     constexpr int kLowest = -512;
     int acc_up = kLowest;
-    bool odd = false;
+    // whether the tiles are gone through once more, with all that is not finite taken out of the
+    // products, and the tiles whose values hold such
+    bool careful = false;
+    int odd_from = INT32_MAX, odd_to = -1;
     // without a condition (a wave without a tile fetches the last one, a lane without keys the
     // cache's first page), so that the queries' wait is not for these as well
     Where cur = where(min(ti, last - 1)), next{};
@@ -304,6 +322,7 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 v2f v = {x[s][2 * i], x[s][2 * i + 1]};
+                if constexpr (K::qp == 1) v += v - v;  // an infinity is NaN, as its second plane is
                 if constexpr (SCALED) v = v2f{ldexpf(v[0], up), ldexpf(v[1], up)};
 #pragma unroll
                 for (int pl = 0; pl < K::qp; pl++) q[pl][s][i] = plane(E(), v);
@@ -326,6 +345,26 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
                     if ((s * 64 + 16 * g) / (int)sizeof(C) >= dim) key[t][s] = v4u{0, 0, 0, 0};
         }
         v4f score[2] = {};
+        // A key's infinity times the planes of a query would be NaN where they differ in sign or end
+        // in zeros: it counts once, by the query's sign.
+        if constexpr (!CODES && K::qp > 1)
+            if (careful) {
+#pragma unroll
+                for (int s = 0; s < STEPS; s++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        v4u bad, sign;
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            const uint32_t mask = not_finite(E(), key[t][s][w]);
+                            bad[w] = key[t][s][w] & mask;
+                            key[t][s][w] &= ~mask;
+                            sign[w] = signs(HALF ? 0x3c00u : 0x3f80u, q[0][s][w]);
+                        }
+                        score[t] = product(E(), bad, sign, score[t]);
+                    }
+                settle(score[0], score[1]);
+            }
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
 #pragma unroll
@@ -381,33 +420,24 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
             l += x[i];
         }
 
-        // Where some rows of the wave see a key and others do not, its values that are not finite
-        // count as zeros: zero times them is not zero.  The rows that do see them get them
-        // after the loop.  (Of codes only the scale may be so, which each row has as its own.)
+        // Values that are not finite count as zeros, and are added to the rows that see them after
+        // the loop: zero times them is not zero, nor is a plane of a weight.  (Of codes only the
+        // scale may be so, which each row has as its own.)
         if constexpr (!CODES)
-            if (lo < hi && (ti + 1) * kKeyTile > lo) {
-                // an exponent of ones carries into the sign's place
-                constexpr uint32_t exponent = HALF ? 0x7c007c00u : 0x7f807f80u, one = HALF ? 0x04000400u : 0x00800080u;
-                uint32_t carried = 0;
+            if (careful) {
+                uint32_t any = 0;
 #pragma unroll
                 for (int i = 0; i < 8; i++)
 #pragma unroll
                     for (int h = 0; h < G::H; h++)
 #pragma unroll
-                        for (int w = 0; w < G::VW; w++) carried |= (val[i][h][w] & exponent) + one;
-                if (__any(carried & 0x80008000u)) {
-                    odd = true;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        if (ti * kKeyTile + 16 * (i / 4) + 4 * g + i % 4 < lo) continue;
-#pragma unroll
-                        for (int h = 0; h < G::H; h++)
-#pragma unroll
-                            for (int w = 0; w < G::VW; w++) {
-                                const uint32_t bad = ((val[i][h][w] & exponent) + one) & 0x80008000u;
-                                val[i][h][w] &= (bad & 0x8000u ? 0u : 0xffffu) | (bad >> 31 ? 0u : 0xffff0000u);
-                            }
-                    }
+                        for (int w = 0; w < G::VW; w++) {
+                            any |= carried(E(), val[i][h][w]);
+                            val[i][h][w] &= ~not_finite(E(), val[i][h][w]);
+                        }
+                if (__any(any & 0x80008000u)) {
+                    odd_from = min(odd_from, ti);
+                    odd_to = ti;
                 }
             }
         if constexpr (CODES) {
@@ -476,15 +506,35 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
             }
         if constexpr (more.value) fetch_values(next);
     };
-    for (; ti + kw_all < end; ti += kw_all, cur = next) step(std::true_type{});
-    if (ti < end) step(std::false_type{});
-    settle(acc);
+    while (true) {
+        for (; ti + kw_all < end; ti += kw_all, cur = next) step(std::true_type{});
+        if (ti < end) step(std::false_type{});
+        settle(acc);
+        if constexpr (CODES) break;
+        if (careful) break;
+        // not finite: some key or value is not, that a row sees or that met a weight of zero
+        v4f none = acc[0] * 0.0f;
+#pragma unroll
+        for (int i = 1; i < NC; i++) none += acc[i] * 0.0f;
+        const float sum = (none[0] + none[1]) + (none[2] + none[3]) + l * 0.0f;
+        if (!__any(sum != sum)) break;
+        careful = true;
+        ti = first + kw;
+        page0 = first_page;
+        numbers = table[min(page0 + lane, a.max_pages - 1)];
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; i++) acc[i] = v4f{0, 0, 0, 0};
+        cur = where(min(ti, last - 1));
+        fetch_keys(cur);
+        fetch_values(cur);
+    }
     l = far_sum(l);
     // what was not finite, to the rows that see it
     if constexpr (!CODES)
-        if (odd) {
-            for (int j = max(lo, 0); j < hi; j++) {
-                if (j / kKeyTile < first || (j / kKeyTile - first) % kw_all != kw || j / kKeyTile >= end) continue;
+        for (int tile = odd_from; tile <= odd_to; tile += kw_all)
+            for (int j = tile * kKeyTile; j < min(hi, (tile + 1) * kKeyTile); j++) {
                 const int number = table[j >> shift];
                 if (j >= mine || (uint32_t)number >= (uint32_t)c.n_pages) continue;
                 const int64_t at = ((int64_t)number * c.n_kv_heads + kv) * c.page + (j & (c.page - 1));
@@ -500,7 +550,6 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
                             if (!(fabsf(v) <= 3.4028235e38f)) acc[h * DV + i][r] += v;
                         }
             }
-        }
     // the waves of the same rows joined: each scales its sums to the maximum of all
     if (g == 0) {
         stat[wave][0][n] = m;

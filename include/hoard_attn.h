@@ -40,7 +40,7 @@ extern "C" {
    With HOARD_TYPE_I8 a row of head_dim values is held as codes and one scale
    s = max |x| / 127: code = x / s rounded to nearest, ties to even, value = s * code.
    A row of zeros has the scale 0; one that holds an infinity or a NaN is NaN
-   throughout. */
+   throughout, and a value's scale that is infinite makes as much of it. */
 typedef struct hoard_kv_cache {
     void *k, *v;              /* [n_pages][n_kv_heads][page][head_dim] of `type`, 16-byte aligned */
     float *k_scale, *v_scale; /* [n_pages][n_kv_heads][page] with HOARD_TYPE_I8, 16-byte aligned; else NULL */
@@ -133,7 +133,12 @@ int hoard_heads_workspace(const hoard_heads_args *a, size_t *bytes);
    held to 2^-16 of each (2^-22 for fp32 activations) or, over f16 and I8 caches, to 2^-37
    of the row's largest, whichever is more; with I8 a weight's product with its value's
    scale is held so, by the keys that the row sees.  A weight below 2^-126 may count as
-   none.  1 <= n_new <= 64,
+   none.
+   What a row sees that is not finite counts as in the formula, wherever it lies: a score
+   of -infinity weighs nothing (where all are, the row is as one that sees no key), one
+   of +infinity or NaN makes the row NaN, as a query does that is not finite; an infinity
+   among the values makes its column infinite, NaN beside one of the other sign, and
+   either of these where its weight is too small for 32 bits.  1 <= n_new <= 64,
    n_q_heads a multiple of the cache's n_kv_heads up to 1024, n_seq * n_new < 2^24,
    max_pages * page <= 2^30.
    workspace: hoard_attn_workspace's bytes (possibly 0), 16-byte aligned, used by the
