@@ -147,7 +147,7 @@ __device__ __forceinline__ void rotate(int rope, const Place &p, const Turn &t, 
     for (int j = 0; j < 4; j++) {
         const float s = back ? -t.s[j] : t.s[j];
         float &x = rope == HOARD_ROPE_HALVES ? v[j] : v[2 * j], &y = rope == HOARD_ROPE_HALVES ? v[4 + j] : v[2 * j + 1];
-        const float nx = x * t.c[j] - y * s, ny = y * t.c[j] + x * s;
+        const float nx = fmaf(x, t.c[j], -(y * s)), ny = fmaf(y, t.c[j], x * s);
         x = nx;
         y = ny;
     }
