@@ -190,8 +190,8 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     typedef typename K::E E;
     constexpr bool CODES = sizeof(C) == 1, HALF = __is_same(E, f16), SCALED = HALF && !__is_same(T, f16);
     constexpr int DV = G::DV, NC = G::NC, STEPS = G::STEPS;
-    // f16 weights reach from 2^15 down
-    constexpr float kLift = HALF ? 15.0f : 0.0f;
+    // f16 weights reach from 2^15 down (those of codes by their own power)
+    constexpr float kLift = HALF && !CODES ? 32768.0f : 1.0f;
     __shared__ float stat[kAttnWaves][2][16];
     __shared__ v4f outs[kAttnWaves][16][16 * DV / 4 + 1];
 
@@ -413,7 +413,7 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
                 for (int i = 0; i < NC; i++) acc[i] *= f;
             }
         }
-        const float base = (m > -INFINITY ? m : 0.0f) - kLift;
+        const float base = m > -INFINITY ? m : 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             x[i] = exp2_of(x[i] - base);
@@ -479,7 +479,8 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
         v4u weight[K::pp];
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            v2f v = {x[2 * w], x[2 * w + 1]};
+            // lifted here, not in the exponent, which would lose digits and, from 2^24 on, the lift
+            v2f v = {x[2 * w] * kLift, x[2 * w + 1] * kLift};
 #pragma unroll
             for (int pl = 0; pl < K::pp; pl++) weight[pl][w] = plane(E(), v);
         }
@@ -561,12 +562,11 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     const float base = top > -INFINITY ? top : 0.0f;
     for (int w = 0; w < kw_all; w++) total += exp2_of(stat[w * p.row_waves + rw][0][n] - base) * stat[w * p.row_waves + rw][1][n];
     // of codes the maxima are whole numbers, and the step between them goes with acc's power
-    const float f = total == 0.0f ? 0.0f : CODES ? 1.0f / total : exp2_of(m - base) / total;
+    const float f = total == 0.0f ? 0.0f : CODES ? 1.0f / total : exp2_of(m - base) / total * (1.0f / kLift);
     const int out_up = CODES ? acc_up + kCodeShift + (int)fmaxf(m - base, -2048.0f) : 0;
     if (kw == 0 && g == 0 && row0 + n < rows) {
         const int64_t out = ((int64_t)seq * a.n_new + row / group) * a.n_q_heads + kv * group + row % group;
-        // the lift leaves before the logarithm, whose digits would be spent on it
-        const float log2_sum = base + log2f(total * (HALF ? 1.0f / 32768.0f : 1.0f));
+        const float log2_sum = base + log2f(total);
         if (part >= 0) p.part_lse[part * p.block_rows + rw * 16 + n] = log2_sum;
         else if (a.lse) a.lse[out] = log2_sum * 0.6931471805599453f;
     }
