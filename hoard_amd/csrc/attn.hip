@@ -9,6 +9,7 @@ namespace hoard {
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 
 // A wave joins a row where there are many of them, of few parts each (64 sequences by 32 heads, two
 // parts: 4.9 us, a workgroup a row 7.3; 80 tokens by 16 heads, 9 parts: 7.3 and 5.7).
@@ -32,8 +33,9 @@ __device__ __forceinline__ RowParts row_parts(const AttnCall &p, int token, int 
                     (from_run + (own ? 0 : (int64_t)seq * lanes + of)) * p.block_rows + row % p.block_rows};
 }
 
-// out = sum_s w_s part_s,  w_s = 2^(lse_s - m) / sum: the parts of one row, each already
-// divided by its own sum.
+// out = sum_s w_s part_s,  w_s = l_s 2^(m_s - m) / sum: the parts of one row, each already
+// divided by its own sum l_s of weights, formed by its own largest score m_s.  (Not by the logarithm
+// of the two: far from zero it would have no digits left for the sum.)
 //
 // A workgroup takes a row: four columns a thread, the parts dealt to the threads left over,
 // which meet in LDS.  What a thread reads first it asks for before the weights are known: the
@@ -47,19 +49,20 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall p) {
     const RowParts row = row_parts(p, token, head);
     if (row.parts == 1) return;
     const int lane = threadIdx.x & 63, dim = p.c.head_dim;
-    const float mine = (int)threadIdx.x < row.parts ? p.part_lse[row.first + (int64_t)threadIdx.x * row.step] : -INFINITY;
+    const v2f none = {-INFINITY, 0.0f};
+    const v2f mine = (int)threadIdx.x < row.parts ? reinterpret_cast<const v2f *>(p.part_stat)[row.first + (int64_t)threadIdx.x * row.step] : none;
     const int quads = dim / 4, deep = 256 / quads, quad = threadIdx.x % quads, from = threadIdx.x / quads;
     const float *part = p.part_out + row.first * dim + 4 * quad;
     v4f ahead[kFetch];
 #pragma unroll
     for (int i = 0; i < kFetch; i++)
         ahead[i] = *reinterpret_cast<const v4f *>(part + (int64_t)min(from + i * deep, row.parts - 1) * row.step * dim);
-    const float top = wave_max_f(mine);
+    const float top = wave_max_f(mine[0]);
     if (lane == 0) stat[0][wave_index()] = top;
     __syncthreads();
     float m = fmaxf(fmaxf(stat[0][0], stat[0][1]), fmaxf(stat[0][2], stat[0][3]));
     m = m > -INFINITY ? m : 0.0f;
-    const float w = exp2f(mine - m), s = wave_sum_f(w);  // a NaN is everyone's
+    const float w = exp2f(mine[0] - m) * mine[1], s = wave_sum_f(w);  // a NaN is everyone's
     if (lane == 0) stat[1][wave_index()] = s;
     weight[threadIdx.x] = w;
     __syncthreads();
@@ -95,18 +98,20 @@ __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnCall p) {
     const int lane = threadIdx.x & 63, dim = p.c.head_dim, quad = min(lane, dim / 4 - 1);
     const float *part = p.part_out + row.first * dim + 4 * quad;
     const v4f first = *reinterpret_cast<const v4f *>(part), second = *reinterpret_cast<const v4f *>(part + (int64_t)row.step * dim);
-    float lse[kRuns / 64], m = -INFINITY, sum = 0.0f;
+    const v2f none = {-INFINITY, 0.0f};
+    v2f stat[kRuns / 64];
+    float m = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kRuns / 64; i++) {
-        lse[i] = i * 64 + lane < row.parts ? p.part_lse[row.first + (int64_t)(i * 64 + lane) * row.step] : -INFINITY;
-        m = fmaxf(m, lse[i]);
+        stat[i] = i * 64 + lane < row.parts ? reinterpret_cast<const v2f *>(p.part_stat)[row.first + (int64_t)(i * 64 + lane) * row.step] : none;
+        m = fmaxf(m, stat[i][0]);
     }
     m = wave_max_f(m);
     m = m > -INFINITY ? m : 0.0f;
     v4f o = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < kRuns / 64; i++) {
-        const float w = exp2f(lse[i] - m);
+        const float w = exp2f(stat[i][0] - m) * stat[i][1];
         sum += w;
 #pragma unroll 4
         for (int j = 0; j < min(row.parts - i * 64, 64); j++) {
@@ -154,8 +159,8 @@ AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work)
     p.split = attn_lanes(p) < 2 * kRuns && a.n_seq <= kMaxSplitSeqs && tiles_most > kWholeTiles && attn_lanes(p) * tiles_most < 1 << 28;
     if (p.split) {
         p.part_out = work;
-        p.part_lse = work ? work + attn_parts(p) * p.block_rows * c.head_dim : nullptr;
-        p.sums = work ? reinterpret_cast<int32_t *>(p.part_lse + attn_parts(p) * p.block_rows) : nullptr;
+        p.part_stat = work ? work + attn_parts(p) * p.block_rows * c.head_dim : nullptr;
+        p.sums = work ? reinterpret_cast<int32_t *>(p.part_stat + 2 * attn_parts(p) * p.block_rows) : nullptr;
     }
     return p;
 }
@@ -166,7 +171,7 @@ constexpr int64_t kMaxGrid = 1 << 23;
 
 size_t attn_work_bytes(const hoard_kv_cache &c, const hoard_attn_args &a) {
     const AttnCall p = call_of(c, a, nullptr);
-    return p.split ? sizeof(float) * ((size_t)(c.head_dim + 1) * attn_parts(p) * p.block_rows + a.n_seq + 2) : 0;
+    return p.split ? sizeof(float) * ((size_t)(c.head_dim + 2) * attn_parts(p) * p.block_rows + a.n_seq + 2) : 0;
 }
 
 hipError_t launch_attn(const hoard_kv_cache &c, const hoard_attn_args &a, float *work, hipStream_t s) {

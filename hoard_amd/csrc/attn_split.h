@@ -46,7 +46,8 @@ struct AttnCall {
     int row_blocks;  // workgroups over the rows
     int block_rows;  // rows of a workgroup
     int min_run;     // tiles of a run, at least: one a wave
-    float *part_out, *part_lse;  // [parts][block_rows][head_dim] and [parts][block_rows], with split
+    float *part_out, *part_stat;  // [parts][block_rows][head_dim], and [parts][block_rows] of the largest score
+                                  // and the weights' sum by it, with split
     int32_t *sums;   // [n_seq + 2]: tiles of all lanes of the sequences up to each, a run's, whether
                      // runs hold one lane's tiles only; with split
 };
@@ -153,6 +154,6 @@ hipError_t launch_attn_i8(const AttnCall &p, hipStream_t s);
 // Lanes of work, workgroups of the tiles' kernel, and parts in the workspace.
 inline int64_t attn_lanes(const AttnCall &p) { return (int64_t)p.a.n_seq * p.c.n_kv_heads * p.row_blocks; }
 inline int attn_grid(const AttnCall &p) { return (int)attn_lanes(p) + (p.split ? kRuns : 0); }
-inline int64_t attn_parts(const AttnCall &p) { return p.split ? kRuns + attn_lanes(p) : 0; }
+inline int64_t attn_parts(const AttnCall &p) { return p.split ? kRuns - 1 + attn_lanes(p) : 0; }
 
 }  // namespace hoard

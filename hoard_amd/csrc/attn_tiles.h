@@ -566,9 +566,8 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
     const int out_up = CODES ? acc_up + kCodeShift + (int)fmaxf(m - base, -2048.0f) : 0;
     if (kw == 0 && g == 0 && row0 + n < rows) {
         const int64_t out = ((int64_t)seq * a.n_new + row / group) * a.n_q_heads + kv * group + row % group;
-        const float log2_sum = base + log2f(total);
-        if (part >= 0) p.part_lse[part * p.block_rows + rw * 16 + n] = log2_sum;
-        else if (a.lse) a.lse[out] = log2_sum * 0.6931471805599453f;
+        if (part >= 0) reinterpret_cast<v2f *>(p.part_stat)[part * p.block_rows + rw * 16 + n] = v2f{top, total};
+        else if (a.lse) a.lse[out] = (base + log2f(total)) * 0.6931471805599453f;
     }
 #pragma unroll
     for (int h = 0; h < G::H; h++) {

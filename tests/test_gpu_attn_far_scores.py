@@ -12,7 +12,7 @@ F32, F16, BF16, I8 = torch.float32, torch.float16, torch.bfloat16, torch.int8
 
 @pytest.mark.parametrize("ct", [F16, BF16, I8])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("n", [240])
+@pytest.mark.parametrize("n", [240, 1300])
 @pytest.mark.parametrize("size", [1.0, 2.0 ** 10, 2.0 ** 16, 2.0 ** 40])
 def test_the_largest_alone(size, n, dtype, ct):
     """Keys whose scores are 0, 16 size, 32 size, .. in turns of 100: the result is the mean of the values of the largest.
