@@ -34,8 +34,9 @@ __device__ __forceinline__ RowParts row_parts(const AttnCall &p, int token, int 
 }
 
 // out = sum_s w_s part_s,  w_s = l_s 2^(m_s - m) / sum: the parts of one row, each already
-// divided by its own sum l_s of weights, formed by its own largest score m_s.  (Not by the logarithm
-// of the two: far from zero it would have no digits left for the sum.)
+// divided by its own sum l_s of weights, formed by its own largest score m_s.  (Not by the
+// logarithm of the two: far from zero it would have no digits left for the sum.)  The weights are
+// divided before they meet the parts, so that no sum is larger than these are.
 //
 // A workgroup takes a row: four columns a thread, the parts dealt to the threads left over,
 // which meet in LDS.  What a thread reads first it asks for before the weights are known: the
@@ -71,10 +72,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall p) {
     if (from < deep) {
 #pragma unroll
         for (int i = 0; i < kFetch; i++)
-            if (from + i * deep < row.parts) o += weight[from + i * deep] * ahead[i];
+            if (from + i * deep < row.parts) o += weight[from + i * deep] * f * ahead[i];
 #pragma unroll 4
         for (int i = from + kFetch * deep; i < row.parts; i += deep)
-            o += weight[i] * *reinterpret_cast<const v4f *>(part + (int64_t)i * row.step * dim);
+            o += weight[i] * f * *reinterpret_cast<const v4f *>(part + (int64_t)i * row.step * dim);
     }
     outs[threadIdx.x] = o;
     __syncthreads();
@@ -83,7 +84,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall p) {
         for (int i = 1; i < deep; i++) o += outs[i * quads + quad];
         T *to = static_cast<T *>(p.a.out) + out * dim + 4 * quad;
 #pragma unroll
-        for (int k = 0; k < 4; k++) to[k] = (T)(o[k] * f);
+        for (int k = 0; k < 4; k++) to[k] = (T)o[k];
     }
     if (threadIdx.x == 0 && p.a.lse) p.a.lse[out] = (m + log2f(sum)) * 0.6931471805599453f;
 }
@@ -108,23 +109,28 @@ __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnCall p) {
     }
     m = wave_max_f(m);
     m = m > -INFINITY ? m : 0.0f;
+    float weight[kRuns / 64];
+#pragma unroll
+    for (int i = 0; i < kRuns / 64; i++) {
+        weight[i] = exp2f(stat[i][0] - m) * stat[i][1];
+        sum += weight[i];
+    }
+    sum = wave_sum_f(sum);
+    const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
     v4f o = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < kRuns / 64; i++) {
-        const float w = exp2f(stat[i][0] - m) * stat[i][1];
-        sum += w;
+        const float w = weight[i] * f;
 #pragma unroll 4
         for (int j = 0; j < min(row.parts - i * 64, 64); j++) {
             const float wj = readlane_f(w, j);
             o += wj * (i == 0 && j < 2 ? (j ? second : first) : *reinterpret_cast<const v4f *>(part + (int64_t)(i * 64 + j) * row.step * dim));
         }
     }
-    sum = wave_sum_f(sum);
-    const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
     if (lane < dim / 4) {
         T *to = static_cast<T *>(p.a.out) + out * dim + 4 * quad;
 #pragma unroll
-        for (int k = 0; k < 4; k++) to[k] = (T)(o[k] * f);
+        for (int k = 0; k < 4; k++) to[k] = (T)o[k];
     }
     if (lane == 0 && p.a.lse) p.a.lse[out] = (m + log2f(sum)) * 0.6931471805599453f;
 }

@@ -39,3 +39,20 @@ def test_the_largest_alone(size, n, dtype, ct):
     # the key as the cache rounds it
     top = float(torch.tensor(scale)) * 128.0 * float(A.values(c.k, c.k_scale)[6, 0, 3, 0])
     assert abs(float(got.lse[0, 0]) - top) <= 8 * A.U32 * top + 3
+
+
+@pytest.mark.parametrize("ct", [BF16, I8])
+@pytest.mark.parametrize("seqs,n", [(1, 6000), (66, 1200), (140, 1200)])
+def test_large_values_in_many_parts(seqs, n, ct):
+    """Values of 1e36 and all keys alike: their mean, of which no sum of parts may be larger than 32 bits hold.  A term a
+    key rounds a few times, each to 2^-15 for its weight."""
+    from hoard_amd import attn
+    c = attn.KVCache.new(n // 16 + 1, 16, 1, 64, ct)
+    x = torch.randn((c.n_pages * 16, 1, 64), generator=torch.Generator().manual_seed(1)).abs()
+    attn.kv_write(c, torch.arange(len(x), dtype=torch.int32, device="cuda"), x.cuda(), 1e36 * x.cuda())
+    pages = torch.arange(c.n_pages, dtype=torch.int32, device="cuda").expand(seqs, -1).contiguous()
+    lens = (n - torch.arange(seqs)).to(torch.int32).cuda()
+    got = attn.attn_decode(torch.zeros((seqs, 8, 64), dtype=BF16, device="cuda"), c, pages, lens).out
+    v = A.values(c.v, c.v_scale).transpose(1, 2).reshape(-1, 64)
+    want = torch.stack([v[:int(m)].mean(0) for m in lens]).unsqueeze(1).expand(seqs, 8, 64)
+    A.close(got, want, A.stored(want, want * (2.0 ** -15 + 2 * n * A.U32), BF16), "out")
