@@ -384,8 +384,9 @@ __device__ __forceinline__ void attn_part(const AttnCall &p, int seq, int lane_n
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             x[i] = score[i / 4][i % 4] * to_log2;
-            if constexpr (CODES) x[i] *= key_scale[i / 4][i % 4];
-            if constexpr (CODES || SCALED) x[i] = ldexpf(x[i], down);
+            // the powers of two meet before the score, whose size they leave 32 bits by
+            if constexpr (CODES) x[i] *= ldexpf(key_scale[i / 4][i % 4], down);
+            else if constexpr (SCALED) x[i] = ldexpf(x[i], down);
         }
         if constexpr (more.value) fetch_keys(next);
         if (!full) {

@@ -133,3 +133,13 @@ def test_scales_of_zero_and_below_the_normal_range():
     check(q, c, pages, lens, 0.125)
     c.v_scale.zero_()
     assert not attn.attn_decode(q, c, pages, lens).out.any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1e-36, 1e-20, 1e20, 1e36])
+def test_queries_and_keys_of_opposite_sizes(size, dtype):
+    """Scores of order 4 of queries and keys each far from one."""
+    c = cache_of(5, 2, 128, 41)
+    c.k_scale /= size
+    q = size * torch.randn((2, 8, 128), generator=gen(42))
+    check(q.to(dtype).cuda(), c, dev([[4, 0, 2, 1, 3]]), dev([[70, 71]]), float(torch.tensor(4.0 / 128 ** 0.5)))
