@@ -193,7 +193,8 @@ def rope_freq(rot_dim: int, base: float, device="cuda"):
 
 def split_heads(qkv, n_q: int, n_kv: int, dim: int):
     """The q, k and v heads of a fused projection's rows [tokens, (n_q + 2 n_kv) * dim], as views."""
-    _need(isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.shape[1] == (n_q + 2 * n_kv) * dim, "qkv: no matrix of that many heads")
+    _need(isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.shape[1] == (n_q + 2 * n_kv) * dim,
+          "qkv: no matrix of that many heads")
     return torch.split(qkv.view(qkv.shape[0], n_q + 2 * n_kv, dim), [n_q, n_kv, n_kv], dim=1)
 
 

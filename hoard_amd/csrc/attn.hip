@@ -147,9 +147,10 @@ void join(const AttnCall &p, hipStream_t s) {
 constexpr int kWholeTiles = 16;
 
 // Waves side by side over the rows where there are more than 16, which so read a tile at about
-// the same time.  (Two tiles of rows a wave, that unpack keys and values once for both, took 30 to
-// 36 us against 27 to 33 for 16 sequences of 3 new tokens by 8 heads, 3000 keys, and spilled in
-// fp32 at 256 columns.)
+// the same time; of three tiles of rows the fourth wave has none.  (Two tiles of rows a wave, that
+// unpack keys and values once for both, took 38.5 us against 47 for 16 new tokens of one sequence
+// over 32768 keys, but 30 to 36 against 27 to 33 for 16 sequences of 3 new tokens by 8 heads, 3000
+// keys, and spilled in fp32 at 256 columns.)
 AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work) {
     AttnCall p{};
     p.c = c;
@@ -159,8 +160,10 @@ AttnCall call_of(const hoard_kv_cache &c, const hoard_attn_args &a, float *work)
     p.row_blocks = (tiles + p.row_waves - 1) / p.row_waves;
     p.min_run = kAttnWaves / p.row_waves;
     p.block_rows = rows < 16 * p.row_waves ? rows : 16 * p.row_waves;
-    // cut where the lanes alone would leave the chip half empty or uneven, and there is something
-    // to cut; the row of tiles, three times (runs behind its end have numbers too), in 32 bits
+    // cut where the lanes alone would leave the chip half empty, and there is something to cut (by
+    // the table's width: how uneven the lengths are only the device knows, so one long sequence
+    // among 512 lanes is not cut: 100000 tokens among 127 sequences of 500 by 4 key heads 752 us, 62
+    // among 126); the row of tiles, three times (runs behind its end have numbers too), in 32 bits
     const int64_t tiles_most = ((int64_t)a.max_pages * c.page + kKeyTile - 1) / kKeyTile;
     p.split = attn_lanes(p) < 2 * kRuns && a.n_seq <= kMaxSplitSeqs && tiles_most > kWholeTiles && attn_lanes(p) * tiles_most < 1 << 28;
     if (p.split) {

@@ -16,9 +16,9 @@
 // tile's are used, so that half a tile or more is in flight all the time.
 //
 // Bound by memory from some 10 MB on: 131071 tokens of 8-bit codes by 4 key heads of 128 (138
-// MB) take 29 us, 4.8 TB/s, and 4.6 for the join; 8 x 2048 tokens by 16 key heads in f16 (134 MB)
-// 30 (27.5 at best, 4.9 TB/s); below, by the latencies one after the other (lengths, pages and queries, keys,
-// joining the waves: 4 us) and a tile's 1 us a wave: 257 tokens 7.2 us.  A load of keys takes 64
+// MB) take 29 us, 4.8 TB/s, and 4.8 for the join; 8 x 2048 tokens by 16 key heads in f16 (134 MB)
+// 31 (28.2 at best, 4.8 TB/s); below, by the latencies one after the other (lengths, pages and queries, keys,
+// joining the waves: 4 us) and a tile's 1 us a wave: 257 tokens 7.4 us.  A load of keys takes 64
 // bytes of each of 16 rows: one CU reads 16-bit caches at 62 bytes a ns so (138 in whole rows),
 // three times what it gets where all of them read.
 //
